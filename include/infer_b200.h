@@ -87,6 +87,32 @@ INFER_API int infer_kv_append(const infer_kv_pool_t* pool, const void* k, const 
                     int64_t n_tokens, void* workspace, size_t workspace_bytes, void* stream);
 INFER_API size_t infer_kv_append_workspace_bytes(const infer_kv_pool_t* pool);
 
+/* Rows of the pools read back as bf16, the inverse of infer_kv_append: row i of k_out and v_out ([n_tokens,
+ * n_kv_heads, 128] bf16, row pitches in ELEMENTS) is the row in flat slot slot_mapping[i]; e4m3 pools give
+ * bf16(byte * scale of its page and head), the product taken in fp32 and rounded once.  A slot outside the pool
+ * (negative: padding) gives a row of zeros; the same slot may be asked for more than once.  Capturable, no scratch. */
+INFER_API int infer_kv_load(const infer_kv_pool_t* pool, void* k_out, void* v_out, int64_t k_row_stride,
+                    int64_t v_row_stride, const int32_t* slot_mapping, int64_t n_tokens, void* stream);
+
+/* Rotary positions of q and k + KV append in one pass, bf16 pools.  The first rot_dim dims of every head (a multiple
+ * of 16, at most 128) are rotated in pairs by the angle positions[t] * inv_freq[pair]: pairs (i, i + rot_dim / 2), or
+ * (2i, 2i + 1) with interleaved != 0; the dims behind rot_dim are copied.  inv_freq: double [rot_dim / 2] on the
+ * device, radians per position (context scaling is a matter of its values); the angle is reduced in 64 bits, so any
+ * position below 2^52 keeps its digits.  cosine and sine are multiplied by factor.  q, k, v: bf16 [n_tokens, heads, 128]
+ * with free row strides (ELEMENTS); q_out may be q itself.  k goes rotated and v unchanged to slot slot_mapping[t];
+ * slots outside the pool are skipped (q_out is written all the same).  The rotation runs in fp32 and rounds once. */
+INFER_API int infer_rotary_append(const infer_kv_pool_t* pool, void* q_out, int64_t q_out_row_stride, const void* q,
+                        const void* k, const void* v, int64_t q_row_stride, int64_t k_row_stride, int64_t v_row_stride,
+                        const int64_t* positions, const double* inv_freq, int rot_dim, int interleaved, float factor,
+                        const int32_t* slot_mapping, int64_t n_tokens, int n_q_heads, void* stream);
+
+/* The same rotation without a pool: k_out [n_tokens, n_kv_heads, 128] receives the rotated k (for an e4m3 pool,
+ * infer_kv_append quantises these rows).  q_out may be q and k_out may be k. */
+INFER_API int infer_rotary_embed(void* q_out, void* k_out, int64_t q_out_row_stride, int64_t k_out_row_stride, const void* q,
+                       const void* k, int64_t q_row_stride, int64_t k_row_stride, const int64_t* positions,
+                       const double* inv_freq, int rot_dim, int interleaved, float factor, int64_t n_tokens, int n_q_heads,
+                       int n_kv_heads, void* stream);
+
 /* Fused per-head RMSNorm + rotary embedding + KV append: one pass over the fused qkv rows
  * instead of the four the reference model makes before attention (q_norm and k_norm,
  * infer/models/Qwen3.py:116-121 with infer/ops/norm.py:63-73; the in-place rotary embedding of
@@ -152,6 +178,19 @@ INFER_API int infer_paged_decode_append(const infer_kv_pool_t* pool, void* out, 
                               const int32_t* context_lens, const int32_t* block_tables, int64_t bt_stride,
                               int batch, int n_q_heads, float softmax_scale, void* workspace,
                               size_t workspace_bytes, void* stream);
+/* infer_paged_decode and infer_paged_decode_append for a layer whose queries see a sliding window: of the keys
+ * 0 .. context_lens[b] - 1 of a sequence the last `window` (the query's own among them; >= 1) and the first `sinks`
+ * (>= 0).  Block-table entries of pages without a visible key are not read, so such pages may have been given back.
+ * softmax_scale has to be a positive finite number.  Everything else as above, e4m3 pools included where they are. */
+INFER_API int infer_paged_decode_window(const infer_kv_pool_t* pool, void* out, const void* q,
+                              const int32_t* context_lens, const int32_t* block_tables, int64_t bt_stride, int batch,
+                              int n_q_heads, float softmax_scale, int window, int sinks, void* workspace,
+                              size_t workspace_bytes, void* stream);
+INFER_API int infer_paged_decode_append_window(const infer_kv_pool_t* pool, void* out, const void* q, const void* k,
+                              const void* v, int64_t k_row_stride, int64_t v_row_stride, const int32_t* context_lens,
+                              const int32_t* block_tables, int64_t bt_stride, int batch, int n_q_heads,
+                              float softmax_scale, int window, int sinks, void* workspace, size_t workspace_bytes,
+                              void* stream);
 INFER_API size_t infer_paged_decode_workspace_bytes(const infer_kv_pool_t* pool, int batch, int n_q_heads);
 
 /* Paged chunked-prefill attention.  Replaces the prefill branch

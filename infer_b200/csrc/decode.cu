@@ -96,9 +96,38 @@ struct TailMaps {
 };
 static_assert(TmaSmem::patch % 16 == 0, "the staging rows are written by 16-byte asynchronous copies");
 
+// The smallest box of 16, 32, 64 or 128 token rows that covers rows [r0, r1) of a tile of tile_rows rows, as its place in
+// the tile: rows [row, row + (16 << box)).  box = -1: the whole tile.
+struct TileBox {
+    int box, row;
+};
+__device__ __forceinline__ TileBox tile_box(int r0, int r1, int tile_rows) {
+    TileBox b = {-1, 0};
+#pragma unroll
+    for (int i = kTailMaps - 1; i >= 0; --i) {
+        const int size = 16 << i, row = min(r0 & ~15, tile_rows - size);
+        if (size < tile_rows && row + size >= r1) {
+            b.box = i;
+            b.row = row;
+        }
+    }
+    return b;
+}
+// Rows of tile `tile` between its first and its last visible key.
+__device__ __forceinline__ TileBox window_box(const WindowTiles& w, int len, int tile, int tile_rows) {
+    const int tok0 = tile * tile_rows;
+    const int lo = max(w.start - tok0, 0), hi = min(len - tok0, tile_rows);      // the window's part, empty if lo >= hi
+    const int sink = min(w.sinks - tok0, tile_rows);                              // the first keys' part is [0, sink)
+    return tile_box(sink > 0 ? 0 : lo, lo < hi ? hi : sink, tile_rows);
+}
+
 __device__ __forceinline__ void consumer_bar() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
-template <int HPC>
+// WINDOW: only the last p.window and the first p.sinks keys of a sequence are visible.  Tiles without a visible key are
+// not in the numbering at all (their pages may be gone from the block table), and of a tile that is partly visible the
+// smallest box that covers its visible rows is copied; without that, a window of 1024 keys behind an unaligned start
+// would read up to 127 rows too many, and 4 sink tokens 128.
+template <int HPC, bool WINDOW>
 __global__ void __launch_bounds__(kTmaThreads, 1) decode_tma_kernel(DecodeParams p,
                                                                     const __grid_constant__ CUtensorMap map_k,
                                                                     const __grid_constant__ CUtensorMap map_v,
@@ -131,7 +160,8 @@ __global__ void __launch_bounds__(kTmaThreads, 1) decode_tma_kernel(DecodeParams
     // launches never share an SM - each takes nearly all of its shared memory - so nothing is lost.)
     if (p.new_k != nullptr) pdl_wait();
     uint8_t* s_rem = smem + TmaSmem::rem;
-    build_tile_prefix(p.context_lens, p.batch, TT, s_tp, s_scan, s_rem, p.seg_overhead);   // ends with __syncthreads
+    build_tile_prefix<WINDOW>(p.context_lens, p.batch, TT, s_tp, s_scan, s_rem, p.seg_overhead, p.window,
+                              p.sinks);                                    // ends with __syncthreads
     // Everything above only reads step metadata; the pools and q may still be written by the
     // kernel in front of this one (the append) when this kernel was launched programmatically.
     pdl_launch_dependents();
@@ -152,10 +182,17 @@ __global__ void __launch_bounds__(kTmaThreads, 1) decode_tma_kernel(DecodeParams
         for (int g = lo; g < hi && ok;) {
             const Segment sg = locate_segment(s_tp, p.batch, ng, g, hi, p.seg_overhead);
             const int32_t* table = p.block_tables + int64_t(sg.b) * p.bt_stride;
+            int ctx = 0;
+            WindowTiles win;
+            if constexpr (WINDOW) {
+                ctx = p.context_lens[sg.b];
+                win = window_tiles(ctx, TT, p.window, p.sinks);
+            }
             for (int t = sg.t0; t < sg.t1; ++t, ++it) {
                 const uint32_t s = it % kStages, ph = (it / kStages) & 1;
                 if (!mbar_wait(empty0 + s * 8, ph ^ 1, p.wait_limit)) { ok = false; break; }
-                const int tok0 = t * TT;
+                const int tile = WINDOW ? tile_of(win, t) : t;
+                const int tok0 = tile * TT;
                 const int page = table[tok0 / p.block_size];
                 const int slot0 = page * p.block_size + tok0 % p.block_size;
                 const uint32_t bar = full0 + s * 8;
@@ -167,7 +204,18 @@ __global__ void __launch_bounds__(kTmaThreads, 1) decode_tma_kernel(DecodeParams
                 const CUtensorMap* mk = &map_k;
                 const CUtensorMap* mv = &map_v;
                 uint32_t bytes = 2 * kTileBytes;
-                if (t == sg.ntiles - 1) {
+                int row = 0;                              // first row of the tile that is copied
+                if constexpr (WINDOW) {
+                    const TileBox box = window_box(win, ctx, tile, TT);
+#pragma unroll
+                    for (int i = 0; i < kTailMaps; ++i)
+                        if (box.box == i) {
+                            mk = &tails.k[i];
+                            mv = &tails.v[i];
+                            bytes = 4 * HPC * (16 << i) * 128;
+                            row = box.row;
+                        }
+                } else if (t == sg.ntiles - 1) {
                     const int rem = s_rem[sg.b];
 #pragma unroll
                     for (int i = kTailMaps - 1; i >= 0; --i)
@@ -183,8 +231,8 @@ __global__ void __launch_bounds__(kTmaThreads, 1) decode_tma_kernel(DecodeParams
                     const int head = sg.hg * HPC + hl;
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
-                        tma_load_3d(kdst + (hl * 2 + half) * SUB, mk, bar, half * 64, head, slot0);
-                        tma_load_3d(vdst + (hl * 2 + half) * SUB, mv, bar, half * 64, head, slot0);
+                        tma_load_3d(kdst + (hl * 2 + half) * SUB + row * 128, mk, bar, half * 64, head, slot0 + row);
+                        tma_load_3d(vdst + (hl * 2 + half) * SUB + row * 128, mv, bar, half * 64, head, slot0 + row);
                     }
                 }
             }
@@ -216,6 +264,8 @@ __global__ void __launch_bounds__(kTmaThreads, 1) decode_tma_kernel(DecodeParams
             continue;
         }
         const int ctx = p.context_lens[sg.b];
+        WindowTiles win;
+        if constexpr (WINDOW) win = window_tiles(ctx, TT, p.window, p.sinks);
         const int head = sg.hg * HPC + hl;
         // Query fragments: rows 0..group-1 of the 16-row A operand, zero elsewhere.
         uint32_t qa[8][2];
@@ -254,9 +304,13 @@ __global__ void __launch_bounds__(kTmaThreads, 1) decode_tma_kernel(DecodeParams
         for (int t = sg.t0; t < sg.t1; ++t, ++it) {
             const uint32_t s = it % kStages, ph = (it / kStages) & 1;
             if (ok && !mbar_wait(full0 + s * 8, ph, p.wait_limit)) ok = false;
-            const int tok_w = t * TT + tw * 16;            // first token of this warp's 16
+            const int tok_w = (WINDOW ? tile_of(win, t) : t) * TT + tw * 16;   // first token of this warp's 16
             const int valid = ctx - tok_w;                  // tokens of the 16 that exist
-            if (ok && valid > 0) {
+            auto seen = [&](int i) { return WINDOW ? key_visible(win, ctx, tok_w + i) : i < valid; };
+            // some of the 16 are visible / not all of them are
+            auto some = [&] { return valid > 0 && (!WINDOW || tok_w + 16 > win.start || tok_w < win.sinks); };
+            auto partly = [&] { return valid < 16 || (WINDOW && tok_w < win.start && tok_w + 16 > win.sinks); };
+            if (ok && some()) {
                 const uint32_t kbase = tiles_u32 + s * (2 * kTileBytes) + (hl * 2) * SUB;
                 const uint32_t vbase = kbase + kTileBytes;
                 if (appends && t == sg.ntiles - 1 && ((ctx - 1) % TT) / 16 == tw) {
@@ -285,11 +339,11 @@ __global__ void __launch_bounds__(kTmaThreads, 1) decode_tma_kernel(DecodeParams
                     mma_bf16(sc[0], qa[kk][0], 0u, qa[kk][1], 0u, b00, b01);
                     mma_bf16(sc[1], qa[kk][0], 0u, qa[kk][1], 0u, b10, b11);
                 }
-                if (valid < 16) {
+                if (partly()) {
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        if (j * 8 + 2 * tig >= valid) sc[j][0] = -INFINITY;
-                        if (j * 8 + 2 * tig + 1 >= valid) sc[j][1] = -INFINITY;
+                        if (!seen(j * 8 + 2 * tig)) sc[j][0] = -INFINITY;
+                        if (!seen(j * 8 + 2 * tig + 1)) sc[j][1] = -INFINITY;
                     }
                 }
                 float mx = fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[1][0], sc[1][1]));
@@ -312,10 +366,10 @@ __global__ void __launch_bounds__(kTmaThreads, 1) decode_tma_kernel(DecodeParams
                     const int chunk16 = (n2 & 3) * 2 + (mi >> 1);
                     uint32_t v0, v1, v2, v3;
                     ldsm_x4_trans(vbase + (n2 >> 2) * SUB + swz128(row, chunk16), v0, v1, v2, v3);
-                    if (valid < 16) {
-                        // rows past the context may hold anything (0 * NaN): clear them
-                        const uint32_t keep_lo = (2 * tig < valid ? 0x0000ffffu : 0u) | (2 * tig + 1 < valid ? 0xffff0000u : 0u);
-                        const uint32_t keep_hi = (8 + 2 * tig < valid ? 0x0000ffffu : 0u) | (9 + 2 * tig < valid ? 0xffff0000u : 0u);
+                    if (partly()) {
+                        // rows past the context (or outside of the window) may hold anything (0 * NaN): clear them
+                        const uint32_t keep_lo = (seen(2 * tig) ? 0x0000ffffu : 0u) | (seen(2 * tig + 1) ? 0xffff0000u : 0u);
+                        const uint32_t keep_hi = (seen(8 + 2 * tig) ? 0x0000ffffu : 0u) | (seen(9 + 2 * tig) ? 0xffff0000u : 0u);
                         v0 &= keep_lo; v2 &= keep_lo;
                         v1 &= keep_hi; v3 &= keep_hi;
                     }
@@ -435,7 +489,7 @@ struct Fp8Smem {
     static constexpr int total = rem + kMaxBatch;
 };
 
-template <int HPC>
+template <int HPC, bool WINDOW>
 __global__ void __launch_bounds__(kTmaThreads, 1) decode_tma_fp8_kernel(DecodeParams p,
                                                                           const __grid_constant__ CUtensorMap map_k,
                                                                           const __grid_constant__ CUtensorMap map_v,
@@ -470,7 +524,7 @@ __global__ void __launch_bounds__(kTmaThreads, 1) decode_tma_fp8_kernel(DecodePa
         fence_proxy_async();
     }
     uint8_t* s_rem = smem + L::rem;
-    build_tile_prefix(p.context_lens, p.batch, TT, s_tp, s_scan, s_rem, p.seg_overhead);
+    build_tile_prefix<WINDOW>(p.context_lens, p.batch, TT, s_tp, s_scan, s_rem, p.seg_overhead, p.window, p.sinks);
     pdl_launch_dependents();
     pdl_wait();
 
@@ -489,9 +543,16 @@ __global__ void __launch_bounds__(kTmaThreads, 1) decode_tma_fp8_kernel(DecodePa
         for (int g = lo; g < hi && ok;) {
             const Segment sg = locate_segment(s_tp, p.batch, ng, g, hi, p.seg_overhead);
             const int32_t* table = p.block_tables + int64_t(sg.b) * p.bt_stride;
+            int ctx = 0;
+            WindowTiles win;
+            if constexpr (WINDOW) {
+                ctx = p.context_lens[sg.b];
+                win = window_tiles(ctx, TT, p.window, p.sinks);
+            }
             for (int t = sg.t0; t < sg.t1; ++t, ++it) {
                 const uint32_t s = it % kStages, ph = (it / kStages) & 1;
-                const int tok0 = t * TT;
+                const int tile = WINDOW ? tile_of(win, t) : t;
+                const int tok0 = tile * TT;
                 const int page = table[tok0 / p.block_size];
                 const int slot0 = page * p.block_size + tok0 % p.block_size;
                 const bool page_ok = page >= 0 && page < p.num_blocks;
@@ -514,7 +575,18 @@ __global__ void __launch_bounds__(kTmaThreads, 1) decode_tma_fp8_kernel(DecodePa
                 const CUtensorMap* mk = &map_k;
                 const CUtensorMap* mv = &map_v;
                 uint32_t bytes = 2 * kTileBytes;
-                if (t == sg.ntiles - 1) {
+                int row = 0;
+                if constexpr (WINDOW) {
+                    const TileBox box = window_box(win, ctx, tile, TT);
+#pragma unroll
+                    for (int i = 0; i < kTailMaps; ++i)
+                        if (box.box == i) {
+                            mk = &tails.k[i];
+                            mv = &tails.v[i];
+                            bytes = 2 * HPC * (16 << i) * 128;
+                            row = box.row;
+                        }
+                } else if (t == sg.ntiles - 1) {
                     const int rem = s_rem[sg.b];
 #pragma unroll
                     for (int i = kTailMaps - 1; i >= 0; --i)
@@ -527,8 +599,8 @@ __global__ void __launch_bounds__(kTmaThreads, 1) decode_tma_fp8_kernel(DecodePa
                 mbar_expect_tx(bar, bytes);               // release: the scales above are visible to the waiters
 #pragma unroll
                 for (int hl = 0; hl < HPC; ++hl) {        // the heads' boxes back to back: adjacent lines of every token row
-                    tma_load_3d(kdst + hl * kHeadBytes, mk, bar, 0, sg.hg * HPC + hl, slot0);
-                    tma_load_3d(vdst + hl * kHeadBytes, mv, bar, 0, sg.hg * HPC + hl, slot0);
+                    tma_load_3d(kdst + hl * kHeadBytes + row * 128, mk, bar, 0, sg.hg * HPC + hl, slot0 + row);
+                    tma_load_3d(vdst + hl * kHeadBytes + row * 128, mv, bar, 0, sg.hg * HPC + hl, slot0 + row);
                 }
             }
             g += sg.span;
@@ -561,6 +633,8 @@ __global__ void __launch_bounds__(kTmaThreads, 1) decode_tma_fp8_kernel(DecodePa
             continue;
         }
         const int ctx = p.context_lens[sg.b];
+        WindowTiles win;
+        if constexpr (WINDOW) win = window_tiles(ctx, TT, p.window, p.sinks);
         const int head = sg.hg * HPC + hl;
         // B fragments of Q^T in f16: column gid is query head gid of the group.  MMA k-slots
         // (2t, 2t+1, 2t+8, 2t+9) of a 16-dim chunk carry dims (4t, 4t+1, 4t+2, 4t+3): the order in
@@ -592,8 +666,11 @@ __global__ void __launch_bounds__(kTmaThreads, 1) decode_tma_fp8_kernel(DecodePa
             const float c_k = s_meta[(s * HPC + hl) * 2 + 0] * p.scale_log2;
             const float vs = s_meta[(s * HPC + hl) * 2 + 1];
             const int row0 = tw * TPW;                      // this warp's tokens of the tile
-            const int valid = ctx - (t * TT + row0);
-            if (ok && valid > 0) {
+            const int tok_w = (WINDOW ? tile_of(win, t) : t) * TT + row0;
+            const int valid = ctx - tok_w;
+            auto some = [&] { return valid > 0 && (!WINDOW || tok_w + TPW > win.start || tok_w < win.sinks); };
+            auto seen = [&](int i) { return WINDOW ? key_visible(win, ctx, tok_w + i) : i < valid; };
+            if (ok && some()) {
                 const uint32_t kbase = tiles_u32 + s * (2 * kTileBytes) + hl * kHeadBytes;
                 const uint32_t vbase = kbase + kTileBytes;
                 // S^T: NH 16-token tiles, each with an even-chunk and an odd-chunk accumulator
@@ -623,7 +700,7 @@ __global__ void __launch_bounds__(kTmaThreads, 1) decode_tma_fp8_kernel(DecodePa
                 for (int h = 0; h < NH; ++h)
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
-                        const bool dead = h * 16 + x * 8 + gid >= valid;
+                        const bool dead = WINDOW ? !seen(h * 16 + x * 8 + gid) : h * 16 + x * 8 + gid >= valid;
                         sv[h][x][0] = dead ? -INFINITY : sc[h][0][2 * x] + sc[h][1][2 * x];
                         sv[h][x][1] = dead ? -INFINITY : sc[h][0][2 * x + 1] + sc[h][1][2 * x + 1];
                     }
@@ -674,13 +751,17 @@ __global__ void __launch_bounds__(kTmaThreads, 1) decode_tma_fp8_kernel(DecodePa
                     // 2t 2t+1" into "head gid, tokens 2t 2t+1"
                     const uint32_t pb0 = movmatrix_trans(pp[h][0]), pb1 = movmatrix_trans(pp[h][1]);
                     const int vh = valid - h * 16;          // tokens of this half that exist
+                    auto partly = [&] {
+                        return vh < 16 || (WINDOW && tok_w + h * 16 < win.start && tok_w + h * 16 + 16 > win.sinks);
+                    };
 #pragma unroll
                     for (int c2 = 0; c2 < 4; ++c2) {
                         uint32_t r0, r1, r2, r3;   // (tokens 0-7, chunk 2c2), (8-15, 2c2), (0-7, 2c2+1), (8-15, 2c2+1)
                         ldsm_x4_trans(vbase + swz128(row0 + h * 16 + (mi & 1) * 8 + mr, c2 * 2 + (mi >> 1)), r0, r1, r2, r3);
-                        if (vh < 16) {
-                            const uint32_t keep_lo = (2 * tig < vh ? 0x0000ffffu : 0u) | (2 * tig + 1 < vh ? 0xffff0000u : 0u);
-                            const uint32_t keep_hi = (8 + 2 * tig < vh ? 0x0000ffffu : 0u) | (9 + 2 * tig < vh ? 0xffff0000u : 0u);
+                        if (partly()) {
+                            const int i = h * 16 + 2 * tig;
+                            const uint32_t keep_lo = (seen(i) ? 0x0000ffffu : 0u) | (seen(i + 1) ? 0xffff0000u : 0u);
+                            const uint32_t keep_hi = (seen(i + 8) ? 0x0000ffffu : 0u) | (seen(i + 9) ? 0xffff0000u : 0u);
                             r0 &= keep_lo; r2 &= keep_lo;
                             r1 &= keep_hi; r3 &= keep_hi;
                         }
@@ -818,31 +899,36 @@ static TailMaps tail_maps(const infer_kv_pool* pool) {
     return tails;
 }
 
-template <int HPC>
+template <int HPC, bool WINDOW = false>
 static int launch_bf16(const DecodeParams& p, const infer_kv_pool* pool, int grid, cudaStream_t st) {
     int idx = 0;
     while ((16 << idx) != 128 / HPC) ++idx;
     const TailMaps tails = tail_maps(pool);
-    IB_CUDA(launch_pdl(decode_tma_kernel<HPC>, dim3(grid), dim3(kTmaThreads), TmaSmem::total + 1024, st, p,
+    IB_CUDA(launch_pdl(decode_tma_kernel<HPC, WINDOW>, dim3(grid), dim3(kTmaThreads), TmaSmem::total + 1024, st, p,
                        pool->maps[idx].k, pool->maps[idx].v, tails));
     return INFER_OK;
 }
 
-template <int HPC>
+template <int HPC, bool WINDOW = false>
 static int launch_fp8(const DecodeParams& p, const infer_kv_pool* pool, int grid, cudaStream_t st) {
     int idx = 0;
     while ((16 << idx) != kFp8TileTokens / HPC) ++idx;
-    IB_CUDA(launch_pdl(decode_tma_fp8_kernel<HPC>, dim3(grid), dim3(kTmaThreads), Fp8Smem<HPC>::total + 1024, st, p,
+    IB_CUDA(launch_pdl(decode_tma_fp8_kernel<HPC, WINDOW>, dim3(grid), dim3(kTmaThreads), Fp8Smem<HPC>::total + 1024, st, p,
                        pool->maps[idx].k, pool->maps[idx].v, tail_maps(pool)));
     return INFER_OK;
 }
 
 template <int HPC>
 static cudaError_t allow_smem() {
-    cudaError_t e = cudaFuncSetAttribute(decode_tma_kernel<HPC>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    cudaError_t e = cudaFuncSetAttribute(decode_tma_kernel<HPC, false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          TmaSmem::total + 1024);
     if (e != cudaSuccess) return e;
-    return cudaFuncSetAttribute(decode_tma_fp8_kernel<HPC>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    return cudaFuncSetAttribute(decode_tma_fp8_kernel<HPC, false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                Fp8Smem<HPC>::total + 1024);
+}
+template <int HPC>
+static cudaError_t allow_smem_window_fp8() {
+    return cudaFuncSetAttribute(decode_tma_fp8_kernel<HPC, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                 Fp8Smem<HPC>::total + 1024);
 }
 
@@ -853,6 +939,11 @@ int decode_prepare_device() {
     if (e == cudaSuccess) e = allow_smem<2>();
     if (e == cudaSuccess) e = allow_smem<4>();
     if (e == cudaSuccess) e = allow_smem<8>();
+    if (e == cudaSuccess)
+        e = cudaFuncSetAttribute(decode_tma_kernel<1, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, TmaSmem::total + 1024);
+    if (e == cudaSuccess) e = allow_smem_window_fp8<1>();
+    if (e == cudaSuccess) e = allow_smem_window_fp8<2>();
+    if (e == cudaSuccess) e = allow_smem_window_fp8<4>();
     if (e != cudaSuccess) {
         set_cuda_error(e);
         return INFER_ERR_CUDA;
@@ -873,10 +964,15 @@ struct NewRows {
     int64_t k_stride = 0, v_stride = 0;
 };
 
+// Which keys a query sees: the last `window` of its sequence (0 = all of them) and the first `sinks`.
+struct Window {
+    int window = 0, sinks = 0;
+};
+
 static int paged_decode(const infer_kv_pool_t* pool, void* out, const void* q, const int32_t* context_lens,
                         const int32_t* block_tables, int64_t bt_stride, int batch, int n_q_heads, float softmax_scale,
                         void* workspace, size_t workspace_bytes, cudaStream_t st, int force_hpc, uint32_t wait_limit,
-                        int stall_producer, const NewRows& rows = NewRows()) {
+                        int stall_producer, const NewRows& rows = NewRows(), const Window& win = Window()) {
     if (!pool || !out || !q || !context_lens || !block_tables) return INFER_ERR_NULL;
     if (rows.k || rows.v) {
         if (!rows.k || !rows.v) return INFER_ERR_NULL;
@@ -915,6 +1011,8 @@ static int paged_decode(const infer_kv_pool_t* pool, void* out, const void* q, c
     p.wait_limit = wait_limit;
     p.stall_producer = stall_producer;
     p.seg_overhead = kSegOverheadTiles;
+    p.window = win.window;
+    p.sinks = win.sinks;
     p.new_k = static_cast<const __nv_bfloat16*>(rows.k);
     p.new_v = static_cast<const __nv_bfloat16*>(rows.v);
     p.new_k_stride = rows.k_stride;
@@ -926,7 +1024,13 @@ static int paged_decode(const infer_kv_pool_t* pool, void* out, const void* q, c
     p.ws_o = reinterpret_cast<float*>(ws + lay.o_off);
 
     int rc;
-    if (pool->dtype == INFER_KV_E4M3) {
+    if (win.window > 0) {
+        // the tile shapes that decode_config chooses by itself
+        if (pool->dtype == INFER_KV_BF16) rc = launch_bf16<1, true>(p, pool, cfg.grid, st);
+        else if (cfg.hpc == 4) rc = launch_fp8<4, true>(p, pool, cfg.grid, st);
+        else if (cfg.hpc == 2) rc = launch_fp8<2, true>(p, pool, cfg.grid, st);
+        else rc = launch_fp8<1, true>(p, pool, cfg.grid, st);
+    } else if (pool->dtype == INFER_KV_E4M3) {
         switch (cfg.hpc) {
             case 1: rc = launch_fp8<1>(p, pool, cfg.grid, st); break;
             case 2: rc = launch_fp8<2>(p, pool, cfg.grid, st); break;
@@ -1007,6 +1111,41 @@ int infer_paged_decode_append(const infer_kv_pool_t* pool, void* out, const void
     rows.v_stride = v_row_stride;
     return ib::paged_decode(pool, out, q, context_lens, block_tables, bt_stride, batch, n_q_heads, softmax_scale,
                             workspace, workspace_bytes, static_cast<cudaStream_t>(stream_), 0, ib::kDefaultWaitLimit, 0, rows);
+}
+
+// A window that is not positive, or a scale that is not a positive number (a masked score is -infinity times the scale).
+static bool window_ok(int window, int sinks, float softmax_scale) {
+    return window > 0 && sinks >= 0 && softmax_scale > 0.f && softmax_scale < INFINITY;
+}
+
+int infer_paged_decode_window(const infer_kv_pool_t* pool, void* out, const void* q, const int32_t* context_lens,
+                              const int32_t* block_tables, int64_t bt_stride, int batch, int n_q_heads, float softmax_scale,
+                              int window, int sinks, void* workspace, size_t workspace_bytes, void* stream_) {
+    if (!window_ok(window, sinks, softmax_scale)) return INFER_ERR_GEOMETRY;
+    ib::Window win;
+    win.window = window;
+    win.sinks = sinks;
+    return ib::paged_decode(pool, out, q, context_lens, block_tables, bt_stride, batch, n_q_heads, softmax_scale, workspace,
+                            workspace_bytes, static_cast<cudaStream_t>(stream_), 0, ib::kDefaultWaitLimit, 0, ib::NewRows(), win);
+}
+
+int infer_paged_decode_append_window(const infer_kv_pool_t* pool, void* out, const void* q, const void* k, const void* v,
+                                     int64_t k_row_stride, int64_t v_row_stride, const int32_t* context_lens,
+                                     const int32_t* block_tables, int64_t bt_stride, int batch, int n_q_heads,
+                                     float softmax_scale, int window, int sinks, void* workspace, size_t workspace_bytes,
+                                     void* stream_) {
+    if (!k || !v) return INFER_ERR_NULL;
+    if (!window_ok(window, sinks, softmax_scale)) return INFER_ERR_GEOMETRY;
+    ib::NewRows rows;
+    rows.k = k;
+    rows.v = v;
+    rows.k_stride = k_row_stride;
+    rows.v_stride = v_row_stride;
+    ib::Window win;
+    win.window = window;
+    win.sinks = sinks;
+    return ib::paged_decode(pool, out, q, context_lens, block_tables, bt_stride, batch, n_q_heads, softmax_scale, workspace,
+                            workspace_bytes, static_cast<cudaStream_t>(stream_), 0, ib::kDefaultWaitLimit, 0, rows, win);
 }
 
 int infer_selftest_paged_decode(const infer_kv_pool_t* pool, void* out, const void* q, const int32_t* context_lens,

@@ -47,6 +47,7 @@ struct DecodeParams {
     uint32_t wait_limit;   // polls before a barrier wait gives up
     int stall_producer;    // self-test only: the producer arms no copy, so every wait runs out
     int seg_overhead;      // what starting and finishing a (sequence, head group) costs a CTA, in tiles (see below)
+    int window, sinks;     // windowed kernels only: the last `window` keys and the first `sinks` ones are visible
     // fused append (bf16 pools): the step's new rows [batch][n_kv_heads][128], row b going to position
     // context_lens[b] - 1 of sequence b; null = the pools already hold them
     const __nv_bfloat16* new_k;
@@ -78,20 +79,50 @@ inline DecodeLayout decode_layout(int grid, int rows) {
 
 #ifdef __CUDACC__
 
+// Tiles of a sequence of `len` keys that hold a visible key when the query, its last token, sees the last `window` keys
+// and the first `sinks` ones.  They are numbered 0 .. count - 1 without the gap between the two parts: tile t of the list
+// is tile t of the sequence below `n_sink` and tile t + skip from there on.  Where the parts meet or share a tile, the
+// list is one run from tile 0 (n_sink = skip = 0).
+struct WindowTiles {
+    int start;      // first key of the window
+    int sinks;      // keys of the first part (at most len)
+    int n_sink, skip, count;
+};
+__device__ __forceinline__ WindowTiles window_tiles(int len, int tile_tokens, int window, int sinks) {
+    WindowTiles w;
+    w.start = max(len - window, 0);
+    w.sinks = min(sinks, len);
+    w.n_sink = (w.sinks + tile_tokens - 1) / tile_tokens;
+    const int first = w.start / tile_tokens;
+    w.skip = max(first - w.n_sink, 0);
+    if (w.skip == 0) w.n_sink = 0;
+    w.count = (len + tile_tokens - 1) / tile_tokens - w.skip;
+    return w;
+}
+__device__ __forceinline__ int tile_of(const WindowTiles& w, int t) { return t < w.n_sink ? t : t + w.skip; }
+__device__ __forceinline__ bool key_visible(const WindowTiles& w, int len, int key) {
+    return key < len && (key >= w.start || key < w.sinks);
+}
+
 // Exclusive prefix of tiles per sequence into shared memory (s_tp[batch] = total).
 // Every thread of the CTA must call it (blockDim.x a multiple of 32, at most 1024); ends with
 // a __syncthreads().  Warp-shuffle scan, then the warp totals through shared memory.
 // With s_rem (one byte per sequence, optional) it also records how many tokens the sequence's last tile holds
 // (context_len mod tile_tokens; 0 = a full tile), for a producer that copies only the rows that exist.
+// WINDOW: only the tiles of window_tiles() count.
+template <bool WINDOW = false>
 __device__ inline void build_tile_prefix(const int32_t* __restrict__ context_lens, int batch, int tile_tokens,
                                          int* s_tp, int* s_scratch /* 32 ints */, uint8_t* s_rem = nullptr,
-                                         int seg_overhead = 0) {
+                                         int seg_overhead = 0, int window = 0, int sinks = 0) {
     const int nt = blockDim.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int per = (batch + nt - 1) / nt;
     const int lo = min(batch, tid * per), hi = min(batch, lo + per);
     int sum = 0;
     // tiles of a sequence in the padded numbering (per head group); an empty sequence has none
-    auto padded = [&](int len) { return len > 0 ? (len + tile_tokens - 1) / tile_tokens + seg_overhead : 0; };
+    auto padded = [&](int len) {
+        if constexpr (WINDOW) return len > 0 ? window_tiles(len, tile_tokens, window, sinks).count + seg_overhead : 0;
+        else return len > 0 ? (len + tile_tokens - 1) / tile_tokens + seg_overhead : 0;
+    };
     for (int i = lo; i < hi; ++i) sum += padded(context_lens[i]);
     int incl = sum;
 #pragma unroll

@@ -5,6 +5,11 @@
 * ``paged_attn_decode`` / ``paged_attn_prefill`` - the two calls the reference makes into
   the flash_attn package (infer/ops/attention.py:110-121), with the keyword names it uses.
 * ``flash_attn_prefill(Q, K, V, O)`` - the reference's own dense op (src/bindings.cpp:9).
+* ``load_kvcache`` - rows of the pools read back as bf16; ``rotary_append`` / ``rotary_embedding`` - rotary
+  positions in general form, with or without the append.  They have no counterpart in the reference.
+
+Sliding windows: the paged attention ops take ``window`` (how many keys a query sees, its own among them;
+None = all) and ``sinks`` (how many first keys stay visible in front of the window).
 
 Every op launches hand-written sm_100a kernels through the C ABI on the current CUDA
 stream and is also registered as ``torch.ops._C.<name>`` with out-parameter schemas in
@@ -235,10 +240,117 @@ def qk_norm_rope_append(q, k, v, q_norm_weight, k_norm_weight, eps, positions, c
     return q_out
 
 
+def _rows(what, name, x, device=None):
+    """``x`` as rows [T, H, 128] of bf16 with contiguous heads on the GPU; their pitch in elements."""
+    if x.dim() != 3 or x.dtype != torch.bfloat16 or not x.is_cuda or x.shape[2] != 128:
+        raise RuntimeError(f"{what}: {name} must be a bf16 CUDA tensor [T, H, 128]")
+    if x.stride(2) != 1 or (x.shape[1] > 1 and x.stride(1) != 128):
+        raise RuntimeError(f"{what}: {name} must have contiguous heads")
+    if device is not None and x.device != device:
+        raise RuntimeError(f"{what}: {name} is on {x.device}, the call on {device}")
+    return x.stride(0) if x.shape[0] > 1 else x.shape[1] * 128
+
+
+def _vector(what, name, x, n, dtype, device):
+    if x.dtype != dtype or not x.is_cuda or x.device != device or x.numel() != n or not x.is_contiguous():
+        raise RuntimeError(f"{what}: {name} must be a contiguous {str(dtype)[6:]} tensor of {n} values on {device}")
+
+
+def load_kvcache(k_cache, v_cache, slot_mapping, k_scale=None, v_scale=None, k_out=None, v_out=None):
+    """The cached rows of ``slot_mapping`` (int32, any order, repeats allowed) as bf16 -> (k, v), each ``[n, Hkv, 128]``:
+    the inverse of ``store_kvcache``.  e4m3 pools: byte * scale of its page and head, in fp32, rounded once.  Slots
+    outside the pool (-1: padding) give rows of zeros.  ``k_out`` / ``v_out`` may be column slices of a wider row."""
+    pool = pool_of(k_cache, v_cache, k_scale, v_scale)
+    n = slot_mapping.numel()
+    _vector("load_kvcache", "slot_mapping", slot_mapping, n, torch.int32, pool.device)
+    shape = (n, pool.n_kv_heads, pool.head_dim)
+    k_out, v_out = (torch.empty(shape, dtype=torch.bfloat16, device=pool.device) if t is None else t for t in (k_out, v_out))
+    pitch = []
+    for name, t in (("k_out", k_out), ("v_out", v_out)):
+        pitch.append(_rows("load_kvcache", name, t, pool.device))
+        if tuple(t.shape) != shape:
+            raise RuntimeError(f"load_kvcache: {name} must be {list(shape)}")
+    with _on_device(pool.device):
+        rc = _lib.load().infer_kv_load(pool.handle, _ptr(k_out), _ptr(v_out), pitch[0], pitch[1], _ptr(slot_mapping), n, _stream())
+    _lib.check(rc, "load_kvcache")
+    return k_out, v_out
+
+
+def _rotary_args(what, q, k, positions, inv_freq, q_out, device):
+    t = q.shape[0]
+    q_pitch, k_pitch = _rows(what, "q", q, device), _rows(what, "k", k, device)
+    if k.shape[0] != t:
+        raise RuntimeError(f"{what}: q and k must have the same number of rows")
+    _vector(what, "positions", positions, t, torch.int64, device)
+    _vector(what, "inv_freq", inv_freq, inv_freq.numel(), torch.float64, device)
+    if q_out is None:
+        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    q_out_pitch = _rows(what, "q_out", q_out, device)
+    if q_out.shape != q.shape:
+        raise RuntimeError(f"{what}: q_out must have the shape of q")
+    return q_out, q_pitch, k_pitch, q_out_pitch
+
+
+def rotary_append(q, k, v, positions, inv_freq, k_cache, v_cache, slot_mapping, interleaved=False, attention_factor=1.0,
+                  q_out=None):
+    """Rotary positions of q and k and ``store_kvcache`` of k and v in one kernel (bf16 pools).
+
+    The first ``rot_dim = 2 * inv_freq.numel()`` dims of every head (a multiple of 16, at most 128) are rotated in pairs
+    ``(i, i + rot_dim / 2)``, or ``(2i, 2i + 1)`` with ``interleaved``, by ``positions[t] * inv_freq[i]``; the others stay.
+    ``inv_freq``: float64 (see ``rotary.rotary_frequencies`` for scaled contexts); angles are reduced in 64 bits, the
+    rotation runs in 32 and rounds once.  ``attention_factor`` multiplies cosine and sine.  q, k, v are ``[T, H, 128]`` views
+    (column slices of the fused qkv output are fine); returns the rotated q, contiguous, or in ``q_out`` (may be ``q``).
+    Rows with a slot outside the pool are not stored."""
+    pool = pool_of(k_cache, v_cache)
+    q_out, q_pitch, k_pitch, q_out_pitch = _rotary_args("rotary_append", q, k, positions, inv_freq, q_out, pool.device)
+    v_pitch, t = _rows("rotary_append", "v", v, pool.device), q.shape[0]
+    if k.shape != v.shape or k.shape[1] != pool.n_kv_heads:
+        raise RuntimeError("rotary_append: k and v must have the pool's heads and q's rows")
+    _vector("rotary_append", "slot_mapping", slot_mapping, t, torch.int32, pool.device)
+    with _on_device(pool.device):
+        rc = _lib.load().infer_rotary_append(pool.handle, _ptr(q_out), q_out_pitch, _ptr(q), _ptr(k), _ptr(v), q_pitch, k_pitch,
+                                             v_pitch, _ptr(positions), _ptr(inv_freq), 2 * inv_freq.numel(), int(interleaved),
+                                             float(attention_factor), _ptr(slot_mapping), t, q.shape[1], _stream())
+    _lib.check(rc, "rotary_append")
+    return q_out
+
+
+def rotary_embedding(q, k, positions, inv_freq, interleaved=False, attention_factor=1.0, q_out=None, k_out=None):
+    """``rotary_append`` without the append -> (q, k) rotated; in front of ``store_kvcache`` for an e4m3 pool.
+    ``q_out`` / ``k_out`` may be ``q`` / ``k``."""
+    q_out, q_pitch, k_pitch, q_out_pitch = _rotary_args("rotary_embedding", q, k, positions, inv_freq, q_out, q.device)
+    if k_out is None:
+        k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    k_out_pitch = _rows("rotary_embedding", "k_out", k_out, q.device)
+    if k_out.shape != k.shape:
+        raise RuntimeError("rotary_embedding: k_out must have the shape of k")
+    with _on_device(q.device):
+        rc = _lib.load().infer_rotary_embed(_ptr(q_out), _ptr(k_out), q_out_pitch, k_out_pitch, _ptr(q), _ptr(k), q_pitch, k_pitch,
+                                            _ptr(positions), _ptr(inv_freq), 2 * inv_freq.numel(), int(interleaved),
+                                            float(attention_factor), q.shape[0], q.shape[1], k.shape[1], _stream())
+    _lib.check(rc, "rotary_embedding")
+    return q_out, k_out
+
+
+def _window(what, window, sinks):
+    """``window`` and ``sinks`` as the library takes them: 0 = no window."""
+    if window is None:
+        if sinks:
+            raise RuntimeError(f"{what}: sinks without a window (every key is visible)")
+        return 0, 0
+    window, sinks = int(window), int(sinks)
+    if window < 1 or sinks < 0:
+        raise RuntimeError(f"{what}: window must be at least 1 and sinks at least 0")
+    return min(window, 0x7fffffff), min(sinks, 0x7fffffff)
+
+
 # --------------------------------------------------------------------------- decode
 def paged_attn_decode(q, k_cache, v_cache, cache_seqlens, block_table, softmax_scale,
-                      out=None, k_scale=None, v_scale=None, workspace=None):
+                      out=None, k_scale=None, v_scale=None, workspace=None, window=None, sinks=0):
     """q [B, Hq, 128] (or [B, 1, Hq, 128] as the reference passes it) -> same shape.
+
+    ``window`` / ``sinks``: only the last ``window`` keys of a sequence (the newest among them) and its first ``sinks``
+    ones are visible; pages without a visible key are not read, nor are their entries in ``block_table``.
 
     ``q`` and ``out`` may also be pinned host tensors: the kernel then reads the queries from, and writes the
     output rows straight into, host memory (a pinned tensor's address is valid on the device), which saves
@@ -259,14 +371,20 @@ def paged_attn_decode(q, k_cache, v_cache, cache_seqlens, block_table, softmax_s
             raise RuntimeError(f"paged_attn_decode: {name} must be an int32 CUDA tensor")
     if block_table.stride(-1) != 1:
         raise RuntimeError("paged_attn_decode: block_table rows must be contiguous")
+    window, sinks = _window("paged_attn_decode", window, sinks)
     pool = pool_of(k_cache, v_cache, k_scale, v_scale)
     o = torch.empty(q3.shape, dtype=q3.dtype, device=pool.device) if out is None else out.view(q3.shape)
     lib = _lib.load()
     b, hq, _ = q3.shape
     ws = workspace if workspace is not None else _SCRATCH.get(pool.device, "decode", pool.decode_workspace_bytes(b, hq))
     with _on_device(pool.device):
-        rc = _call_decode(lib, pool.handle, _ptr(o), _ptr(q3), _ptr(cache_seqlens), _ptr(block_table),
-                          block_table.stride(0), b, hq, float(softmax_scale), _ptr(ws), ws.numel(), _stream())
+        if window:
+            rc = lib.infer_paged_decode_window(pool.handle, _ptr(o), _ptr(q3), _ptr(cache_seqlens), _ptr(block_table),
+                                               block_table.stride(0), b, hq, float(softmax_scale), window, sinks, _ptr(ws),
+                                               ws.numel(), _stream())
+        else:
+            rc = _call_decode(lib, pool.handle, _ptr(o), _ptr(q3), _ptr(cache_seqlens), _ptr(block_table),
+                              block_table.stride(0), b, hq, float(softmax_scale), _ptr(ws), ws.numel(), _stream())
         _lib.check(rc, "paged_attn_decode")
         if _CHECK and not torch.cuda.is_current_stream_capturing():
             _lib.check(lib.infer_paged_decode_status(_ptr(ws), _stream()), "paged_attn_decode (device status)")
@@ -274,13 +392,14 @@ def paged_attn_decode(q, k_cache, v_cache, cache_seqlens, block_table, softmax_s
 
 
 def paged_attn_decode_append(q, key, value, k_cache, v_cache, cache_seqlens, block_table, softmax_scale,
-                             out=None, workspace=None):
+                             out=None, workspace=None, window=None, sinks=0):
     """``store_kvcache(key, value, ...)`` and ``paged_attn_decode(q, ...)`` of one decode step in ONE launch
     (bf16 pools; the two calls of infer/ops/attention.py:109 and :117-121).  ``key`` / ``value`` are the step's
     new rows ``[B, Hkv, 128]`` (column slices of a fused qkv output are fine), row b belonging to position
     ``cache_seqlens[b] - 1`` of sequence b; the slot is read off ``block_table``, so no ``slot_mapping`` is
     needed.  The pools end up as after ``store_kvcache``.  ``q``, ``key``, ``value`` and ``out`` may be pinned
-    host tensors (see ``paged_attn_decode``)."""
+    host tensors, ``window`` and ``sinks`` limit the visible keys (see ``paged_attn_decode``)."""
+    window, sinks = _window("paged_attn_decode_append", window, sinks)
     shape = q.shape
     q3 = q.reshape(shape[0], shape[-2], shape[-1])
     if q3.dtype != torch.bfloat16 or not q3.is_contiguous():
@@ -307,9 +426,12 @@ def paged_attn_decode_append(q, key, value, k_cache, v_cache, cache_seqlens, blo
     v_pitch = value.stride(0) if b > 1 else row
     ws = workspace if workspace is not None else _SCRATCH.get(pool.device, "decode", pool.decode_workspace_bytes(b, hq))
     with _on_device(pool.device):
-        rc = lib.infer_paged_decode_append(pool.handle, _ptr(o), _ptr(q3), _ptr(key), _ptr(value), k_pitch, v_pitch,
-                                           _ptr(cache_seqlens), _ptr(block_table), block_table.stride(0), b, hq,
-                                           float(softmax_scale), _ptr(ws), ws.numel(), _stream())
+        args = (pool.handle, _ptr(o), _ptr(q3), _ptr(key), _ptr(value), k_pitch, v_pitch, _ptr(cache_seqlens),
+                _ptr(block_table), block_table.stride(0), b, hq, float(softmax_scale))
+        if window:
+            rc = lib.infer_paged_decode_append_window(*args, window, sinks, _ptr(ws), ws.numel(), _stream())
+        else:
+            rc = lib.infer_paged_decode_append(*args, _ptr(ws), ws.numel(), _stream())
         _lib.check(rc, "paged_attn_decode_append")
         if _CHECK and not torch.cuda.is_current_stream_capturing():
             _lib.check(lib.infer_paged_decode_status(_ptr(ws), _stream()), "paged_attn_decode_append (device status)")
