@@ -10,8 +10,10 @@ from .context import get_context
 
 
 class Attention(torch.nn.Module):
-    def __init__(self, num_heads: int, head_dim: int, scale: float, num_kv_heads: int):
+    def __init__(self, num_heads: int, head_dim: int, scale: float, num_kv_heads: int, window: int | None = None, sinks: int = 0):
+        """``window`` / ``sinks``: a sliding-window layer, whose queries see the last ``window`` keys and the first ``sinks``."""
         super().__init__()
+        self.window, self.sinks = window, sinks
         self.num_heads, self.head_dim, self.scale, self.num_kv_heads = num_heads, head_dim, scale, num_kv_heads
         self.k_cache = self.v_cache = torch.tensor([])
         self.k_scale = self.v_scale = None        # set together with uint8 pools for FP8 KV
@@ -29,7 +31,7 @@ class Attention(torch.nn.Module):
             # holds as well (infer/engine/model_runner.py:110-126); rows with context_len 0 (the padding of a
             # captured batch, slot -1 there) are skipped by both.
             O = ops.paged_attn_decode_append(Q.contiguous(), K, V, self.k_cache, self.v_cache, ctx.context_lens,
-                                             ctx.block_tables, self.scale)
+                                             ctx.block_tables, self.scale, window=self.window, sinks=self.sinks)
             return O.view(-1, self.num_heads * self.head_dim)
         ops.store_kvcache(K, V, self.k_cache, self.v_cache, ctx.slot_mapping, self.k_scale, self.v_scale)
         if ctx.is_prefill:
@@ -37,8 +39,10 @@ class Attention(torch.nn.Module):
             if block_tables is None:
                 raise RuntimeError("Attention: prefill needs block_tables (keys are read from the pools)")
             O = ops.paged_attn_prefill(Q.contiguous(), self.k_cache, self.v_cache, ctx.cu_seqlens_q, ctx.cu_seqlens_k,
-                                       ctx.max_seqlen_q, ctx.max_seqlen_k, self.scale, block_tables)
+                                       ctx.max_seqlen_q, ctx.max_seqlen_k, self.scale, block_tables,
+                                       k_scale=self.k_scale, v_scale=self.v_scale, window=self.window, sinks=self.sinks)
         else:
             O = ops.paged_attn_decode(Q.contiguous(), self.k_cache, self.v_cache, ctx.context_lens, ctx.block_tables,
-                                      self.scale, k_scale=self.k_scale, v_scale=self.v_scale)
+                                      self.scale, k_scale=self.k_scale, v_scale=self.v_scale, window=self.window,
+                                      sinks=self.sinks)
         return O.view(-1, self.num_heads * self.head_dim)

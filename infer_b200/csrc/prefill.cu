@@ -23,7 +23,7 @@ static std::mutex g_prefill_status_mutex;
 
 // Device address of the status word on the current device; nullptr (the kernels then report
 // nothing) if it cannot be looked up.
-static int* prefill_status_word() {
+int* prefill_status_word() {
     int dev = -1;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return nullptr;
     std::lock_guard<std::mutex> lock(g_prefill_status_mutex);

@@ -26,6 +26,9 @@ struct PrefillParams {
     int stall_producer;       // self-test only: the producer loads nothing, so every wait runs out
 };
 
+// Device address of the prefill kernels' status word on the current device (prefill.cu); nullptr if it cannot be looked up.
+int* prefill_status_word();
+
 // mma.sync path (prefill_mma.cu): 64 query rows per CTA.
 int launch_prefill_mma(bool paged, const PrefillParams& p, const CUtensorMap& mk, const CUtensorMap& mv, int max_q,
                        int batch, cudaStream_t st);

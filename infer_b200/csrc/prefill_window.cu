@@ -1,0 +1,786 @@
+// Paged prefill attention with a sliding window and sinks over bf16 pools, and with or without them over e4m3 pools, on
+// the 5th-generation tensor cores.
+//
+// Query i of a sequence (its position in the sequence) sees key j when j <= i and (i - j < window or j < sinks).
+//     out_i = sum_j softmax_j(scale * q_i . k_j) v_j,    k_j = byte * k_scale[page(j), head] in an e4m3 pool, v_j likewise.
+//
+// The pipeline is that of prefill_tc.cu (two query tiles of 128 rows per CTA that share every 128-key tile, S and O in
+// tensor memory, P written back to tensor memory, one softmax warpgroup per query tile with a row per thread, a lazy
+// reference maximum).  What differs:
+//
+// Rows.  A query tile holds the query heads of ONE kv head over 128 / group consecutive tokens (row = token * group +
+//   head), for any group size, loaded with one TMA box per half.  A chunk of 45 tokens with four heads per kv head fills
+//   1.4 tiles instead of four a third full, and a tile spans few positions, so that a window cuts its key range close.
+// Keys.  A CTA walks the tiles that hold a key visible to any of its rows: those of the sinks, then those from the start
+//   of its first row's window on.  Block-table entries of other pages are never read.  V rows that no row of the CTA sees
+//   are cleared before the tensor core reads them: P is 0 there, but 0 times a stale NaN is not.
+// Few rows.  When the (row block, kv head, sequence) triples do not fill the GPU, the key tiles of a CTA are split over
+//   several, each leaving maximum, sum and accumulator per row in 32 bits, and a second kernel joins them.
+// e4m3.  TMA brings the raw bytes (16 KiB per tile, half of bf16's traffic) into two staging slots and a fourth warpgroup
+//   turns them into f16 operand tiles (e4m3 -> f16 is exact, one conversion instruction per two values, next to softmax
+//   warps that leave more than half of the issue slots idle).  Q is brought to f16 in place, each row scaled by a power of
+//   two that puts its largest value into [1, 2): exact but for values 2^-14 below it.  The K scale of a tile's page and
+//   the row's power of two go into the factor of the softmax exponent.  The V scale goes into P: P = 2^(x - m) * 2^kBias *
+//   v_scale / v_ref, where v_ref is the largest V scale met so far within a factor of 8; the row sum takes it out again
+//   with one multiplication per tile, the output multiplies by v_ref.  P in f16 then lies below 2^(6 + 6 + 3) and keeps 11
+//   bits down to 2^-14 - 6 of the row's maximum, where bf16 would keep 8.  A page whose V scale is 2^-20 of v_ref or less
+//   loses bits of its values, which is an error of 2^-33 v_ref.
+//
+// Every wait is bounded; one that runs out raises the abort flag, every role drains to the common epilogue, tensor memory
+// is freed and the status word of the prefill kernels is set.
+#include <atomic>
+
+#include "prefill.cuh"
+#include "tcgen05.cuh"
+
+namespace ib {
+
+constexpr int kPwRows = 128;                  // rows per query tile (= TMEM lanes)
+constexpr int kPwKeys = 128;                  // keys per K/V tile
+constexpr int kPwHalf = 128 * 128;            // bytes of one [128 rows][64 elems] swizzled sub-tile
+constexpr int kPwTile = 2 * kPwHalf;          // 32 KiB: one Q, K or V tile of 16-bit elements
+constexpr int kPwRaw = 128 * 128;             // 16 KiB: one K or V tile of e4m3 bytes
+constexpr int kPwScaleRing = 8;               // a tile's scales stay here from its K's load to its softmax: at most 6 tiles
+// tensor memory columns: S (shared by the two tiles) at 0, P of tile i at 128 + 64 i, O of tile i at 256 + 128 i
+constexpr uint32_t kPwTmemP = 128, kPwTmemO = 256;
+constexpr int kPwSoftmaxWarps = 8;
+constexpr int kPwProducer = 8, kPwIssueS = 9, kPwIssuePV = 10;   // warp roles; 0-7 softmax, 11 idle, 12-15 converters (e4m3)
+
+template <bool FP8>
+struct PwCfg {
+    static constexpr int k_stages = FP8 ? 2 : 3, v_stages = 2, raw_slots = FP8 ? 2 : 0;
+    static constexpr int threads = (kPwSoftmaxWarps + (FP8 ? 8 : 4)) * 32;
+    static constexpr int q = 0;
+    static constexpr int k = q + 2 * kPwTile;
+    static constexpr int v = k + k_stages * kPwTile;
+    static constexpr int raw = v + v_stages * kPwTile;
+    static constexpr int bars = raw + raw_slots * kPwRaw;
+    static constexpr int n_bars = 26;
+    static constexpr int misc = bars + n_bars * 8;                    // tmem base, abort flag
+    static constexpr int scales = misc + 16;                          // [kPwScaleRing] (k scale, v scale)
+    static constexpr int qscale = scales + (FP8 ? kPwScaleRing * 8 : 0);    // [2][128] power of two taken out of a Q row
+    static constexpr int total = qscale + (FP8 ? 2 * kPwRows * 4 : 0);
+    // the probabilities' exponent: how far the reference maximum may lag, and what is added to it
+    static constexpr float lazy = FP8 ? 6.f : 8.f, bias = FP8 ? 6.f : 0.f;
+};
+
+enum PwBar { PW_Q_FULL = 0, PW_K_FULL = 1, PW_K_EMPTY = 4, PW_V_FULL = 7, PW_V_EMPTY = 9, PW_S_FULL = 11, PW_P_FULL = 13,
+             PW_PV_DONE = 15, PW_DRAIN = 17, PW_S_FREE = 19, PW_RAW_FULL = 20, PW_RAW_EMPTY = 22, PW_Q_READY = 24 };
+
+struct PwParams {
+    __nv_bfloat16* out;
+    const int32_t* cu_q;
+    const int32_t* cu_k;
+    const int32_t* block_tables;
+    int64_t bt_stride;
+    const float* k_scale;
+    const float* v_scale;
+    int n_q_heads, n_kv_heads, group;
+    int tokens;              // tokens per query tile: 128 / group
+    int block_size, num_blocks;
+    int window, sinks;       // window: 0x7fffffff = none
+    float scale_log2;
+    int splits;              // CTAs that share the key tiles of a row block
+    int64_t total_q;
+    float* part_ml;          // splits > 1: [splits][total_q * n_q_heads][2] maximum (log2), sum
+    float* part_o;           // [splits][total_q * n_q_heads][128]
+    int* status;             // may be null
+    uint32_t wait_limit;
+    int stall_producer;
+};
+
+template <bool FP8>
+__global__ void __launch_bounds__(PwCfg<FP8>::threads, 1) prefill_window_kernel(PwParams p, const __grid_constant__ CUtensorMap map_q,
+                                                                                const __grid_constant__ CUtensorMap map_k,
+                                                                                const __grid_constant__ CUtensorMap map_v) {
+    using C = PwCfg<FP8>;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const uint32_t base = smem_u32(smem);
+    volatile uint32_t* s_tmem = reinterpret_cast<volatile uint32_t*>(smem + C::misc);
+    volatile int* s_abort = reinterpret_cast<volatile int*>(smem + C::misc + 4);
+    volatile float* s_scale = reinterpret_cast<volatile float*>(smem + C::scales);
+    volatile float* s_qscale = reinterpret_cast<volatile float*>(smem + C::qscale);
+    auto bar = [&](int which, int idx = 0) { return base + uint32_t(C::bars) + uint32_t(which + idx) * 8; };
+
+    const int b = blockIdx.z;
+    const int kvh = blockIdx.y / p.splits, split = blockIdx.y - kvh * p.splits;
+    const int xb = int(gridDim.x) - 1 - int(blockIdx.x);    // longest rows first
+    const int q0 = p.cu_q[b];
+    const int lq = p.cu_q[b + 1] - q0, lk = p.cu_k[b + 1] - p.cu_k[b];
+    const int shift = lk - lq;                              // position of the first query row
+    const int tok0 = xb * 2 * p.tokens;                     // first token of the CTA
+    if (tok0 >= lq) return;                                 // whole CTA leaves before any barrier or TMEM use
+    const bool two = tok0 + p.tokens < lq;                  // the second tile has rows
+    // key tiles: [0, n_sink) and [n_sink + skip, last], list entry x is tile x below n_sink and x + skip from there on
+    const int pos_lo = shift + tok0, pos_hi = shift + min(lq, tok0 + 2 * p.tokens) - 1;
+    const bool windowed = p.window < lk;
+    const int first_key = windowed ? max(pos_lo - p.window + 1, 0) : 0;
+    const int sinks = windowed ? min(p.sinks, lk) : 0;
+    int n_sink = (sinks + kPwKeys - 1) / kPwKeys;
+    const int skip = max(first_key / kPwKeys - n_sink, 0);
+    if (skip == 0) n_sink = 0;
+    const int n_all = pos_hi < 0 ? 0 : pos_hi / kPwKeys + 1 - skip;
+    const int per_split = (n_all + p.splits - 1) / p.splits;
+    const int x0 = min(n_all, split * per_split), n = min(n_all, x0 + per_split) - x0;
+    auto tile_at = [&](int j) { return x0 + j < n_sink ? x0 + j : x0 + j + skip; };
+
+    if (n <= 0) {
+        // nothing is visible here: zeros, or an empty part
+        const int rows = min(lq - tok0, 2 * p.tokens) * p.group;
+        for (int i = threadIdx.x; i < rows * 16; i += C::threads) {
+            const int r = i >> 4, tok = tok0 + r / p.group, head = kvh * p.group + r % p.group;
+            const int64_t row = int64_t(q0 + tok) * p.n_q_heads + head;
+            if (p.splits == 1) {
+                reinterpret_cast<uint4*>(p.out + row * kHeadDim)[i & 15] = make_uint4(0, 0, 0, 0);
+            } else if ((i & 15) == 0) {
+                reinterpret_cast<float2*>(p.part_ml)[int64_t(split) * p.total_q * p.n_q_heads + row] = make_float2(-INFINITY, 0.f);
+            }
+        }
+        return;
+    }
+    // The roles of the third warpgroup sit in the first four hardware warps (see prefill_tc.cu), the converters in the last.
+    const int hw = int(threadIdx.x >> 5), lane = threadIdx.x & 31;
+    const int warp = hw < 4 ? hw + kPwSoftmaxWarps : hw < 12 ? hw - 4 : hw;
+
+    if (threadIdx.x == 0) {
+        mbar_init(bar(PW_Q_FULL), 1);
+        mbar_init(bar(PW_Q_READY), 4);
+        for (int i = 0; i < C::k_stages; ++i) {
+            mbar_init(bar(PW_K_FULL, i), FP8 ? 4 : 1);
+            mbar_init(bar(PW_K_EMPTY, i), 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(bar(PW_V_FULL, i), FP8 ? 4 : 1);
+            mbar_init(bar(PW_V_EMPTY, i), 1);
+            mbar_init(bar(PW_S_FULL, i), 1);
+            mbar_init(bar(PW_P_FULL, i), 128);
+            mbar_init(bar(PW_PV_DONE, i), 1);
+            mbar_init(bar(PW_DRAIN, i), 1);
+            mbar_init(bar(PW_RAW_FULL, i), 1);
+            mbar_init(bar(PW_RAW_EMPTY, i), 4);
+        }
+        mbar_init(bar(PW_S_FREE), 128);                     // the warpgroup that copied the S buffer to registers
+        *s_abort = 0;
+        fence_mbar_init();
+        fence_proxy_async();
+    }
+    if (warp == kPwIssueS) {
+        // all 512 columns (one CTA per SM by shared-memory use)
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                     ::"r"(base + uint32_t(C::misc)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = __shfl_sync(0xffffffffu, *s_tmem, 0);   // warp-uniform by construction
+    bool ok = true;
+    // V rows of key tile `tile` that some row of the CTA sees: [0, sink_end) and [begin, end)
+    auto seen_rows = [&](int tile, int& sink_end, int& begin, int& end) {
+        const int kb = tile * kPwKeys;
+        sink_end = max(sinks - kb, 0);
+        begin = first_key - kb;
+        end = pos_hi + 1 - kb;
+    };
+
+    // Register budget.  bf16: 384 threads x 168 at launch, the third warpgroup hands 64 per thread to the softmax
+    // warpgroups.  e4m3: 512 threads x 128, roles and converters keep 56.  Both end at 200 per softmax thread.
+    if (hw < 4) {
+        if constexpr (FP8) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;" ::: "memory");
+        else asm volatile("setmaxnreg.dec.sync.aligned.u32 104;" ::: "memory");
+        if (warp == kPwProducer) {
+            // ============================================================= TMA producer
+            if (lane == 0 && !p.stall_producer) {
+                tma_prefetch_desc(&map_q);
+                tma_prefetch_desc(&map_k);
+                tma_prefetch_desc(&map_v);
+                const int n_q = two ? 2 : 1;
+                mbar_expect_tx(bar(PW_Q_FULL), n_q * 2 * p.tokens * p.group * 128);
+                for (int i = 0; i < n_q; ++i)
+                    for (int half = 0; half < 2; ++half)
+                        tma_load_3d(base + C::q + i * kPwTile + half * kPwHalf, &map_q, bar(PW_Q_FULL), half * 64, kvh * p.group,
+                                    q0 + tok0 + i * p.tokens);
+                const int32_t* table = p.block_tables + int64_t(b) * p.bt_stride;
+                auto page_of = [&](int tile) {
+                    const int idx = tile * kPwKeys / p.block_size;
+                    return idx < p.bt_stride ? table[idx] : -1;
+                };
+                // a page outside of the pool gives rows of zeros (TMA fills what lies outside of the tensor)
+                auto slot_of = [&](int tile, int page) {
+                    return page >= 0 && page < p.num_blocks ? page * p.block_size + tile * kPwKeys % p.block_size : -kPwKeys;
+                };
+                if constexpr (FP8) {
+                    // order K0, K1, V0, K2, V1, ...: K of the next tile is needed before V of this one
+                    int issued = 0;
+                    auto load_raw = [&](const CUtensorMap* map, int slot) {
+                        const int s = issued & 1;
+                        if (!tc_wait(bar(PW_RAW_EMPTY, s), ((issued >> 1) & 1) ^ 1, s_abort, p.wait_limit)) { ok = false; return; }
+                        mbar_expect_tx(bar(PW_RAW_FULL, s), kPwRaw);
+                        tma_load_3d(base + C::raw + s * kPwRaw, map, bar(PW_RAW_FULL, s), 0, kvh, slot);
+                        ++issued;
+                    };
+                    int page = page_of(tile_at(0)), v_slot = 0;      // page of tile j, looked up one tile ahead
+                    for (int j = 0; j <= n && ok; ++j) {
+                        int k_slot = 0;
+                        if (j < n) {
+                            const bool in = page >= 0 && page < p.num_blocks;
+                            const float ks = in ? p.k_scale[int64_t(page) * p.n_kv_heads + kvh] : 0.f;
+                            const float vs = in ? p.v_scale[int64_t(page) * p.n_kv_heads + kvh] : 0.f;
+                            k_slot = slot_of(tile_at(j), page);
+                            if (j + 1 < n) page = page_of(tile_at(j + 1));
+                            s_scale[(j % kPwScaleRing) * 2] = ks;     // released by the arrival on RAW_FULL
+                            s_scale[(j % kPwScaleRing) * 2 + 1] = vs;
+                            load_raw(&map_k, k_slot);
+                        }
+                        if (j >= 1 && ok) load_raw(&map_v, v_slot);
+                        v_slot = k_slot;
+                    }
+                    // never leave with a copy in flight: wait (bounded) for everything that was armed
+                    mbar_wait(bar(PW_Q_FULL), 0, p.wait_limit);
+                    for (int i = max(0, issued - 2); i < issued; ++i) mbar_wait(bar(PW_RAW_FULL, i & 1), (i >> 1) & 1, p.wait_limit);
+                } else {
+                    auto load_tile = [&](const CUtensorMap* map, uint32_t dst, uint32_t full, int slot) {
+                        mbar_expect_tx(full, kPwTile);
+                        tma_load_3d(dst, map, full, 0, kvh, slot);
+                        tma_load_3d(dst + kPwHalf, map, full, 64, kvh, slot);
+                    };
+                    int k_issued = 0, v_issued = 0, v_slot = 0;
+                    for (int j = 0; j <= n && ok; ++j) {
+                        int k_slot = 0;
+                        if (j < n) {
+                            const int s = j % C::k_stages, tile = tile_at(j);
+                            k_slot = slot_of(tile, page_of(tile));
+                            if (tc_wait(bar(PW_K_EMPTY, s), ((j / C::k_stages) & 1) ^ 1, s_abort, p.wait_limit)) {
+                                load_tile(&map_k, base + C::k + s * kPwTile, bar(PW_K_FULL, s), k_slot);
+                                ++k_issued;
+                            } else ok = false;
+                        }
+                        if (j >= 1 && ok) {
+                            const int jv = j - 1, s = jv & 1;
+                            if (tc_wait(bar(PW_V_EMPTY, s), ((jv >> 1) & 1) ^ 1, s_abort, p.wait_limit)) {
+                                load_tile(&map_v, base + C::v + s * kPwTile, bar(PW_V_FULL, s), v_slot);
+                                ++v_issued;
+                            } else ok = false;
+                        }
+                        v_slot = k_slot;
+                    }
+                    mbar_wait(bar(PW_Q_FULL), 0, p.wait_limit);
+                    for (int j = max(0, k_issued - C::k_stages); j < k_issued; ++j)
+                        mbar_wait(bar(PW_K_FULL, j % C::k_stages), (j / C::k_stages) & 1, p.wait_limit);
+                    for (int j = max(0, v_issued - 2); j < v_issued; ++j) mbar_wait(bar(PW_V_FULL, j & 1), (j >> 1) & 1, p.wait_limit);
+                }
+            }
+        } else if (warp == kPwIssueS) {
+            // ============================================================= MMA issue: the S products
+            // S_0(0) S_1(0) S_0(1) S_1(1) ...: each once the warpgroup of the previous one has copied the S buffer (S_FREE)
+            constexpr uint32_t idesc_s = tc_idesc(false, FP8);
+            const uint64_t q_desc0 = tc_desc(base + C::q, 16), k_desc0 = tc_desc(base + C::k, 16);
+            int n_s = 0;                               // S products issued so far
+            auto issue_s = [&](int i, int stage) {     // S = Q_i K^T  (K_FULL of that stage already awaited)
+                if (n_s > 0 && !tc_wait(bar(PW_S_FREE), (n_s - 1) & 1, s_abort, p.wait_limit)) { ok = false; return; }
+                ++n_s;
+                tc_fence_after();
+                if (elect_one()) {
+                    const uint64_t qd = q_desc0 + uint64_t(i * (kPwTile >> 4));
+                    const uint64_t kd = k_desc0 + uint64_t(stage * (kPwTile >> 4));
+#pragma unroll
+                    for (int kk = 0; kk < 8; ++kk) {
+                        const uint32_t off = ((kk >> 2) * kPwHalf + (kk & 3) * 32) >> 4;
+                        tc_mma(tmem, qd + off, kd + off, idesc_s, kk > 0);
+                    }
+                    tc_commit(bar(PW_S_FULL, i));
+                }
+                __syncwarp();
+            };
+            if (!tc_wait(bar(FP8 ? PW_Q_READY : PW_Q_FULL), 0, s_abort, p.wait_limit)) ok = false;
+            int ks = 0, kph = 0;                                           // stage and phase of K_j
+            for (int j = 0; j < n && ok; ++j) {
+                if (!tc_wait(bar(PW_K_FULL, ks), kph, s_abort, p.wait_limit)) { ok = false; break; }
+                issue_s(0, ks);
+                if (ok && two) issue_s(1, ks);
+                if (!ok) break;
+                if (elect_one()) tc_commit(bar(PW_K_EMPTY, ks));              // all S(j) are issued
+                __syncwarp();
+                if (++ks == C::k_stages) { ks = 0; kph ^= 1; }
+            }
+            // all tensor-core work issued by this warp must have retired before TMEM is freed
+            if (elect_one()) tc_commit(bar(PW_DRAIN, 0));
+            __syncwarp();
+            mbar_wait(bar(PW_DRAIN, 0), 0, p.wait_limit);
+        } else if (warp == kPwIssuePV) {
+            // ============================================================= MMA issue: the P V products
+            constexpr uint32_t idesc_pv = tc_idesc(true, FP8);
+            const uint64_t v_desc0 = tc_desc(base + C::v, kPwHalf);
+            auto issue_pv = [&](int i, int stage, int j) {   // O_i += P_i V  (V_FULL of that stage already awaited)
+                if (!tc_wait(bar(PW_P_FULL, i), j & 1, s_abort, p.wait_limit)) { ok = false; return; }
+                tc_fence_after();
+                if (elect_one()) {
+                    const uint64_t vd = v_desc0 + uint64_t(stage * (kPwTile >> 4));
+                    const uint32_t p_tmem = tmem + kPwTmemP + i * 64;
+#pragma unroll
+                    for (int kk = 0; kk < 8; ++kk)     // 16 keys: 8 packed columns of P, 16 rows of V
+                        tc_mma_ts(tmem + kPwTmemO + i * 128, p_tmem + kk * 8, vd + uint32_t(kk * 16 * 128 >> 4), idesc_pv,
+                                  (j > 0 || kk > 0) ? 1u : 0u);
+                    tc_commit(bar(PW_PV_DONE, i));
+                }
+                __syncwarp();
+            };
+            for (int j = 0; j < n && ok; ++j) {
+                const int vs = j & 1;
+                if (!tc_wait(bar(PW_V_FULL, vs), (j >> 1) & 1, s_abort, p.wait_limit)) { ok = false; break; }
+                if constexpr (!FP8) {
+                    // clear the rows that nobody sees (e4m3: the converters did)
+                    int sink_end, begin, end;
+                    seen_rows(tile_at(j), sink_end, begin, end);
+                    if (end < kPwKeys || begin > sink_end) {
+                        uint8_t* vt = smem + C::v + vs * kPwTile;
+                        for (int x = lane; x < kPwKeys * 8; x += 32) {
+                            const int r = x >> 3;
+                            if (r < sink_end || (r >= begin && r < end)) continue;
+                            *reinterpret_cast<uint4*>(vt + x * 16) = make_uint4(0, 0, 0, 0);
+                            *reinterpret_cast<uint4*>(vt + kPwHalf + x * 16) = make_uint4(0, 0, 0, 0);
+                        }
+                        fence_proxy_async();
+                        __syncwarp();
+                    }
+                }
+                issue_pv(0, vs, j);
+                if (ok && two) issue_pv(1, vs, j);
+                if (!ok) break;
+                if (elect_one()) tc_commit(bar(PW_V_EMPTY, vs));              // all products with V_j are issued
+                __syncwarp();
+            }
+            if (elect_one()) tc_commit(bar(PW_DRAIN, 1));
+            __syncwarp();
+            mbar_wait(bar(PW_DRAIN, 1), 0, p.wait_limit);
+        }
+    } else if (FP8 && hw >= 12) {
+        // ================================================================= converters: e4m3 bytes -> f16 operand tiles
+        if constexpr (FP8) {
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 56;" ::: "memory");
+            const int t = int(threadIdx.x) - 12 * 32;                         // 0 .. 127
+            if (!tc_wait(bar(PW_Q_FULL), 0, s_abort, p.wait_limit)) ok = false;
+            if (ok) {
+                // Q in place, one row per thread; the sixteen 16-byte chunks of a row lie at different banks for the
+                // eight rows of a phase
+                for (int i = 0; i < (two ? 2 : 1); ++i) {
+                    const uint32_t row = base + C::q + i * kPwTile;
+                    uint32_t top = 0;                                         // largest magnitude, as bf16 bits
+                    for (int c = 0; c < 16; ++c) {
+                        const uint4 w = ld_shared_v4(row + (c >> 3) * kPwHalf + swz128(t, c & 7));
+                        const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) top = max(top, max(v[k] & 0x7fffu, (v[k] >> 16) & 0x7fffu));
+                    }
+                    const int e = min(max(int(top >> 7) - 127, -126), 126);
+                    const float down = __uint_as_float(uint32_t(127 - e) << 23);
+                    s_qscale[i * kPwRows + t] = __uint_as_float(uint32_t(127 + e) << 23);
+                    for (int c = 0; c < 16; ++c) {
+                        const uint32_t at = row + (c >> 3) * kPwHalf + swz128(t, c & 7);
+                        uint4 w = ld_shared_v4(at);
+                        uint32_t* v = reinterpret_cast<uint32_t*>(&w);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            v[k] = pack_f16(__uint_as_float(v[k] << 16) * down, __uint_as_float(v[k] & 0xffff0000u) * down);
+                        st_shared_v4(at, w);
+                    }
+                }
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(PW_Q_READY));
+            }
+            // one raw tile after the other, in the order of the producer
+            int seq = 0;
+            auto convert = [&](uint32_t dst, uint32_t full, bool is_v, int j) {
+                const int s = seq & 1;
+                if (!tc_wait(bar(PW_RAW_FULL, s), (seq >> 1) & 1, s_abort, p.wait_limit)) { ok = false; return; }
+                ++seq;
+                int sink_end = kPwKeys, begin = 0, end = kPwKeys;
+                if (is_v) {
+                    seen_rows(tile_at(j), sink_end, begin, end);
+                    if (s_scale[(j % kPwScaleRing) * 2 + 1] == 0.f) sink_end = 0, end = 0;     // a scale of 0: values of 0
+                }
+                const uint32_t src = base + C::raw + s * kPwRaw;
+                const int c = t & 7;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    uint4 w[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) w[i] = ld_shared_v4(src + swz128((h * 4 + i) * 16 + (t >> 3), c));
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int r = (h * 4 + i) * 16 + (t >> 3);
+                        if (is_v && !(r < sink_end || (r >= begin && r < end))) w[i] = make_uint4(0, 0, 0, 0);
+                        uint4 lo, hi;
+                        e4m3x4_to_f16x2x2(w[i].x, lo.x, lo.y);
+                        e4m3x4_to_f16x2x2(w[i].y, lo.z, lo.w);
+                        e4m3x4_to_f16x2x2(w[i].z, hi.x, hi.y);
+                        e4m3x4_to_f16x2x2(w[i].w, hi.z, hi.w);
+                        // sixteen dims become two chunks; lanes 4-7 of a row store the second one first, so that the eight
+                        // lanes of a phase (whose two halves of the dims share banks) hit eight different chunks
+                        const uint32_t half = dst + (c >> 2) * kPwHalf;
+                        const bool swap = c >= 4;
+                        st_shared_v4(half + swz128(r, (c & 3) * 2 + (swap ? 1 : 0)), swap ? hi : lo);
+                        st_shared_v4(half + swz128(r, (c & 3) * 2 + (swap ? 0 : 1)), swap ? lo : hi);
+                    }
+                }
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(full);
+                    mbar_arrive(bar(PW_RAW_EMPTY, s));
+                }
+            };
+            for (int j = 0; j <= n && ok; ++j) {
+                if (j < n) {
+                    const int s = j & 1;
+                    if (tc_wait(bar(PW_K_EMPTY, s), ((j >> 1) & 1) ^ 1, s_abort, p.wait_limit))
+                        convert(base + C::k + s * kPwTile, bar(PW_K_FULL, s), false, j);
+                    else ok = false;
+                }
+                if (j >= 1 && ok) {
+                    const int jv = j - 1, s = jv & 1;
+                    if (tc_wait(bar(PW_V_EMPTY, s), ((jv >> 1) & 1) ^ 1, s_abort, p.wait_limit))
+                        convert(base + C::v + s * kPwTile, bar(PW_V_FULL, s), true, jv);
+                    else ok = false;
+                }
+            }
+        }
+    } else {
+        // ================================================================= softmax, one row per thread
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 200;" ::: "memory");
+        const int g = warp >> 2;                                   // query tile of this warpgroup
+        const int r = (warp & 3) * 32 + lane;                      // row in the tile == TMEM lane
+        const uint32_t lane_sel = uint32_t((warp & 3) * 32) << 16;
+        const int n_kt = g == 0 || two ? n : 0;
+        const int tile_tok = tok0 + g * p.tokens;                  // first token of the tile
+        const int tile_lo = shift + tile_tok, tile_hi = shift + min(lq, tile_tok + p.tokens) - 1;
+        const int tok = tile_tok + r / p.group;
+        const bool live = r < p.tokens * p.group && tok < lq;      // rows behind the tokens of the tile or the sequence hold anything
+        const int pos = min(shift + tok, tile_hi);
+        const uint32_t s_addr = tmem + lane_sel;                   // the S buffer is shared by the two tiles
+        const uint32_t p_addr = tmem + lane_sel + kPwTmemP + g * 64;
+        const uint32_t o_addr = tmem + lane_sel + kPwTmemO + g * 128;
+        float m_ref = -INFINITY, l_run = 0.f;                      // reference maximum (log2 domain), row sum
+        float v_ref = 0.f;                                         // e4m3: V scale that O is expressed in, 0 = none yet
+        float c_row = p.scale_log2;
+        if (FP8 && n_kt > 0) {
+            if (!tc_wait(bar(PW_Q_READY), 0, s_abort, p.wait_limit)) ok = false;
+            c_row *= s_qscale[g * kPwRows + r];
+        }
+
+        for (int j = 0; j < n_kt; ++j) {
+            if (ok && !tc_wait(bar(PW_S_FULL, g), j & 1, s_abort, p.wait_limit)) ok = false;
+            if (!ok) continue;
+            tc_fence_after();
+            const int kb = tile_at(j) * kPwKeys;
+            uint32_t sv[128];                                      // the whole row of S in registers
+            tc_ld32(s_addr, *reinterpret_cast<uint32_t(*)[32]>(&sv[0]));
+            tc_ld32(s_addr + 32, *reinterpret_cast<uint32_t(*)[32]>(&sv[32]));
+            tc_ld32(s_addr + 64, *reinterpret_cast<uint32_t(*)[32]>(&sv[64]));
+            tc_ld32(s_addr + 96, *reinterpret_cast<uint32_t(*)[32]>(&sv[96]));
+            tc_wait_ld();
+            // the row is in registers: the tensor core may overwrite the S buffer
+            tc_fence_before();
+            mbar_arrive(bar(PW_S_FREE));
+            float c_tile = c_row, v_scale = 1.f;
+            if constexpr (FP8) {
+                c_tile *= s_scale[(j % kPwScaleRing) * 2];
+                v_scale = s_scale[(j % kPwScaleRing) * 2 + 1];
+                if (c_tile == 0.f) {                               // a K scale of 0 (or a row of Q): scores of 0
+#pragma unroll
+                    for (int i = 0; i < 128; ++i) sv[i] = 0u;
+                    c_tile = 1.f;
+                }
+            }
+            if (kb + kPwKeys - 1 > tile_lo) {                      // keys behind a row's own position
+                const int limit = pos - kb;                        // columns <= limit are visible
+#pragma unroll
+                for (int i = 0; i < 128; ++i)
+                    if (i > limit) sv[i] = 0xff800000u;            // -inf
+            }
+            if (windowed && kb <= tile_hi - p.window && kb + kPwKeys > sinks) {
+                const int start = pos - p.window + 1 - kb, sink = sinks - kb;     // columns >= start or < sink are visible
+#pragma unroll
+                for (int i = 0; i < 128; ++i)
+                    if (i < start && i >= sink) sv[i] = 0xff800000u;
+            }
+            float mx0 = -INFINITY, mx1 = -INFINITY, mx2 = -INFINITY, mx3 = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 128; i += 8) {
+                mx0 = fmax3(mx0, __uint_as_float(sv[i]), __uint_as_float(sv[i + 1]));
+                mx1 = fmax3(mx1, __uint_as_float(sv[i + 2]), __uint_as_float(sv[i + 3]));
+                mx2 = fmax3(mx2, __uint_as_float(sv[i + 4]), __uint_as_float(sv[i + 5]));
+                mx3 = fmax3(mx3, __uint_as_float(sv[i + 6]), __uint_as_float(sv[i + 7]));
+            }
+            const float mx = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)) * c_tile;    // -inf: this row sees none of the tile
+            // move the reference only when the maximum outgrew it by more than 2^lazy
+            const bool move = mx > m_ref + C::lazy || (m_ref == -INFINITY && mx > -INFINITY);
+            float v_factor = 1.f;                                  // what a larger V scale makes of O
+            if constexpr (FP8) {
+                if (v_ref == 0.f) v_ref = v_scale;                 // O is 0 so far
+                else if (v_scale > 8.f * v_ref) {
+                    v_factor = v_ref / v_scale;
+                    v_ref = v_scale;
+                }
+            }
+            if (__any_sync(0xffffffffu, move || v_factor != 1.f)) {
+                const float m_new = move ? mx : m_ref;
+                const float alpha = m_ref == -INFINITY ? 0.f : fast_exp2(m_ref - m_new);
+                if (j > 0) {
+                    // O holds tiles < j once P V_{j-1} has retired; P V_j cannot start before P_FULL below
+                    if (!tc_wait(bar(PW_PV_DONE, g), (j - 1) & 1, s_abort, p.wait_limit)) { ok = false; continue; }
+                    tc_fence_after();
+                    const float f = alpha * v_factor;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t v[32];
+                        tc_ld32(o_addr + c * 32, v);
+                        tc_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
+                        tc_st32(o_addr + c * 32, v);
+                    }
+                    tc_wait_st();
+                }
+                l_run *= alpha;
+                m_ref = m_new;
+            }
+            float up = m_ref == -INFINITY ? 0.f : -m_ref;          // added to the exponent
+            float down = 1.f;                                      // takes the V scale out of the row sum
+            if constexpr (FP8) {
+                up += C::bias;
+                if (v_scale > 0.f && v_scale != v_ref) {
+                    const float ratio = fmaxf(__fdividef(v_scale, v_ref), 1e-18f);
+                    up += __log2f(ratio);
+                    down = __fdividef(1.f, ratio);
+                }
+            }
+            // the tensor core must be done reading P of the previous key tile (long since, as a rule)
+            if (j > 0 && !tc_wait(bar(PW_PV_DONE, g), (j - 1) & 1, s_abort, p.wait_limit)) { ok = false; continue; }
+            // P = exp2(S * c + up) as packed 16-bit values
+            uint64_t rsa = pk2(0.f, 0.f), rsb = pk2(0.f, 0.f);
+            const uint64_t c2 = pk2(c_tile, c_tile), up2 = pk2(up, up);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                uint32_t pk[32];
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    const int c = h * 64 + 2 * i;
+                    const uint64_t x2 = ffma2(pk2(__uint_as_float(sv[c]), __uint_as_float(sv[c + 1])), c2, up2);
+                    float e0, e1;
+                    upk2(x2, e0, e1);
+                    e0 = fast_exp2(e0);
+                    e1 = fast_exp2(e1);
+                    if (i & 1) rsb = fadd2(rsb, pk2(e0, e1)); else rsa = fadd2(rsa, pk2(e0, e1));
+                    pk[i] = FP8 ? pack_f16(e0, e1) : pack_bf16(e0, e1);
+                }
+                tc_st32(p_addr + h * 32, pk);
+            }
+            float rs0, rs1, rs2, rs3;
+            upk2(rsa, rs0, rs1);
+            upk2(rsb, rs2, rs3);
+            l_run = fmaf((rs0 + rs1) + (rs2 + rs3), down, l_run);
+            tc_wait_st();
+            tc_fence_before();
+            mbar_arrive(bar(PW_P_FULL, g));
+        }
+        // O is complete once the last P V has retired
+        if (n_kt > 0 && ok && !tc_wait(bar(PW_PV_DONE, g), (n_kt - 1) & 1, s_abort, p.wait_limit)) ok = false;
+        if (n_kt > 0 && ok) {
+            tc_fence_after();
+            const float unit = FP8 ? v_ref : 1.f;
+            const float f = p.splits > 1 ? unit : l_run > 0.f ? unit / l_run : 0.f;
+            const bool any = l_run > 0.f;                           // a row that sees nothing gives zeros
+            const int64_t row = int64_t(q0 + tok) * p.n_q_heads + kvh * p.group + r % p.group;
+            const int64_t part = int64_t(split) * p.total_q * p.n_q_heads + row;
+            if (p.splits > 1 && live) reinterpret_cast<float2*>(p.part_ml)[part] = make_float2(any ? m_ref : -INFINITY, l_run);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                uint32_t v[32];
+                tc_ld32(o_addr + c * 32, v);
+                tc_wait_ld();
+                if (!live) continue;
+#pragma unroll
+                for (int i = 0; i < 32; ++i) v[i] = any ? __float_as_uint(__uint_as_float(v[i]) * f) : 0u;
+                if (p.splits > 1) {
+                    uint4* dst = reinterpret_cast<uint4*>(p.part_o + part * kHeadDim + c * 32);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) dst[i] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+                } else {
+                    uint4* dst = reinterpret_cast<uint4*>(p.out + row * kHeadDim + c * 32);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        uint4 w;
+                        w.x = pack_bf16(__uint_as_float(v[8 * i]), __uint_as_float(v[8 * i + 1]));
+                        w.y = pack_bf16(__uint_as_float(v[8 * i + 2]), __uint_as_float(v[8 * i + 3]));
+                        w.z = pack_bf16(__uint_as_float(v[8 * i + 4]), __uint_as_float(v[8 * i + 5]));
+                        w.w = pack_bf16(__uint_as_float(v[8 * i + 6]), __uint_as_float(v[8 * i + 7]));
+                        dst[i] = w;
+                    }
+                }
+            }
+            tc_fence_before();
+        }
+    }
+
+    // ===================================================================== common epilogue
+    tc_fence_before();
+    __syncthreads();
+    if (warp == kPwIssueS) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    }
+    if (threadIdx.x == 0 && *s_abort && p.status) atomicExch(p.status, 0x5AFE0006);
+}
+
+// Joins the parts of every (token, head): a warp per row.  Rows outside of the sequences are left alone.
+__global__ void __launch_bounds__(256) prefill_join_kernel(__nv_bfloat16* out, const float* part_ml, const float* part_o,
+                                                           const int32_t* cu_q, int batch, int64_t rows, int n_q_heads, int splits) {
+    const int64_t row = (int64_t(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
+    const int lane = threadIdx.x & 31;
+    if (row < int64_t(cu_q[0]) * n_q_heads || row >= min(int64_t(cu_q[batch]) * n_q_heads, rows)) return;
+    const float2* ml = reinterpret_cast<const float2*>(part_ml) + row;
+    float m = -INFINITY;
+    for (int s = 0; s < splits; ++s) m = fmaxf(m, ml[s * rows].x);
+    float l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s = 0; s < splits; ++s) {
+        const float2 x = ml[s * rows];
+        if (x.x == -INFINITY) continue;
+        const float a = exp2f(x.x - m);
+        const float4 v = reinterpret_cast<const float4*>(part_o + (s * rows + row) * kHeadDim)[lane];
+        l = fmaf(x.y, a, l);
+        o.x = fmaf(v.x, a, o.x);
+        o.y = fmaf(v.y, a, o.y);
+        o.z = fmaf(v.z, a, o.z);
+        o.w = fmaf(v.w, a, o.w);
+    }
+    const float f = l > 0.f ? 1.f / l : 0.f;
+    uint2 w;
+    w.x = pack_bf16(o.x * f, o.y * f);
+    w.y = pack_bf16(o.z * f, o.w * f);
+    *reinterpret_cast<uint2*>(out + row * kHeadDim + lane * 4) = w;
+}
+
+// Over how many CTAs the key tiles of a row block are spread: as many as keep every SM at one CTA, when a CTA has at
+// least four tiles to give away (one tile costs about 1.5 us, setting a CTA up and joining the parts about 5).
+static int prefill_splits(const infer_kv_pool* pool, int batch, int max_q, int max_k, int n_q_heads, int window, int sinks) {
+    const int group = n_q_heads / pool->n_kv_heads, tokens = kPwRows / group;
+    const int64_t blocks = int64_t((max_q + 2 * tokens - 1) / (2 * tokens)) * pool->n_kv_heads * batch;
+    int64_t tiles = (int64_t(max_k) + kPwKeys - 1) / kPwKeys;
+    if (window > 0) {
+        const int64_t seen = (int64_t(window) + 2 * tokens + kPwKeys - 1) / kPwKeys + 1 + (int64_t(sinks) + kPwKeys - 1) / kPwKeys;
+        if (seen < tiles) tiles = seen;
+    }
+    int64_t splits = blocks > 0 ? pool->sm_count / blocks : 1;
+    if (splits > tiles / 2) splits = tiles / 2;
+    return splits < 1 ? 1 : int(splits);
+}
+
+static size_t prefill_part_bytes(int splits, int64_t rows) { return size_t(splits) * rows * (2 + kHeadDim) * sizeof(float); }
+
+template <bool FP8>
+static int launch_prefill_window(const PwParams& p, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, dim3 grid,
+                                 cudaStream_t st) {
+    const int smem = PwCfg<FP8>::total + 1024;
+    static std::atomic<bool> prepared[64];     // the shared-memory limit is raised once per device
+    int dev = 0;
+    IB_CUDA(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64 || !prepared[dev].load(std::memory_order_acquire)) {
+        IB_CUDA(cudaFuncSetAttribute(prefill_window_kernel<FP8>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        if (dev >= 0 && dev < 64) prepared[dev].store(true, std::memory_order_release);
+    }
+    prefill_window_kernel<FP8><<<grid, PwCfg<FP8>::threads, smem, st>>>(p, mq, mk, mv);
+    return check_launch();
+}
+
+static int paged_prefill_window(const infer_kv_pool_t* pool, void* out, const void* q, int64_t total_q, const int32_t* cu_seqlens_q,
+                                const int32_t* cu_seqlens_k, const int32_t* block_tables, int64_t bt_stride, int batch,
+                                int max_seqlen_q, int max_seqlen_k, int n_q_heads, float softmax_scale, int window, int sinks,
+                                void* workspace, size_t workspace_bytes, cudaStream_t st, uint32_t wait_limit, int stall_producer) {
+    if (!(softmax_scale > 0.f) || !(softmax_scale < INFINITY) || window < 0 || sinks < 0) return INFER_ERR_GEOMETRY;
+    if (!pool || !out || !q || !cu_seqlens_q || !cu_seqlens_k || !block_tables) return INFER_ERR_NULL;
+    if (batch < 0 || n_q_heads <= 0 || n_q_heads % pool->n_kv_heads != 0 || n_q_heads / pool->n_kv_heads > kPwRows || bt_stride <= 0 ||
+        max_seqlen_q < 0 || max_seqlen_k < 0 || batch > 65535 || n_q_heads > 65535 || total_q < 0 ||
+        total_q > int64_t(batch) * max_seqlen_q || total_q >= (int64_t(1) << 31))
+        return INFER_ERR_GEOMETRY;
+    if (!aligned16(out) || !aligned16(q)) return INFER_ERR_ALIGN;
+    if (workspace && !aligned16(workspace)) return INFER_ERR_WORKSPACE;
+    if (total_q == 0 || batch == 0) return INFER_OK;
+    const int64_t rows = total_q * n_q_heads;
+    int splits = prefill_splits(pool, batch, max_seqlen_q, max_seqlen_k, n_q_heads, window, sinks);
+    while (splits > 1 && (!workspace || prefill_part_bytes(splits, rows) > workspace_bytes)) --splits;
+    PwParams p{};
+    p.out = static_cast<__nv_bfloat16*>(out);
+    p.cu_q = cu_seqlens_q;
+    p.cu_k = cu_seqlens_k;
+    p.block_tables = block_tables;
+    p.bt_stride = bt_stride;
+    p.k_scale = pool->k_scale;
+    p.v_scale = pool->v_scale;
+    p.n_q_heads = n_q_heads;
+    p.n_kv_heads = pool->n_kv_heads;
+    p.group = n_q_heads / pool->n_kv_heads;
+    p.tokens = kPwRows / p.group;
+    p.block_size = pool->block_size;
+    p.num_blocks = int(pool->num_blocks);
+    p.window = window > 0 ? window : 0x7fffffff;
+    p.sinks = sinks;
+    p.scale_log2 = softmax_scale * 1.4426950408889634f;
+    p.splits = splits;
+    p.total_q = total_q;
+    if (splits > 1) {
+        p.part_o = static_cast<float*>(workspace);
+        p.part_ml = p.part_o + size_t(splits) * rows * kHeadDim;
+    }
+    p.status = prefill_status_word();
+    p.wait_limit = wait_limit;
+    p.stall_producer = stall_producer;
+    CUtensorMap mq;   // q [total_q, Hq, 128]: a box is one kv head's query heads of `tokens` tokens; zeros past total_q
+    int rc = encode_map_3d(&mq, q, 2, kHeadDim, uint64_t(n_q_heads), uint64_t(total_q), 256, uint64_t(n_q_heads) * 256, 64,
+                           uint32_t(p.group), uint32_t(p.tokens));
+    if (rc != INFER_OK) return rc;
+    const dim3 grid((max_seqlen_q + 2 * p.tokens - 1) / (2 * p.tokens), pool->n_kv_heads * splits, batch);
+    if (pool->dtype == INFER_KV_E4M3) rc = launch_prefill_window<true>(p, mq, pool->maps[3].k, pool->maps[3].v, grid, st);
+    else rc = launch_prefill_window<false>(p, mq, pool->maps[3].k, pool->maps[3].v, grid, st);
+    if (rc != INFER_OK || splits == 1) return rc;
+    prefill_join_kernel<<<unsigned((rows + 7) / 8), 256, 0, st>>>(p.out, p.part_ml, p.part_o, cu_seqlens_q, batch, rows, n_q_heads,
+                                                                  splits);
+    return check_launch();
+}
+
+}  // namespace ib
+
+extern "C" {
+
+size_t infer_paged_prefill_window_workspace_bytes(const infer_kv_pool_t* pool, int64_t total_q, int batch, int max_seqlen_q,
+                                                  int max_seqlen_k, int n_q_heads, int window, int sinks) {
+    if (!pool || total_q <= 0 || batch <= 0 || n_q_heads <= 0 || n_q_heads % pool->n_kv_heads != 0 ||
+        n_q_heads / pool->n_kv_heads > ib::kPwRows || max_seqlen_q < 0 || max_seqlen_k < 0 || window < 0 || sinks < 0)
+        return 0;
+    const int splits = ib::prefill_splits(pool, batch, max_seqlen_q, max_seqlen_k, n_q_heads, window, sinks);
+    return splits > 1 ? ib::prefill_part_bytes(splits, total_q * n_q_heads) : 0;
+}
+
+int infer_paged_prefill_window(const infer_kv_pool_t* pool, void* out, const void* q, int64_t total_q, const int32_t* cu_seqlens_q,
+                               const int32_t* cu_seqlens_k, const int32_t* block_tables, int64_t bt_stride, int batch,
+                               int max_seqlen_q, int max_seqlen_k, int n_q_heads, float softmax_scale, int window, int sinks,
+                               void* workspace, size_t workspace_bytes, void* stream_) {
+    return ib::paged_prefill_window(pool, out, q, total_q, cu_seqlens_q, cu_seqlens_k, block_tables, bt_stride, batch, max_seqlen_q,
+                                    max_seqlen_k, n_q_heads, softmax_scale, window, sinks, workspace, workspace_bytes,
+                                    static_cast<cudaStream_t>(stream_), ib::kDefaultWaitLimit, 0);
+}
+
+int infer_selftest_paged_prefill_window(const infer_kv_pool_t* pool, void* out, const void* q, int64_t total_q,
+                                        const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, const int32_t* block_tables,
+                                        int64_t bt_stride, int batch, int max_seqlen_q, int max_seqlen_k, int n_q_heads,
+                                        float softmax_scale, int window, int sinks, void* workspace, size_t workspace_bytes,
+                                        void* stream_, uint32_t wait_limit, int stall_producer) {
+    return ib::paged_prefill_window(pool, out, q, total_q, cu_seqlens_q, cu_seqlens_k, block_tables, bt_stride, batch, max_seqlen_q,
+                                    max_seqlen_k, n_q_heads, softmax_scale, window, sinks, workspace, workspace_bytes,
+                                    static_cast<cudaStream_t>(stream_), wait_limit ? wait_limit : ib::kDefaultWaitLimit, stall_producer);
+}
+
+}  // extern "C"

@@ -49,7 +49,7 @@ class _on_device:
             self.guard.__exit__(*exc)
 
 
-# The three attention entry points are reached through these one-line functions so that the test
+# The attention entry points are reached through these one-line functions so that the test
 # suite can route a call to the library's self-test entry points (infer_b200/selftest.py).
 def _call_decode(lib, *args):
     return lib.infer_paged_decode(*args)
@@ -57,6 +57,10 @@ def _call_decode(lib, *args):
 
 def _call_prefill(lib, *args):
     return lib.infer_paged_prefill(*args)
+
+
+def _call_prefill_window(lib, *args):
+    return lib.infer_paged_prefill_window(*args)
 
 
 def _call_dense(lib, *args):
@@ -440,25 +444,52 @@ def paged_attn_decode_append(q, key, value, k_cache, v_cache, cache_seqlens, blo
 
 # --------------------------------------------------------------------------- prefill
 def paged_attn_prefill(q, k_cache, v_cache, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k,
-                       softmax_scale, block_table, out=None):
+                       softmax_scale, block_table, out=None, k_scale=None, v_scale=None, window=None, sinks=0, workspace=None):
     """q [total_q, Hq, 128]; keys come from the pools through block_table; causal,
-    bottom-right aligned (the flash_attn_varlen_func convention)."""
+    bottom-right aligned (the flash_attn_varlen_func convention).
+
+    e4m3 pools come with their ``k_scale`` / ``v_scale``.  ``window`` / ``sinks``: a query sees the ``window`` keys up to its
+    own position and the first ``sinks`` of its sequence; entries of ``block_table`` for pages without a visible key are not
+    read.  With either, a query that sees no key gives zeros.  ``workspace``: uint8 scratch for chunks of few rows over many
+    keys (see ``infer_paged_prefill_window``); by default it comes from the allocator of the current stream, call by call."""
     if q.dtype != torch.bfloat16 or not q.is_contiguous() or q.dim() != 3:
         raise RuntimeError("paged_attn_prefill: q must be contiguous bf16 [total_q, Hq, 128]")
     for name, t in (("cu_seqlens_q", cu_seqlens_q), ("cu_seqlens_k", cu_seqlens_k), ("block_table", block_table)):
         if t.dtype != torch.int32 or not t.is_cuda:
             raise RuntimeError(f"paged_attn_prefill: {name} must be an int32 CUDA tensor")
-    pool = pool_of(k_cache, v_cache)
+    window, sinks = _window("paged_attn_prefill", window, sinks)
+    pool = pool_of(k_cache, v_cache, k_scale, v_scale)
     o = torch.empty_like(q) if out is None else out
     lib = _lib.load()
+    batch, args = cu_seqlens_q.numel() - 1, ()
+    if pool.fp8 or window:
+        _check_prefill_window(q, o, cu_seqlens_q, cu_seqlens_k, block_table, batch, pool)
+        need = lib.infer_paged_prefill_window_workspace_bytes(pool.handle, q.shape[0], batch, int(max_seqlen_q), int(max_seqlen_k),
+                                                              q.shape[1], window, sinks)
+        if workspace is None and need:
+            workspace = torch.empty(need, dtype=torch.uint8, device=pool.device)
+        args = (window, sinks, _ptr(workspace), workspace.numel() if workspace is not None else 0)
     with _on_device(pool.device):
-        rc = _call_prefill(lib, pool.handle, _ptr(o), _ptr(q), q.shape[0], _ptr(cu_seqlens_q), _ptr(cu_seqlens_k),
-                                     _ptr(block_table), block_table.stride(0), cu_seqlens_q.numel() - 1,
-                                     int(max_seqlen_q), int(max_seqlen_k), q.shape[1], float(softmax_scale),
-                                     _stream())
+        rc = (_call_prefill_window if args else _call_prefill)(
+            lib, pool.handle, _ptr(o), _ptr(q), q.shape[0], _ptr(cu_seqlens_q), _ptr(cu_seqlens_k), _ptr(block_table),
+            block_table.stride(0), batch, int(max_seqlen_q), int(max_seqlen_k), q.shape[1], float(softmax_scale), *args, _stream())
         _lib.check(rc, "paged_attn_prefill")
         _check_prefill_status(lib, "paged_attn_prefill")
     return o
+
+
+def _check_prefill_window(q, out, cu_seqlens_q, cu_seqlens_k, block_table, batch, pool):
+    """What the windowed and the e4m3 form check beyond the plain one."""
+    for name, t in (("q", q), ("out", out), ("cu_seqlens_q", cu_seqlens_q), ("cu_seqlens_k", cu_seqlens_k),
+                    ("block_table", block_table)):
+        if t.device != pool.device:
+            raise RuntimeError(f"paged_attn_prefill: {name} must be on the pools' device")
+    if q.shape[2] != 128 or out.shape != q.shape or out.dtype != torch.bfloat16 or not out.is_contiguous():
+        raise RuntimeError("paged_attn_prefill: out must be contiguous bf16 in the shape of q, [total_q, Hq, 128]")
+    if cu_seqlens_k.numel() != batch + 1 or not cu_seqlens_q.is_contiguous() or not cu_seqlens_k.is_contiguous():
+        raise RuntimeError("paged_attn_prefill: cu_seqlens_q and cu_seqlens_k must be contiguous, batch + 1 values each")
+    if block_table.dim() != 2 or block_table.shape[0] < batch or block_table.stride(1) != 1:
+        raise RuntimeError("paged_attn_prefill: block_table must have a row of contiguous entries per sequence")
 
 
 def _check_prefill_status(lib, what):
