@@ -16,15 +16,19 @@
 //   are cleared before the tensor core reads them: P is 0 there, but 0 times a stale NaN is not.
 // Few rows.  When the (row block, kv head, sequence) triples do not fill the GPU, the key tiles of a CTA are split over
 //   several, each leaving maximum, sum and accumulator per row in 32 bits, and a second kernel joins them.
-// e4m3.  TMA brings the raw bytes (16 KiB per tile, half of bf16's traffic) into two staging slots and a fourth warpgroup
-//   turns them into f16 operand tiles (e4m3 -> f16 is exact, one conversion instruction per two values, next to softmax
-//   warps that leave more than half of the issue slots idle).  Q is brought to f16 in place, each row scaled by a power of
-//   two that puts its largest value into [1, 2): exact but for values 2^-14 below it.  The K scale of a tile's page and
-//   the row's power of two go into the factor of the softmax exponent.  The V scale goes into P: P = 2^(x - m) * 2^kBias *
-//   v_scale / v_ref, where v_ref is the largest V scale met so far within a factor of 8; the row sum takes it out again
-//   with one multiplication per tile, the output multiplies by v_ref.  P in f16 then lies below 2^(6 + 6 + 3) and keeps 11
-//   bits down to 2^-14 - 6 of the row's maximum, where bf16 would keep 8.  A page whose V scale is 2^-20 of v_ref or less
-//   loses bits of its values, which is an error of 2^-33 v_ref.
+// e4m3.  S = Q K^T runs on the raw bytes of K (kind::f8f6f4, no conversion): a bf16 value has 8 significant bits, so it is
+//   the exact sum of two e4m3 values, its rounding to 4 bits and the rest.  A warpgroup of converters splits Q once per CTA,
+//   each row scaled by a power of two that puts its largest value into [2^7, 2^8); values 2^-10 below that lose bits of the
+//   second part, an error of 2^-18 of the row's largest.  Two e4m3 products take the tensor core as long as one bf16
+//   product.  P has to keep more bits than that, so V becomes f16: TMA brings its bytes (half of bf16's traffic) into two
+//   staging slots and the converters turn them into operand tiles (e4m3 -> f16 is exact).  When K was converted as well the
+//   kernel was 1.2-1.5 times slower than on a bf16 cache: the S products alone read shared memory at its full rate (128
+//   bytes a clock), and every converted tile moves another 48 KiB through it.
+//   The K scale of a tile's page and the row's power of two go into the factor of the softmax exponent.  The V scale goes
+//   into P: P = 2^(x - m) * 2^bias * v_scale / v_ref, where v_ref is the largest V scale met so far within a factor of 8;
+//   the row sum takes it out again with one multiplication per tile, the output multiplies by v_ref.  P in f16 then lies
+//   below 2^(6 + 6 + 3) and keeps 11 bits down to 2^-20 of the row's maximum, where bf16 would keep 8.  A page whose V scale
+//   is 2^-20 of v_ref or less loses bits of its values, which is an error of 2^-33 v_ref.
 //
 // Every wait is bounded; one that runs out raises the abort flag, every role drains to the common epilogue, tensor memory
 // is freed and the status word of the prefill kernels is set.
@@ -40,7 +44,7 @@ constexpr int kPwKeys = 128;                  // keys per K/V tile
 constexpr int kPwHalf = 128 * 128;            // bytes of one [128 rows][64 elems] swizzled sub-tile
 constexpr int kPwTile = 2 * kPwHalf;          // 32 KiB: one Q, K or V tile of 16-bit elements
 constexpr int kPwRaw = 128 * 128;             // 16 KiB: one K or V tile of e4m3 bytes
-constexpr int kPwScaleRing = 8;               // a tile's scales stay here from its K's load to its softmax: at most 6 tiles
+constexpr int kPwRing = 8;                    // a tile's first key and scales stay here from its K's load to its softmax: 6 tiles at most
 // tensor memory columns: S (shared by the two tiles) at 0, P of tile i at 128 + 64 i, O of tile i at 256 + 128 i
 constexpr uint32_t kPwTmemP = 128, kPwTmemO = 256;
 constexpr int kPwSoftmaxWarps = 8;
@@ -48,24 +52,25 @@ constexpr int kPwProducer = 8, kPwIssueS = 9, kPwIssuePV = 10;   // warp roles; 
 
 template <bool FP8>
 struct PwCfg {
-    static constexpr int k_stages = FP8 ? 2 : 3, v_stages = 2, raw_slots = FP8 ? 2 : 0;
+    static constexpr int k_stages = FP8 ? 4 : 3, v_stages = 2, raw_slots = FP8 ? 2 : 0;
+    static constexpr int k_bytes = FP8 ? kPwRaw : kPwTile;            // of a stage
     static constexpr int threads = (kPwSoftmaxWarps + (FP8 ? 8 : 4)) * 32;
     static constexpr int q = 0;
     static constexpr int k = q + 2 * kPwTile;
-    static constexpr int v = k + k_stages * kPwTile;
+    static constexpr int v = k + k_stages * k_bytes;
     static constexpr int raw = v + v_stages * kPwTile;
     static constexpr int bars = raw + raw_slots * kPwRaw;
-    static constexpr int n_bars = 26;
+    static constexpr int n_bars = 28;
     static constexpr int misc = bars + n_bars * 8;                    // tmem base, abort flag
-    static constexpr int scales = misc + 16;                          // [kPwScaleRing] (k scale, v scale)
-    static constexpr int qscale = scales + (FP8 ? kPwScaleRing * 8 : 0);    // [2][128] power of two taken out of a Q row
+    static constexpr int ring = misc + 16;                            // [kPwRing] first key of a tile, its k scale, its v scale
+    static constexpr int qscale = ring + kPwRing * 16;                // [2][128] power of two taken out of a Q row
     static constexpr int total = qscale + (FP8 ? 2 * kPwRows * 4 : 0);
     // the probabilities' exponent: how far the reference maximum may lag, and what is added to it
     static constexpr float lazy = FP8 ? 6.f : 8.f, bias = FP8 ? 6.f : 0.f;
 };
 
-enum PwBar { PW_Q_FULL = 0, PW_K_FULL = 1, PW_K_EMPTY = 4, PW_V_FULL = 7, PW_V_EMPTY = 9, PW_S_FULL = 11, PW_P_FULL = 13,
-             PW_PV_DONE = 15, PW_DRAIN = 17, PW_S_FREE = 19, PW_RAW_FULL = 20, PW_RAW_EMPTY = 22, PW_Q_READY = 24 };
+enum PwBar { PW_Q_FULL = 0, PW_K_FULL = 1, PW_K_EMPTY = 5, PW_V_FULL = 9, PW_V_EMPTY = 11, PW_S_FULL = 13, PW_P_FULL = 15,
+             PW_PV_DONE = 17, PW_DRAIN = 19, PW_S_FREE = 21, PW_RAW_FULL = 22, PW_RAW_EMPTY = 24, PW_Q_READY = 26 };
 
 struct PwParams {
     __nv_bfloat16* out;
@@ -99,7 +104,7 @@ __global__ void __launch_bounds__(PwCfg<FP8>::threads, 1) prefill_window_kernel(
     const uint32_t base = smem_u32(smem);
     volatile uint32_t* s_tmem = reinterpret_cast<volatile uint32_t*>(smem + C::misc);
     volatile int* s_abort = reinterpret_cast<volatile int*>(smem + C::misc + 4);
-    volatile float* s_scale = reinterpret_cast<volatile float*>(smem + C::scales);
+    volatile int* s_ring = reinterpret_cast<volatile int*>(smem + C::ring);
     volatile float* s_qscale = reinterpret_cast<volatile float*>(smem + C::qscale);
     auto bar = [&](int which, int idx = 0) { return base + uint32_t(C::bars) + uint32_t(which + idx) * 8; };
 
@@ -147,7 +152,7 @@ __global__ void __launch_bounds__(PwCfg<FP8>::threads, 1) prefill_window_kernel(
         mbar_init(bar(PW_Q_FULL), 1);
         mbar_init(bar(PW_Q_READY), 4);
         for (int i = 0; i < C::k_stages; ++i) {
-            mbar_init(bar(PW_K_FULL, i), FP8 ? 4 : 1);
+            mbar_init(bar(PW_K_FULL, i), 1);
             mbar_init(bar(PW_K_EMPTY, i), 1);
         }
         for (int i = 0; i < 2; ++i) {
@@ -184,11 +189,11 @@ __global__ void __launch_bounds__(PwCfg<FP8>::threads, 1) prefill_window_kernel(
         end = pos_hi + 1 - kb;
     };
 
-    // Register budget.  bf16: 384 threads x 168 at launch, the third warpgroup hands 64 per thread to the softmax
-    // warpgroups.  e4m3: 512 threads x 128, roles and converters keep 56.  Both end at 200 per softmax thread.
+    // Register budget.  bf16: 384 threads x 168 at launch = 72 for the third warpgroup and 216 for the softmax ones.
+    // e4m3: 512 x 128 = 48 for roles and converters, 208 for softmax.
     if (hw < 4) {
-        if constexpr (FP8) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;" ::: "memory");
-        else asm volatile("setmaxnreg.dec.sync.aligned.u32 104;" ::: "memory");
+        if constexpr (FP8) asm volatile("setmaxnreg.dec.sync.aligned.u32 48;" ::: "memory");
+        else asm volatile("setmaxnreg.dec.sync.aligned.u32 72;" ::: "memory");
         if (warp == kPwProducer) {
             // ============================================================= TMA producer
             if (lane == 0 && !p.stall_producer) {
@@ -210,35 +215,50 @@ __global__ void __launch_bounds__(PwCfg<FP8>::threads, 1) prefill_window_kernel(
                 auto slot_of = [&](int tile, int page) {
                     return page >= 0 && page < p.num_blocks ? page * p.block_size + tile * kPwKeys % p.block_size : -kPwKeys;
                 };
+                // read by the softmax warps (and the converters) of tile j: released by the arrival that K's copy is armed with
+                auto put_ring = [&](int j, int key0, float ks, float vs) {
+                    volatile int* e = s_ring + (j % kPwRing) * 4;
+                    e[0] = key0;
+                    e[1] = __float_as_int(ks);
+                    e[2] = __float_as_int(vs);
+                };
                 if constexpr (FP8) {
                     // order K0, K1, V0, K2, V1, ...: K of the next tile is needed before V of this one
-                    int issued = 0;
-                    auto load_raw = [&](const CUtensorMap* map, int slot) {
-                        const int s = issued & 1;
-                        if (!tc_wait(bar(PW_RAW_EMPTY, s), ((issued >> 1) & 1) ^ 1, s_abort, p.wait_limit)) { ok = false; return; }
-                        mbar_expect_tx(bar(PW_RAW_FULL, s), kPwRaw);
-                        tma_load_3d(base + C::raw + s * kPwRaw, map, bar(PW_RAW_FULL, s), 0, kvh, slot);
-                        ++issued;
+                    auto load_raw = [&](const CUtensorMap* map, uint32_t dst, uint32_t full, int slot) {
+                        mbar_expect_tx(full, kPwRaw);
+                        tma_load_3d(dst, map, full, 0, kvh, slot);
                     };
                     int page = page_of(tile_at(0)), v_slot = 0;      // page of tile j, looked up one tile ahead
+                    int k_issued = 0, v_issued = 0;
                     for (int j = 0; j <= n && ok; ++j) {
                         int k_slot = 0;
                         if (j < n) {
                             const bool in = page >= 0 && page < p.num_blocks;
                             const float ks = in ? p.k_scale[int64_t(page) * p.n_kv_heads + kvh] : 0.f;
                             const float vs = in ? p.v_scale[int64_t(page) * p.n_kv_heads + kvh] : 0.f;
+                            const int s = j % C::k_stages;
                             k_slot = slot_of(tile_at(j), page);
                             if (j + 1 < n) page = page_of(tile_at(j + 1));
-                            s_scale[(j % kPwScaleRing) * 2] = ks;     // released by the arrival on RAW_FULL
-                            s_scale[(j % kPwScaleRing) * 2 + 1] = vs;
-                            load_raw(&map_k, k_slot);
+                            put_ring(j, tile_at(j) * kPwKeys, ks, vs);
+                            if (tc_wait(bar(PW_K_EMPTY, s), ((j / C::k_stages) & 1) ^ 1, s_abort, p.wait_limit)) {
+                                load_raw(&map_k, base + C::k + s * kPwRaw, bar(PW_K_FULL, s), k_slot);
+                                ++k_issued;
+                            } else ok = false;
                         }
-                        if (j >= 1 && ok) load_raw(&map_v, v_slot);
+                        if (j >= 1 && ok) {
+                            const int jv = j - 1, s = jv & 1;
+                            if (tc_wait(bar(PW_RAW_EMPTY, s), ((jv >> 1) & 1) ^ 1, s_abort, p.wait_limit)) {
+                                load_raw(&map_v, base + C::raw + s * kPwRaw, bar(PW_RAW_FULL, s), v_slot);
+                                ++v_issued;
+                            } else ok = false;
+                        }
                         v_slot = k_slot;
                     }
                     // never leave with a copy in flight: wait (bounded) for everything that was armed
                     mbar_wait(bar(PW_Q_FULL), 0, p.wait_limit);
-                    for (int i = max(0, issued - 2); i < issued; ++i) mbar_wait(bar(PW_RAW_FULL, i & 1), (i >> 1) & 1, p.wait_limit);
+                    for (int j = max(0, k_issued - C::k_stages); j < k_issued; ++j)
+                        mbar_wait(bar(PW_K_FULL, j % C::k_stages), (j / C::k_stages) & 1, p.wait_limit);
+                    for (int j = max(0, v_issued - 2); j < v_issued; ++j) mbar_wait(bar(PW_RAW_FULL, j & 1), (j >> 1) & 1, p.wait_limit);
                 } else {
                     auto load_tile = [&](const CUtensorMap* map, uint32_t dst, uint32_t full, int slot) {
                         mbar_expect_tx(full, kPwTile);
@@ -251,6 +271,7 @@ __global__ void __launch_bounds__(PwCfg<FP8>::threads, 1) prefill_window_kernel(
                         if (j < n) {
                             const int s = j % C::k_stages, tile = tile_at(j);
                             k_slot = slot_of(tile, page_of(tile));
+                            put_ring(j, tile * kPwKeys, 1.f, 1.f);
                             if (tc_wait(bar(PW_K_EMPTY, s), ((j / C::k_stages) & 1) ^ 1, s_abort, p.wait_limit)) {
                                 load_tile(&map_k, base + C::k + s * kPwTile, bar(PW_K_FULL, s), k_slot);
                                 ++k_issued;
@@ -283,11 +304,13 @@ __global__ void __launch_bounds__(PwCfg<FP8>::threads, 1) prefill_window_kernel(
                 tc_fence_after();
                 if (elect_one()) {
                     const uint64_t qd = q_desc0 + uint64_t(i * (kPwTile >> 4));
-                    const uint64_t kd = k_desc0 + uint64_t(stage * (kPwTile >> 4));
+                    const uint64_t kd = k_desc0 + uint64_t(stage * (C::k_bytes >> 4));
 #pragma unroll
                     for (int kk = 0; kk < 8; ++kk) {
                         const uint32_t off = ((kk >> 2) * kPwHalf + (kk & 3) * 32) >> 4;
-                        tc_mma(tmem, qd + off, kd + off, idesc_s, kk > 0);
+                        // e4m3: the two parts of Q lie where bf16 has the two halves of the dims, K is the same for both
+                        if constexpr (FP8) tc_mma_f8(tmem, qd + off, kd + ((kk & 3) * 32 >> 4), idesc_s, kk > 0);
+                        else tc_mma(tmem, qd + off, kd + off, idesc_s, kk > 0);
                     }
                     tc_commit(bar(PW_S_FULL, i));
                 }
@@ -358,50 +381,82 @@ __global__ void __launch_bounds__(PwCfg<FP8>::threads, 1) prefill_window_kernel(
     } else if (FP8 && hw >= 12) {
         // ================================================================= converters: e4m3 bytes -> f16 operand tiles
         if constexpr (FP8) {
-            asm volatile("setmaxnreg.dec.sync.aligned.u32 56;" ::: "memory");
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 48;" ::: "memory");
             const int t = int(threadIdx.x) - 12 * 32;                         // 0 .. 127
             if (!tc_wait(bar(PW_Q_FULL), 0, s_abort, p.wait_limit)) ok = false;
             if (ok) {
-                // Q in place, one row per thread; the sixteen 16-byte chunks of a row lie at different banks for the
-                // eight rows of a phase
+                // Q in place, one row per thread: chunk x (of 16) holds eight bf16; result c (of 8) is the first parts of
+                // chunks 2c and 2c + 1, stored over chunk c, and their second parts, stored over chunk 8 + c.  Chunks that a
+                // store covers before their turn are read ahead.  A thread alone touches its row; the eight rows of a phase
+                // have a chunk at eight different banks.
+#pragma unroll 1
                 for (int i = 0; i < (two ? 2 : 1); ++i) {
                     const uint32_t row = base + C::q + i * kPwTile;
+                    auto chunk = [&](int x) { return row + (x >> 3) * kPwHalf + swz128(t, x & 7); };
                     uint32_t top = 0;                                         // largest magnitude, as bf16 bits
-                    for (int c = 0; c < 16; ++c) {
-                        const uint4 w = ld_shared_v4(row + (c >> 3) * kPwHalf + swz128(t, c & 7));
+#pragma unroll 2
+                    for (int x = 0; x < 16; ++x) {
+                        const uint4 w = ld_shared_v4(chunk(x));
                         const uint32_t v[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
                         for (int k = 0; k < 4; ++k) top = max(top, max(v[k] & 0x7fffu, (v[k] >> 16) & 0x7fffu));
                     }
-                    const int e = min(max(int(top >> 7) - 127, -126), 126);
+                    const int e = min(max(int(top >> 7) - 127 - 7, -126), 126);
                     const float down = __uint_as_float(uint32_t(127 - e) << 23);
-                    s_qscale[i * kPwRows + t] = __uint_as_float(uint32_t(127 + e) << 23);
-                    for (int c = 0; c < 16; ++c) {
-                        const uint32_t at = row + (c >> 3) * kPwHalf + swz128(t, c & 7);
-                        uint4 w = ld_shared_v4(at);
-                        uint32_t* v = reinterpret_cast<uint32_t*>(&w);
+                    // (a row that holds an infinity or a NaN gives NaN)
+                    s_qscale[i * kPwRows + t] = __uint_as_float(top < 0x7f80u ? uint32_t(127 + e) << 23 : 0x7fffffffu);
+                    auto split8 = [&](const uint4& w, uint32_t& h0, uint32_t& h1, uint32_t& l0, uint32_t& l1) {
+                        const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+                        uint32_t h[4], l[4];
 #pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            v[k] = pack_f16(__uint_as_float(v[k] << 16) * down, __uint_as_float(v[k] & 0xffff0000u) * down);
-                        st_shared_v4(at, w);
+                        for (int k = 0; k < 4; ++k) {
+                            const float2 f = make_float2(__uint_as_float(v[k] << 16) * down, __uint_as_float(v[k] & 0xffff0000u) * down);
+                            h[k] = __nv_cvt_float2_to_fp8x2(f, __NV_SATFINITE, __NV_E4M3);
+                            const uint32_t back = e4m3x2_to_f16x2(h[k]);
+                            const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&back));
+                            l[k] = __nv_cvt_float2_to_fp8x2(make_float2(f.x - y.x, f.y - y.y), __NV_SATFINITE, __NV_E4M3);
+                        }
+                        h0 = h[0] | h[1] << 16;
+                        h1 = h[2] | h[3] << 16;
+                        l0 = l[0] | l[1] << 16;
+                        l1 = l[2] | l[3] << 16;
+                    };
+                    auto result = [&](int c, const uint4& wa, const uint4& wb) {
+                        uint4 h, l;
+                        split8(wa, h.x, h.y, l.x, l.y);
+                        split8(wb, h.z, h.w, l.z, l.w);
+                        st_shared_v4(chunk(c), h);
+                        st_shared_v4(chunk(8 + c), l);
+                    };
+                    const uint4 w8 = ld_shared_v4(chunk(8)), w9 = ld_shared_v4(chunk(9));
+                    const uint4 w10 = ld_shared_v4(chunk(10)), w11 = ld_shared_v4(chunk(11));
+#pragma unroll 1
+                    for (int c = 0; c < 4; ++c) {
+                        const uint4 wa = ld_shared_v4(chunk(2 * c)), wb = ld_shared_v4(chunk(2 * c + 1));
+                        result(c, wa, wb);
                     }
+                    const uint4 w12 = ld_shared_v4(chunk(12)), w13 = ld_shared_v4(chunk(13));
+                    result(4, w8, w9);
+                    result(5, w10, w11);
+                    const uint4 w14 = ld_shared_v4(chunk(14)), w15 = ld_shared_v4(chunk(15));
+                    result(6, w12, w13);
+                    result(7, w14, w15);
                 }
                 fence_proxy_async();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar(PW_Q_READY));
             }
-            // one raw tile after the other, in the order of the producer
-            int seq = 0;
-            auto convert = [&](uint32_t dst, uint32_t full, bool is_v, int j) {
-                const int s = seq & 1;
-                if (!tc_wait(bar(PW_RAW_FULL, s), (seq >> 1) & 1, s_abort, p.wait_limit)) { ok = false; return; }
-                ++seq;
-                int sink_end = kPwKeys, begin = 0, end = kPwKeys;
-                if (is_v) {
-                    seen_rows(tile_at(j), sink_end, begin, end);
-                    if (s_scale[(j % kPwScaleRing) * 2 + 1] == 0.f) sink_end = 0, end = 0;     // a scale of 0: values of 0
+            for (int j = 0; j < n && ok; ++j) {
+                const int s = j & 1;
+                if (!tc_wait(bar(PW_RAW_FULL, s), (j >> 1) & 1, s_abort, p.wait_limit) ||
+                    !tc_wait(bar(PW_V_EMPTY, s), ((j >> 1) & 1) ^ 1, s_abort, p.wait_limit)) {
+                    ok = false;
+                    break;
                 }
-                const uint32_t src = base + C::raw + s * kPwRaw;
+                int sink_end, begin, end;
+                seen_rows(tile_at(j), sink_end, begin, end);
+                if (__int_as_float(s_ring[(j % kPwRing) * 4 + 2]) == 0.f) sink_end = 0, end = 0;       // a scale of 0: values of 0
+                const uint32_t src = base + C::raw + s * kPwRaw, dst = base + C::v + s * kPwTile;
                 const int c = t & 7;
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
@@ -411,7 +466,7 @@ __global__ void __launch_bounds__(PwCfg<FP8>::threads, 1) prefill_window_kernel(
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const int r = (h * 4 + i) * 16 + (t >> 3);
-                        if (is_v && !(r < sink_end || (r >= begin && r < end))) w[i] = make_uint4(0, 0, 0, 0);
+                        if (!(r < sink_end || (r >= begin && r < end))) w[i] = make_uint4(0, 0, 0, 0);
                         uint4 lo, hi;
                         e4m3x4_to_f16x2x2(w[i].x, lo.x, lo.y);
                         e4m3x4_to_f16x2x2(w[i].y, lo.z, lo.w);
@@ -428,37 +483,24 @@ __global__ void __launch_bounds__(PwCfg<FP8>::threads, 1) prefill_window_kernel(
                 fence_proxy_async();
                 __syncwarp();
                 if (lane == 0) {
-                    mbar_arrive(full);
+                    mbar_arrive(bar(PW_V_FULL, s));
                     mbar_arrive(bar(PW_RAW_EMPTY, s));
-                }
-            };
-            for (int j = 0; j <= n && ok; ++j) {
-                if (j < n) {
-                    const int s = j & 1;
-                    if (tc_wait(bar(PW_K_EMPTY, s), ((j >> 1) & 1) ^ 1, s_abort, p.wait_limit))
-                        convert(base + C::k + s * kPwTile, bar(PW_K_FULL, s), false, j);
-                    else ok = false;
-                }
-                if (j >= 1 && ok) {
-                    const int jv = j - 1, s = jv & 1;
-                    if (tc_wait(bar(PW_V_EMPTY, s), ((jv >> 1) & 1) ^ 1, s_abort, p.wait_limit))
-                        convert(base + C::v + s * kPwTile, bar(PW_V_FULL, s), true, jv);
-                    else ok = false;
                 }
             }
         }
     } else {
         // ================================================================= softmax, one row per thread
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 200;" ::: "memory");
+        if constexpr (FP8) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;" ::: "memory");
+        else asm volatile("setmaxnreg.inc.sync.aligned.u32 216;" ::: "memory");
         const int g = warp >> 2;                                   // query tile of this warpgroup
         const int r = (warp & 3) * 32 + lane;                      // row in the tile == TMEM lane
         const uint32_t lane_sel = uint32_t((warp & 3) * 32) << 16;
         const int n_kt = g == 0 || two ? n : 0;
         const int tile_tok = tok0 + g * p.tokens;                  // first token of the tile
-        const int tile_lo = shift + tile_tok, tile_hi = shift + min(lq, tile_tok + p.tokens) - 1;
         const int tok = tile_tok + r / p.group;
         const bool live = r < p.tokens * p.group && tok < lq;      // rows behind the tokens of the tile or the sequence hold anything
-        const int pos = min(shift + tok, tile_hi);
+        const int pos = shift + min(tok, min(lq, tile_tok + p.tokens) - 1);
+        const int start = windowed ? pos - p.window + 1 : -0x40000000;      // first key of the row's window
         const uint32_t s_addr = tmem + lane_sel;                   // the S buffer is shared by the two tiles
         const uint32_t p_addr = tmem + lane_sel + kPwTmemP + g * 64;
         const uint32_t o_addr = tmem + lane_sel + kPwTmemO + g * 128;
@@ -474,7 +516,6 @@ __global__ void __launch_bounds__(PwCfg<FP8>::threads, 1) prefill_window_kernel(
             if (ok && !tc_wait(bar(PW_S_FULL, g), j & 1, s_abort, p.wait_limit)) ok = false;
             if (!ok) continue;
             tc_fence_after();
-            const int kb = tile_at(j) * kPwKeys;
             uint32_t sv[128];                                      // the whole row of S in registers
             tc_ld32(s_addr, *reinterpret_cast<uint32_t(*)[32]>(&sv[0]));
             tc_ld32(s_addr + 32, *reinterpret_cast<uint32_t(*)[32]>(&sv[32]));
@@ -484,27 +525,30 @@ __global__ void __launch_bounds__(PwCfg<FP8>::threads, 1) prefill_window_kernel(
             // the row is in registers: the tensor core may overwrite the S buffer
             tc_fence_before();
             mbar_arrive(bar(PW_S_FREE));
+            const volatile int* e = s_ring + (j % kPwRing) * 4;
+            const int kb = e[0];
             float c_tile = c_row, v_scale = 1.f;
             if constexpr (FP8) {
-                c_tile *= s_scale[(j % kPwScaleRing) * 2];
-                v_scale = s_scale[(j % kPwScaleRing) * 2 + 1];
-                if (c_tile == 0.f) {                               // a K scale of 0 (or a row of Q): scores of 0
+                c_tile *= __int_as_float(e[1]);
+                v_scale = __int_as_float(e[2]);
+            }
+            // keys behind a row's own position, or in front of its window and behind the sinks: -infinity
+            const bool cut = kb + kPwKeys - 1 > pos || (kb < start && kb + kPwKeys > p.sinks);
+            if (__any_sync(0xffffffffu, cut || (FP8 && c_tile == 0.f))) {
+                if (FP8 && c_tile == 0.f) {                        // a K scale of 0: scores of 0
 #pragma unroll
                     for (int i = 0; i < 128; ++i) sv[i] = 0u;
                     c_tile = 1.f;
                 }
-            }
-            if (kb + kPwKeys - 1 > tile_lo) {                      // keys behind a row's own position
-                const int limit = pos - kb;                        // columns <= limit are visible
+                auto low_bits = [](int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; };
 #pragma unroll
-                for (int i = 0; i < 128; ++i)
-                    if (i > limit) sv[i] = 0xff800000u;            // -inf
-            }
-            if (windowed && kb <= tile_hi - p.window && kb + kPwKeys > sinks) {
-                const int start = pos - p.window + 1 - kb, sink = sinks - kb;     // columns >= start or < sink are visible
+                for (int w = 0; w < 4; ++w) {
+                    const int k0 = kb + w * 32;
+                    const uint32_t seen = low_bits(pos + 1 - k0) & (~low_bits(start - k0) | low_bits(p.sinks - k0));
 #pragma unroll
-                for (int i = 0; i < 128; ++i)
-                    if (i < start && i >= sink) sv[i] = 0xff800000u;
+                    for (int i = 0; i < 32; ++i)
+                        if (!(seen & (1u << i))) sv[w * 32 + i] = 0xff800000u;
+                }
             }
             float mx0 = -INFINITY, mx1 = -INFINITY, mx2 = -INFINITY, mx3 = -INFINITY;
 #pragma unroll
@@ -591,8 +635,8 @@ __global__ void __launch_bounds__(PwCfg<FP8>::threads, 1) prefill_window_kernel(
         if (n_kt > 0 && ok) {
             tc_fence_after();
             const float unit = FP8 ? v_ref : 1.f;
-            const float f = p.splits > 1 ? unit : l_run > 0.f ? unit / l_run : 0.f;
-            const bool any = l_run > 0.f;                           // a row that sees nothing gives zeros
+            const bool any = l_run != 0.f;                          // a row that sees nothing gives zeros
+            const float f = p.splits > 1 ? unit : unit / l_run;
             const int64_t row = int64_t(q0 + tok) * p.n_q_heads + kvh * p.group + r % p.group;
             const int64_t part = int64_t(split) * p.total_q * p.n_q_heads + row;
             if (p.splits > 1 && live) reinterpret_cast<float2*>(p.part_ml)[part] = make_float2(any ? m_ref : -INFINITY, l_run);
@@ -648,7 +692,7 @@ __global__ void __launch_bounds__(256) prefill_join_kernel(__nv_bfloat16* out, c
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int s = 0; s < splits; ++s) {
         const float2 x = ml[s * rows];
-        if (x.x == -INFINITY) continue;
+        if (x.y == 0.f) continue;                       // saw nothing of this part; its accumulator is not written
         const float a = exp2f(x.x - m);
         const float4 v = reinterpret_cast<const float4*>(part_o + (s * rows + row) * kHeadDim)[lane];
         l = fmaf(x.y, a, l);
@@ -657,7 +701,7 @@ __global__ void __launch_bounds__(256) prefill_join_kernel(__nv_bfloat16* out, c
         o.z = fmaf(v.z, a, o.z);
         o.w = fmaf(v.w, a, o.w);
     }
-    const float f = l > 0.f ? 1.f / l : 0.f;
+    const float f = l != 0.f ? 1.f / l : 0.f;
     uint2 w;
     w.x = pack_bf16(o.x * f, o.y * f);
     w.y = pack_bf16(o.z * f, o.w * f);

@@ -19,7 +19,15 @@ __device__ __forceinline__ void tc_mma(uint32_t d_tmem, uint64_t adesc, uint64_t
         ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(acc), "r"(0u)
         : "memory");
 }
-// same, with the A operand in tensor memory (16-bit elements packed two per column)
+// 8-bit operands (K-major, 32 of them per instruction)
+__device__ __forceinline__ void tc_mma_f8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}"
+        ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(acc), "r"(0u)
+        : "memory");
+}
+// same as tc_mma, with the A operand in tensor memory (16-bit elements packed two per column)
 __device__ __forceinline__ void tc_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t acc) {
     asm volatile(
         "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
@@ -65,7 +73,8 @@ __device__ __forceinline__ uint64_t tc_desc(uint32_t smem_addr, uint32_t lbo_byt
     d |= uint64_t(2) << 61;        // SWIZZLE_128B
     return d;
 }
-// kind::f16 instruction descriptor: D f32, A and B both bf16 or both f16, M = N = 128.
+// Instruction descriptor: D f32, M = N = 128; kind::f16 with A and B both bf16 or both f16 (f16 = true), or kind::f8f6f4
+// with both e4m3 (type code 0, as f16 in the other kind).
 constexpr uint32_t tc_idesc(bool b_mn_major, bool f16 = false) {
     return (1u << 4) | (f16 ? 0u : (1u << 7) | (1u << 10)) | (b_mn_major ? (1u << 16) : 0u) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
 }

@@ -28,8 +28,14 @@ _POOLS: dict = {}
 _CHECK = os.environ.get("INFER_B200_CHECK") == "1"    # debugging: read the device status word after each call
 
 
+# What a call costs the host counts as much as the kernel when a step is small: the lean accessors below (the raw stream
+# instead of a Stream object, addresses as plain integers, get_device() for both "on the GPU" and "on which") brought a
+# call of load_kvcache from 19 to 8 us.
+_raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+
+
 def _stream():
-    return C.c_void_p(torch.cuda.current_stream().cuda_stream)
+    return _raw_stream(_current_device())
 
 
 class _on_device:
@@ -38,7 +44,7 @@ class _on_device:
     __slots__ = ("guard",)
 
     def __init__(self, device):
-        self.guard = None if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+        self.guard = None if _current_device() == device.index else torch.cuda.device(device)
 
     def __enter__(self):
         if self.guard is not None:
@@ -105,7 +111,7 @@ _SCRATCH = _Scratch()
 
 
 def _ptr(t):
-    return C.c_void_p(t.data_ptr()) if t is not None else C.c_void_p(0)
+    return t.data_ptr() if t is not None else None
 
 
 class KVPool:
@@ -163,7 +169,7 @@ class KVPool:
 
 def pool_of(k_cache, v_cache, k_scale=None, v_scale=None) -> KVPool:
     """Pool handle for these cache tensors, created on first use (one per layer in practice)."""
-    key = (k_cache.data_ptr(), v_cache.data_ptr(), tuple(k_cache.shape), k_cache.dtype,
+    key = (k_cache.data_ptr(), v_cache.data_ptr(), k_cache.shape, k_cache.dtype,
            k_scale.data_ptr() if k_scale is not None else 0, v_scale.data_ptr() if v_scale is not None else 0)
     # A handle is valid for any tensor with the same addresses, shape and dtype, whatever Python
     # object presents them (a layer view sliced again every step, or new memory at an old address).
@@ -244,20 +250,21 @@ def qk_norm_rope_append(q, k, v, q_norm_weight, k_norm_weight, eps, positions, c
     return q_out
 
 
-def _rows(what, name, x, device=None):
-    """``x`` as rows [T, H, 128] of bf16 with contiguous heads on the GPU; their pitch in elements."""
-    if x.dim() != 3 or x.dtype != torch.bfloat16 or not x.is_cuda or x.shape[2] != 128:
-        raise RuntimeError(f"{what}: {name} must be a bf16 CUDA tensor [T, H, 128]")
-    if x.stride(2) != 1 or (x.shape[1] > 1 and x.stride(1) != 128):
+def _rows(what, name, x, device, shape=None):
+    """Checks that ``x`` is rows [T, H, 128] of bf16 with contiguous heads on GPU ``device``; their pitch in elements."""
+    size, stride = x.shape, x.stride()
+    if x.dtype is not torch.bfloat16 or len(size) != 3 or size[2] != 128 or x.get_device() != device:
+        raise RuntimeError(f"{what}: {name} must be a bf16 CUDA tensor [T, H, 128] on cuda:{device}")
+    if stride[2] != 1 or (size[1] > 1 and stride[1] != 128):
         raise RuntimeError(f"{what}: {name} must have contiguous heads")
-    if device is not None and x.device != device:
-        raise RuntimeError(f"{what}: {name} is on {x.device}, the call on {device}")
-    return x.stride(0) if x.shape[0] > 1 else x.shape[1] * 128
+    if shape is not None and size != shape:
+        raise RuntimeError(f"{what}: {name} must be {list(shape)}")
+    return stride[0] if size[0] > 1 else size[1] * 128
 
 
 def _vector(what, name, x, n, dtype, device):
-    if x.dtype != dtype or not x.is_cuda or x.device != device or x.numel() != n or not x.is_contiguous():
-        raise RuntimeError(f"{what}: {name} must be a contiguous {str(dtype)[6:]} tensor of {n} values on {device}")
+    if x.dtype is not dtype or x.get_device() != device or x.numel() != n or not x.is_contiguous():
+        raise RuntimeError(f"{what}: {name} must be a contiguous {str(dtype)[6:]} tensor of {n} values on cuda:{device}")
 
 
 def load_kvcache(k_cache, v_cache, slot_mapping, k_scale=None, v_scale=None, k_out=None, v_out=None):
@@ -265,34 +272,33 @@ def load_kvcache(k_cache, v_cache, slot_mapping, k_scale=None, v_scale=None, k_o
     the inverse of ``store_kvcache``.  e4m3 pools: byte * scale of its page and head, in fp32, rounded once.  Slots
     outside the pool (-1: padding) give rows of zeros.  ``k_out`` / ``v_out`` may be column slices of a wider row."""
     pool = pool_of(k_cache, v_cache, k_scale, v_scale)
-    n = slot_mapping.numel()
-    _vector("load_kvcache", "slot_mapping", slot_mapping, n, torch.int32, pool.device)
-    shape = (n, pool.n_kv_heads, pool.head_dim)
-    k_out, v_out = (torch.empty(shape, dtype=torch.bfloat16, device=pool.device) if t is None else t for t in (k_out, v_out))
-    pitch = []
-    for name, t in (("k_out", k_out), ("v_out", v_out)):
-        pitch.append(_rows("load_kvcache", name, t, pool.device))
-        if tuple(t.shape) != shape:
-            raise RuntimeError(f"load_kvcache: {name} must be {list(shape)}")
+    dev, n = pool.device.index, slot_mapping.numel()
+    _vector("load_kvcache", "slot_mapping", slot_mapping, n, torch.int32, dev)
+    shape = torch.Size((n, pool.n_kv_heads, pool.head_dim))
+    if k_out is None:
+        k_out = k_cache.new_empty(shape, dtype=torch.bfloat16)
+    if v_out is None:
+        v_out = k_cache.new_empty(shape, dtype=torch.bfloat16)
+    k_pitch, v_pitch = _rows("load_kvcache", "k_out", k_out, dev, shape), _rows("load_kvcache", "v_out", v_out, dev, shape)
     with _on_device(pool.device):
-        rc = _lib.load().infer_kv_load(pool.handle, _ptr(k_out), _ptr(v_out), pitch[0], pitch[1], _ptr(slot_mapping), n, _stream())
+        rc = _lib.load().infer_kv_load(pool.handle, k_out.data_ptr(), v_out.data_ptr(), k_pitch, v_pitch, slot_mapping.data_ptr(), n,
+                                       _stream())
     _lib.check(rc, "load_kvcache")
     return k_out, v_out
 
 
-def _rotary_args(what, q, k, positions, inv_freq, q_out, device):
+def _rotary_args(what, q, k, positions, inv_freq, q_out, dev):
     t = q.shape[0]
-    q_pitch, k_pitch = _rows(what, "q", q, device), _rows(what, "k", k, device)
+    q_pitch, k_pitch = _rows(what, "q", q, dev), _rows(what, "k", k, dev)
     if k.shape[0] != t:
         raise RuntimeError(f"{what}: q and k must have the same number of rows")
-    _vector(what, "positions", positions, t, torch.int64, device)
-    _vector(what, "inv_freq", inv_freq, inv_freq.numel(), torch.float64, device)
+    _vector(what, "positions", positions, t, torch.int64, dev)
+    pairs = inv_freq.numel()
+    _vector(what, "inv_freq", inv_freq, pairs, torch.float64, dev)
     if q_out is None:
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    q_out_pitch = _rows(what, "q_out", q_out, device)
-    if q_out.shape != q.shape:
-        raise RuntimeError(f"{what}: q_out must have the shape of q")
-    return q_out, q_pitch, k_pitch, q_out_pitch
+        q_out = q.new_empty(q.shape)
+        return q_out, q_pitch, k_pitch, q.shape[1] * 128, t, 2 * pairs
+    return q_out, q_pitch, k_pitch, _rows(what, "q_out", q_out, dev, q.shape), t, 2 * pairs
 
 
 def rotary_append(q, k, v, positions, inv_freq, k_cache, v_cache, slot_mapping, interleaved=False, attention_factor=1.0,
@@ -306,15 +312,16 @@ def rotary_append(q, k, v, positions, inv_freq, k_cache, v_cache, slot_mapping, 
     (column slices of the fused qkv output are fine); returns the rotated q, contiguous, or in ``q_out`` (may be ``q``).
     Rows with a slot outside the pool are not stored."""
     pool = pool_of(k_cache, v_cache)
-    q_out, q_pitch, k_pitch, q_out_pitch = _rotary_args("rotary_append", q, k, positions, inv_freq, q_out, pool.device)
-    v_pitch, t = _rows("rotary_append", "v", v, pool.device), q.shape[0]
-    if k.shape != v.shape or k.shape[1] != pool.n_kv_heads:
-        raise RuntimeError("rotary_append: k and v must have the pool's heads and q's rows")
-    _vector("rotary_append", "slot_mapping", slot_mapping, t, torch.int32, pool.device)
+    dev = pool.device.index
+    q_out, q_pitch, k_pitch, q_out_pitch, t, rot = _rotary_args("rotary_append", q, k, positions, inv_freq, q_out, dev)
+    v_pitch = _rows("rotary_append", "v", v, dev)
+    if v.shape != k.shape or k.shape[1] != pool.n_kv_heads:
+        raise RuntimeError("rotary_append: k and v must have q's rows and the pool's heads")
+    _vector("rotary_append", "slot_mapping", slot_mapping, t, torch.int32, dev)
     with _on_device(pool.device):
-        rc = _lib.load().infer_rotary_append(pool.handle, _ptr(q_out), q_out_pitch, _ptr(q), _ptr(k), _ptr(v), q_pitch, k_pitch,
-                                             v_pitch, _ptr(positions), _ptr(inv_freq), 2 * inv_freq.numel(), int(interleaved),
-                                             float(attention_factor), _ptr(slot_mapping), t, q.shape[1], _stream())
+        rc = _lib.load().infer_rotary_append(pool.handle, q_out.data_ptr(), q_out_pitch, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                                             q_pitch, k_pitch, v_pitch, positions.data_ptr(), inv_freq.data_ptr(), rot,
+                                             bool(interleaved), float(attention_factor), slot_mapping.data_ptr(), t, q.shape[1], _stream())
     _lib.check(rc, "rotary_append")
     return q_out
 
@@ -322,16 +329,15 @@ def rotary_append(q, k, v, positions, inv_freq, k_cache, v_cache, slot_mapping, 
 def rotary_embedding(q, k, positions, inv_freq, interleaved=False, attention_factor=1.0, q_out=None, k_out=None):
     """``rotary_append`` without the append -> (q, k) rotated; in front of ``store_kvcache`` for an e4m3 pool.
     ``q_out`` / ``k_out`` may be ``q`` / ``k``."""
-    q_out, q_pitch, k_pitch, q_out_pitch = _rotary_args("rotary_embedding", q, k, positions, inv_freq, q_out, q.device)
+    dev = q.get_device()
+    q_out, q_pitch, k_pitch, q_out_pitch, t, rot = _rotary_args("rotary_embedding", q, k, positions, inv_freq, q_out, dev)
     if k_out is None:
-        k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-    k_out_pitch = _rows("rotary_embedding", "k_out", k_out, q.device)
-    if k_out.shape != k.shape:
-        raise RuntimeError("rotary_embedding: k_out must have the shape of k")
+        k_out = k.new_empty(k.shape)
+    k_out_pitch = _rows("rotary_embedding", "k_out", k_out, dev, k.shape)
     with _on_device(q.device):
-        rc = _lib.load().infer_rotary_embed(_ptr(q_out), _ptr(k_out), q_out_pitch, k_out_pitch, _ptr(q), _ptr(k), q_pitch, k_pitch,
-                                            _ptr(positions), _ptr(inv_freq), 2 * inv_freq.numel(), int(interleaved),
-                                            float(attention_factor), q.shape[0], q.shape[1], k.shape[1], _stream())
+        rc = _lib.load().infer_rotary_embed(q_out.data_ptr(), k_out.data_ptr(), q_out_pitch, k_out_pitch, q.data_ptr(), k.data_ptr(),
+                                            q_pitch, k_pitch, positions.data_ptr(), inv_freq.data_ptr(), rot, bool(interleaved),
+                                            float(attention_factor), t, q.shape[1], k.shape[1], _stream())
     _lib.check(rc, "rotary_embedding")
     return q_out, k_out
 
@@ -346,6 +352,17 @@ def _window(what, window, sinks):
     if window < 1 or sinks < 0:
         raise RuntimeError(f"{what}: window must be at least 1 and sinks at least 0")
     return min(window, 0x7fffffff), min(sinks, 0x7fffffff)
+
+
+def _check_decode_window(what, q3, o, lens, table, pool):
+    """What the windowed form checks beyond the plain one."""
+    b = q3.shape[0]
+    if q3.shape[2] != 128 or o.dtype is not torch.bfloat16 or not o.is_contiguous():
+        raise RuntimeError(f"{what}: q and out must be contiguous bf16 [B, Hq, 128]")
+    if lens.device != pool.device or table.device != pool.device:
+        raise RuntimeError(f"{what}: cache_seqlens and block_table must be on the pools' device")
+    if lens.numel() != b or not lens.is_contiguous() or table.dim() != 2 or table.shape[0] < b or table.stride(1) != 1:
+        raise RuntimeError(f"{what}: cache_seqlens must hold a length, block_table a row of contiguous entries per sequence")
 
 
 # --------------------------------------------------------------------------- decode
@@ -364,7 +381,7 @@ def paged_attn_decode(q, k_cache, v_cache, cache_seqlens, block_table, softmax_s
     ``pool.decode_workspace_bytes(B, Hq)`` bytes reserved for this caller's stream; by default the
     per-device scratch is used (see ``_Scratch``: one stream per device)."""
     shape = q.shape
-    q3 = q.reshape(shape[0], shape[-2], shape[-1])
+    q3 = q if len(shape) == 3 else q.reshape(shape[0], shape[-2], shape[-1])
     if q3.dtype != torch.bfloat16 or not q3.is_contiguous():
         raise RuntimeError("paged_attn_decode: q must be contiguous bf16")
     for name, t in (("q", q3), ("out", out)):
@@ -377,12 +394,13 @@ def paged_attn_decode(q, k_cache, v_cache, cache_seqlens, block_table, softmax_s
         raise RuntimeError("paged_attn_decode: block_table rows must be contiguous")
     window, sinks = _window("paged_attn_decode", window, sinks)
     pool = pool_of(k_cache, v_cache, k_scale, v_scale)
-    o = torch.empty(q3.shape, dtype=q3.dtype, device=pool.device) if out is None else out.view(q3.shape)
+    o = torch.empty(q3.shape, dtype=q3.dtype, device=pool.device) if out is None else out if out.shape == q3.shape else out.view(q3.shape)
     lib = _lib.load()
     b, hq, _ = q3.shape
     ws = workspace if workspace is not None else _SCRATCH.get(pool.device, "decode", pool.decode_workspace_bytes(b, hq))
     with _on_device(pool.device):
         if window:
+            _check_decode_window("paged_attn_decode", q3, o, cache_seqlens, block_table, pool)
             rc = lib.infer_paged_decode_window(pool.handle, _ptr(o), _ptr(q3), _ptr(cache_seqlens), _ptr(block_table),
                                                block_table.stride(0), b, hq, float(softmax_scale), window, sinks, _ptr(ws),
                                                ws.numel(), _stream())
@@ -392,7 +410,7 @@ def paged_attn_decode(q, k_cache, v_cache, cache_seqlens, block_table, softmax_s
         _lib.check(rc, "paged_attn_decode")
         if _CHECK and not torch.cuda.is_current_stream_capturing():
             _lib.check(lib.infer_paged_decode_status(_ptr(ws), _stream()), "paged_attn_decode (device status)")
-    return o.view(shape)
+    return o if o.shape == shape else o.view(shape)
 
 
 def paged_attn_decode_append(q, key, value, k_cache, v_cache, cache_seqlens, block_table, softmax_scale,
@@ -405,7 +423,7 @@ def paged_attn_decode_append(q, key, value, k_cache, v_cache, cache_seqlens, blo
     host tensors, ``window`` and ``sinks`` limit the visible keys (see ``paged_attn_decode``)."""
     window, sinks = _window("paged_attn_decode_append", window, sinks)
     shape = q.shape
-    q3 = q.reshape(shape[0], shape[-2], shape[-1])
+    q3 = q if len(shape) == 3 else q.reshape(shape[0], shape[-2], shape[-1])
     if q3.dtype != torch.bfloat16 or not q3.is_contiguous():
         raise RuntimeError("paged_attn_decode_append: q must be contiguous bf16")
     b, hq, d = q3.shape
@@ -423,7 +441,7 @@ def paged_attn_decode_append(q, key, value, k_cache, v_cache, cache_seqlens, blo
         raise RuntimeError("paged_attn_decode_append: bf16 pools only (store_kvcache + paged_attn_decode for e4m3 pools)")
     if key.shape[1] != pool.n_kv_heads or value.shape != key.shape:
         raise RuntimeError("paged_attn_decode_append: key / value head count differs from the pool's")
-    o = torch.empty(q3.shape, dtype=q3.dtype, device=pool.device) if out is None else out.view(q3.shape)
+    o = torch.empty(q3.shape, dtype=q3.dtype, device=pool.device) if out is None else out if out.shape == q3.shape else out.view(q3.shape)
     lib = _lib.load()
     row = key.shape[1] * d
     k_pitch = key.stride(0) if b > 1 else row
@@ -433,13 +451,14 @@ def paged_attn_decode_append(q, key, value, k_cache, v_cache, cache_seqlens, blo
         args = (pool.handle, _ptr(o), _ptr(q3), _ptr(key), _ptr(value), k_pitch, v_pitch, _ptr(cache_seqlens),
                 _ptr(block_table), block_table.stride(0), b, hq, float(softmax_scale))
         if window:
+            _check_decode_window("paged_attn_decode_append", q3, o, cache_seqlens, block_table, pool)
             rc = lib.infer_paged_decode_append_window(*args, window, sinks, _ptr(ws), ws.numel(), _stream())
         else:
             rc = lib.infer_paged_decode_append(*args, _ptr(ws), ws.numel(), _stream())
         _lib.check(rc, "paged_attn_decode_append")
         if _CHECK and not torch.cuda.is_current_stream_capturing():
             _lib.check(lib.infer_paged_decode_status(_ptr(ws), _stream()), "paged_attn_decode_append (device status)")
-    return o.view(shape)
+    return o if o.shape == shape else o.view(shape)
 
 
 # --------------------------------------------------------------------------- prefill
