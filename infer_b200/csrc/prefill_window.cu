@@ -14,14 +14,18 @@
 // Keys.  A CTA walks the tiles that hold a key visible to any of its rows: those of the sinks, then those from the start
 //   of its first row's window on.  Block-table entries of other pages are never read.  V rows that no row of the CTA sees
 //   are cleared before the tensor core reads them: P is 0 there, but 0 times a stale NaN is not.
+// Many CTAs.  A CTA that is done takes over one that has not been launched yet (clusterlaunchcontrol): barriers, tensor
+//   memory and roles stay, and the Q and first K tiles of the next row block are loaded (and converted) while the softmax
+//   warps finish the current one.  Launched one by one, a CTA cost about 6 us beyond its tiles, a third of the time of a
+//   window of 1024 keys.
 // Few rows.  When the (row block, kv head, sequence) triples do not fill the GPU, the key tiles of a CTA are split over
 //   several, each leaving maximum, sum and accumulator per row in 32 bits, and a second kernel joins them.
 // e4m3.  S = Q K^T runs on the raw bytes of K (kind::f8f6f4, no conversion): a bf16 value has 8 significant bits, so it is
-//   the exact sum of two e4m3 values, its rounding to 4 bits and the rest.  A warpgroup of converters splits Q once per CTA,
+//   the exact sum of two e4m3 values, its rounding to 4 bits and the rest.  The softmax warps split Q once per row block,
 //   each row scaled by a power of two that puts its largest value into [2^7, 2^8); values 2^-10 below that lose bits of the
-//   second part, an error of 2^-18 of the row's largest.  Two e4m3 products take the tensor core as long as one bf16
+//   second part, an error of 2^-16 of the row's largest.  Two e4m3 products take the tensor core as long as one bf16
 //   product.  P has to keep more bits than that, so V becomes f16: TMA brings its bytes (half of bf16's traffic) into two
-//   staging slots and the converters turn them into operand tiles (e4m3 -> f16 is exact).  When K was converted as well the
+//   staging slots and a fourth warpgroup turns them into operand tiles (e4m3 -> f16 is exact).  When K was converted as well the
 //   kernel was 1.2-1.5 times slower than on a bf16 cache: the S products alone read shared memory at its full rate (128
 //   bytes a clock), and every converted tile moves another 48 KiB through it.
 //   The K scale of a tile's page and the row's power of two go into the factor of the softmax exponent.  The V scale goes
@@ -44,7 +48,14 @@ constexpr int kPwKeys = 128;                  // keys per K/V tile
 constexpr int kPwHalf = 128 * 128;            // bytes of one [128 rows][64 elems] swizzled sub-tile
 constexpr int kPwTile = 2 * kPwHalf;          // 32 KiB: one Q, K or V tile of 16-bit elements
 constexpr int kPwRaw = 128 * 128;             // 16 KiB: one K or V tile of e4m3 bytes
-constexpr int kPwRing = 8;                    // a tile's first key and scales stay here from its K's load to its softmax: 6 tiles at most
+constexpr int kPwRing = 8;                    // entries of the tile ring: one lives from its K's load to its P V product, 7 tiles at most
+// A tile's entry: whether some row of the CTA sees only part of it, its first key; e4m3: k scale, what O is multiplied by in
+// front of this tile (1 as a rule), what the V scale adds to the exponents of P, what takes it out of a row sum again, the V
+// scale that O is expressed in from there on; the rows that some query sees, [0, sink_end) and [begin, end).
+enum PwTileEntry { PT_CUT, PT_KEY0, PT_K_SCALE, PT_O_FACTOR, PT_UP, PT_DOWN, PT_V_REF, PT_SINK_END = 8, PT_BEGIN, PT_END, PT_INTS = 16 };
+// a row block's entry in the ring of two: number of key tiles (-1: no more row blocks), whether the second query tile has
+// rows, first row of q, rows and first key position of the sequence, first token of the block, kv head, part, windowed
+enum PwItemEntry { PI_TILES, PI_TWO, PI_Q0, PI_LQ, PI_SHIFT, PI_TOK0, PI_KVH, PI_SPLIT, PI_WINDOWED, PI_INTS = 16 };
 // tensor memory columns: S (shared by the two tiles) at 0, P of tile i at 128 + 64 i, O of tile i at 256 + 128 i
 constexpr uint32_t kPwTmemP = 128, kPwTmemO = 256;
 constexpr int kPwSoftmaxWarps = 8;
@@ -52,7 +63,8 @@ constexpr int kPwProducer = 8, kPwIssueS = 9, kPwIssuePV = 10;   // warp roles; 
 
 template <bool FP8>
 struct PwCfg {
-    static constexpr int k_stages = FP8 ? 4 : 3, v_stages = 2, raw_slots = FP8 ? 2 : 0;
+    static constexpr int k_stages = FP8 ? 2 : 3, v_stages = FP8 ? 3 : 2, raw_slots = FP8 ? 2 : 0;
+    static constexpr int v_loads = FP8 ? raw_slots : v_stages;        // V tiles that TMA can have under way
     static constexpr int k_bytes = FP8 ? kPwRaw : kPwTile;            // of a stage
     static constexpr int threads = (kPwSoftmaxWarps + (FP8 ? 8 : 4)) * 32;
     static constexpr int q = 0;
@@ -60,17 +72,46 @@ struct PwCfg {
     static constexpr int v = k + k_stages * k_bytes;
     static constexpr int raw = v + v_stages * kPwTile;
     static constexpr int bars = raw + raw_slots * kPwRaw;
-    static constexpr int n_bars = 28;
+    static constexpr int n_bars = 36;
     static constexpr int misc = bars + n_bars * 8;                    // tmem base, abort flag
-    static constexpr int ring = misc + 16;                            // [kPwRing] first key of a tile, its k scale, its v scale
-    static constexpr int qscale = ring + kPwRing * 16;                // [2][128] power of two taken out of a Q row
-    static constexpr int total = qscale + (FP8 ? 2 * kPwRows * 4 : 0);
+    static constexpr int claim = misc + 16;                           // answer to a request for another row block
+    static constexpr int ring = claim + 16;                           // [kPwRing][PT_INTS]
+    static constexpr int items = ring + kPwRing * PT_INTS * 4;        // [2][PI_INTS]
+    static constexpr int total = items + 2 * PI_INTS * 4;
     // the probabilities' exponent: how far the reference maximum may lag, and what is added to it
     static constexpr float lazy = FP8 ? 6.f : 8.f, bias = FP8 ? 6.f : 0.f;
 };
 
-enum PwBar { PW_Q_FULL = 0, PW_K_FULL = 1, PW_K_EMPTY = 5, PW_V_FULL = 9, PW_V_EMPTY = 11, PW_S_FULL = 13, PW_P_FULL = 15,
-             PW_PV_DONE = 17, PW_DRAIN = 19, PW_S_FREE = 21, PW_RAW_FULL = 22, PW_RAW_EMPTY = 24, PW_Q_READY = 26 };
+enum PwBar { PW_Q_FULL = 0, PW_K_FULL = 1, PW_K_EMPTY = 5, PW_V_FULL = 9, PW_V_EMPTY = 12, PW_S_FULL = 15, PW_P_FULL = 17,
+             PW_PV_DONE = 19, PW_DRAIN = 21, PW_S_FREE = 23, PW_RAW_FULL = 24, PW_RAW_EMPTY = 26, PW_Q_READY = 28, PW_Q_EMPTY = 30,
+             PW_ITEM_FULL = 31, PW_ITEM_EMPTY = 33, PW_CLAIM = 35 };
+
+// Asks for a thread block of this launch that has not started yet; the answer (16 bytes) arrives on the barrier.
+__device__ __forceinline__ void claim_request(uint32_t answer, uint32_t bar) {
+    mbar_expect_tx(bar, 16);
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];"
+                 ::"r"(answer), "r"(bar) : "memory");
+}
+// The answer: true and the block's indices, or false when every block has started.
+__device__ __forceinline__ bool claim_result(uint32_t answer, int& x, int& y, int& z) {
+    const uint4 w = ld_shared_v4(answer);
+    const uint64_t lo = uint64_t(w.x) | uint64_t(w.y) << 32, hi = uint64_t(w.z) | uint64_t(w.w) << 32;
+    uint32_t got, cx = 0, cy = 0, cz = 0;
+    asm volatile(
+        "{\n\t.reg .b128 r;\n\t.reg .pred p;\n\t"
+        "mov.b128 r, {%4, %5};\n\t"
+        "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t"
+        "mov.u32 %1, 0;\n\tmov.u32 %2, 0;\n\tmov.u32 %3, 0;\n\t"
+        "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%1, %2, %3, _}, r;\n\t}"
+        : "=&r"(got), "=&r"(cx), "=&r"(cy), "=&r"(cz)
+        : "l"(lo), "l"(hi)
+        : "memory");
+    x = int(cx);
+    y = int(cy);
+    z = int(cz);
+    return got != 0;
+}
 
 struct PwParams {
     __nv_bfloat16* out;
@@ -94,6 +135,76 @@ struct PwParams {
     int stall_producer;
 };
 
+// tc_wait for warps that wait most of the time and can be late: they sleep between looks, since their polling takes issue slots
+// from the softmax warps (the converters polling like the others: 507 us, sleeping: 495 us for 148 x 8 row blocks).
+__device__ __forceinline__ bool tc_wait_idle(uint32_t bar, uint32_t parity, volatile int* abort_flag, uint32_t limit) {
+    for (uint32_t i = 0; i < limit; ++i) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if (*abort_flag) return false;
+        __nanosleep(100);
+    }
+    *abort_flag = 1;
+    return false;
+}
+
+// Row t of a Q tile, 128 bf16 in two halves of 64 dims, becomes two rows of 128 e4m3 values in the same place whose sum it is
+// up to a power of two, which is returned (NaN for a row with a value that is not finite, or of 2^126 and more, which leaves
+// no room for the power).  Chunk x (of 16) holds eight bf16; result c (of 8) is the first parts of chunks 2c and 2c + 1,
+// stored over chunk c, and their second parts, stored over chunk 8 + c.  The eight rows of a phase have a chunk at eight
+// different banks.
+// The split is arithmetic on f16 bits: y = q * 2^-e * 2^-8 has the exponents of e4m3 (subnormal ones too) in its upper bits,
+// so the first part is y cut to three bits of mantissa, the second the difference, and the byte of either its sign and the
+// seven bits below bit 14.
+__device__ __forceinline__ float split_q_row(uint32_t tile, int t) {
+    auto chunk = [&](int x) { return tile + (x >> 3) * kPwHalf + swz128(t, x & 7); };
+    uint4 w[16];
+#pragma unroll
+    for (int x = 0; x < 16; ++x) w[x] = ld_shared_v4(chunk(x));
+    __nv_bfloat162 top2[4];                                // largest magnitudes, NaN if there is one
+#pragma unroll
+    for (int x = 0; x < 16; ++x) {
+        const uint32_t v[4] = {w[x].x, w[x].y, w[x].z, w[x].w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const __nv_bfloat162 m = __habs2(*reinterpret_cast<const __nv_bfloat162*>(&v[k]));
+            top2[k] = x == 0 ? m : __hmax2_nan(top2[k], m);
+        }
+    }
+    const __nv_bfloat162 all = __hmax2_nan(__hmax2_nan(top2[0], top2[1]), __hmax2_nan(top2[2], top2[3]));
+    const uint32_t top = __bfloat16_as_ushort(__hmax_nan(__low2bfloat16(all), __high2bfloat16(all))) & 0x7fffu;
+    const int e = min(max(int(top >> 7) - 127 - 7, -118), 118);
+    const float down = __uint_as_float(uint32_t(127 - e - 8) << 23);
+    auto bytes = [](uint32_t y0, uint32_t y1) {            // e4m3 of four f16 scaled by 2^-8
+        const uint32_t b0 = (y0 & 0x80008000u) | ((y0 << 1) & 0x7fff7fffu);
+        const uint32_t b1 = (y1 & 0x80008000u) | ((y1 << 1) & 0x7fff7fffu);
+        return __byte_perm(b0, b1, 0x7531);
+    };
+    auto split8 = [&](const uint4& q, uint32_t& h0, uint32_t& h1, uint32_t& l0, uint32_t& l1) {
+        const uint32_t v[4] = {q.x, q.y, q.z, q.w};
+        uint32_t y[4], l[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            y[k] = pack_f16(__uint_as_float(v[k] << 16) * down, __uint_as_float(v[k] & 0xffff0000u) * down);
+            const uint32_t h = y[k] & 0xff80ff80u;
+            const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&y[k]), *reinterpret_cast<const __half2*>(&h));
+            l[k] = *reinterpret_cast<const uint32_t*>(&d);
+        }
+        h0 = bytes(y[0], y[1]);
+        h1 = bytes(y[2], y[3]);
+        l0 = bytes(l[0], l[1]);
+        l1 = bytes(l[2], l[3]);
+    };
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+        uint4 h, l;
+        split8(w[2 * c], h.x, h.y, l.x, l.y);
+        split8(w[2 * c + 1], h.z, h.w, l.z, l.w);
+        st_shared_v4(chunk(c), h);
+        st_shared_v4(chunk(8 + c), l);
+    }
+    return __uint_as_float(top < (127u + 126u) << 7 ? uint32_t(127 + e) << 23 : 0x7fffffffu);
+}
+
 template <bool FP8>
 __global__ void __launch_bounds__(PwCfg<FP8>::threads, 1) prefill_window_kernel(PwParams p, const __grid_constant__ CUtensorMap map_q,
                                                                                 const __grid_constant__ CUtensorMap map_k,
@@ -105,65 +216,36 @@ __global__ void __launch_bounds__(PwCfg<FP8>::threads, 1) prefill_window_kernel(
     volatile uint32_t* s_tmem = reinterpret_cast<volatile uint32_t*>(smem + C::misc);
     volatile int* s_abort = reinterpret_cast<volatile int*>(smem + C::misc + 4);
     volatile int* s_ring = reinterpret_cast<volatile int*>(smem + C::ring);
-    volatile float* s_qscale = reinterpret_cast<volatile float*>(smem + C::qscale);
+    volatile int* s_item = reinterpret_cast<volatile int*>(smem + C::items);
     auto bar = [&](int which, int idx = 0) { return base + uint32_t(C::bars) + uint32_t(which + idx) * 8; };
 
-    const int b = blockIdx.z;
-    const int kvh = blockIdx.y / p.splits, split = blockIdx.y - kvh * p.splits;
-    const int xb = int(gridDim.x) - 1 - int(blockIdx.x);    // longest rows first
-    const int q0 = p.cu_q[b];
-    const int lq = p.cu_q[b + 1] - q0, lk = p.cu_k[b + 1] - p.cu_k[b];
-    const int shift = lk - lq;                              // position of the first query row
-    const int tok0 = xb * 2 * p.tokens;                     // first token of the CTA
-    if (tok0 >= lq) return;                                 // whole CTA leaves before any barrier or TMEM use
-    const bool two = tok0 + p.tokens < lq;                  // the second tile has rows
-    // key tiles: [0, n_sink) and [n_sink + skip, last], list entry x is tile x below n_sink and x + skip from there on
-    const int pos_lo = shift + tok0, pos_hi = shift + min(lq, tok0 + 2 * p.tokens) - 1;
-    const bool windowed = p.window < lk;
-    const int first_key = windowed ? max(pos_lo - p.window + 1, 0) : 0;
-    const int sinks = windowed ? min(p.sinks, lk) : 0;
-    int n_sink = (sinks + kPwKeys - 1) / kPwKeys;
-    const int skip = max(first_key / kPwKeys - n_sink, 0);
-    if (skip == 0) n_sink = 0;
-    const int n_all = pos_hi < 0 ? 0 : pos_hi / kPwKeys + 1 - skip;
-    const int per_split = (n_all + p.splits - 1) / p.splits;
-    const int x0 = min(n_all, split * per_split), n = min(n_all, x0 + per_split) - x0;
-    auto tile_at = [&](int j) { return x0 + j < n_sink ? x0 + j : x0 + j + skip; };
-
-    if (n <= 0) {
-        // nothing is visible here: zeros, or an empty part
-        const int rows = min(lq - tok0, 2 * p.tokens) * p.group;
-        for (int i = threadIdx.x; i < rows * 16; i += C::threads) {
-            const int r = i >> 4, tok = tok0 + r / p.group, head = kvh * p.group + r % p.group;
-            const int64_t row = int64_t(q0 + tok) * p.n_q_heads + head;
-            if (p.splits == 1) {
-                reinterpret_cast<uint4*>(p.out + row * kHeadDim)[i & 15] = make_uint4(0, 0, 0, 0);
-            } else if ((i & 15) == 0) {
-                reinterpret_cast<float2*>(p.part_ml)[int64_t(split) * p.total_q * p.n_q_heads + row] = make_float2(-INFINITY, 0.f);
-            }
-        }
-        return;
-    }
     // The roles of the third warpgroup sit in the first four hardware warps (see prefill_tc.cu), the converters in the last.
     const int hw = int(threadIdx.x >> 5), lane = threadIdx.x & 31;
     const int warp = hw < 4 ? hw + kPwSoftmaxWarps : hw < 12 ? hw - 4 : hw;
 
     if (threadIdx.x == 0) {
         mbar_init(bar(PW_Q_FULL), 1);
-        mbar_init(bar(PW_Q_READY), 4);
+        mbar_init(bar(PW_Q_READY, 0), 4);
+        mbar_init(bar(PW_Q_READY, 1), 4);
+        mbar_init(bar(PW_Q_EMPTY), 1);
+        mbar_init(bar(PW_CLAIM), 1);
         for (int i = 0; i < C::k_stages; ++i) {
             mbar_init(bar(PW_K_FULL, i), 1);
             mbar_init(bar(PW_K_EMPTY, i), 1);
         }
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < C::v_stages; ++i) {
             mbar_init(bar(PW_V_FULL, i), FP8 ? 4 : 1);
             mbar_init(bar(PW_V_EMPTY, i), 1);
+        }
+        for (int i = 0; i < 2; ++i) {
             mbar_init(bar(PW_S_FULL, i), 1);
             mbar_init(bar(PW_P_FULL, i), 128);
             mbar_init(bar(PW_PV_DONE, i), 1);
             mbar_init(bar(PW_DRAIN, i), 1);
             mbar_init(bar(PW_RAW_FULL, i), 1);
             mbar_init(bar(PW_RAW_EMPTY, i), 4);
+            mbar_init(bar(PW_ITEM_FULL, i), 1);
+            mbar_init(bar(PW_ITEM_EMPTY, i), kPwSoftmaxWarps + 2 + (FP8 ? 4 : 0));     // every warp that reads the entry
         }
         mbar_init(bar(PW_S_FREE), 128);                     // the warpgroup that copied the S buffer to registers
         *s_abort = 0;
@@ -181,116 +263,177 @@ __global__ void __launch_bounds__(PwCfg<FP8>::threads, 1) prefill_window_kernel(
     tc_fence_after();
     const uint32_t tmem = __shfl_sync(0xffffffffu, *s_tmem, 0);   // warp-uniform by construction
     bool ok = true;
-    // V rows of key tile `tile` that some row of the CTA sees: [0, sink_end) and [begin, end)
-    auto seen_rows = [&](int tile, int& sink_end, int& begin, int& end) {
-        const int kb = tile * kPwKeys;
-        sink_end = max(sinks - kb, 0);
-        begin = first_key - kb;
-        end = pos_hi + 1 - kb;
+    // Every role walks the row blocks that the producer publishes, with counters that run on from block to block (a
+    // barrier's phase is the count of its uses).
+    auto item_wait = [&](int item) -> const volatile int* {
+        if (!tc_wait(bar(PW_ITEM_FULL, item & 1), (item >> 1) & 1, s_abort, p.wait_limit)) ok = false;
+        return s_item + (item & 1) * PI_INTS;
+    };
+    auto item_done = [&](int item) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(PW_ITEM_EMPTY, item & 1));
     };
 
     // Register budget.  bf16: 384 threads x 168 at launch = 72 for the third warpgroup and 216 for the softmax ones.
-    // e4m3: 512 x 128 = 48 for roles and converters, 208 for softmax.
+    // e4m3: 512 x 128 = 56 for roles and converters, 200 for softmax.
     if (hw < 4) {
-        if constexpr (FP8) asm volatile("setmaxnreg.dec.sync.aligned.u32 48;" ::: "memory");
+        if constexpr (FP8) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;" ::: "memory");
         else asm volatile("setmaxnreg.dec.sync.aligned.u32 72;" ::: "memory");
         if (warp == kPwProducer) {
-            // ============================================================= TMA producer
-            if (lane == 0 && !p.stall_producer) {
+            // ============================================================= row blocks and TMA
+            if (lane == 0) {
                 tma_prefetch_desc(&map_q);
                 tma_prefetch_desc(&map_k);
                 tma_prefetch_desc(&map_v);
-                const int n_q = two ? 2 : 1;
-                mbar_expect_tx(bar(PW_Q_FULL), n_q * 2 * p.tokens * p.group * 128);
-                for (int i = 0; i < n_q; ++i)
-                    for (int half = 0; half < 2; ++half)
-                        tma_load_3d(base + C::q + i * kPwTile + half * kPwHalf, &map_q, bar(PW_Q_FULL), half * 64, kvh * p.group,
-                                    q0 + tok0 + i * p.tokens);
-                const int32_t* table = p.block_tables + int64_t(b) * p.bt_stride;
-                auto page_of = [&](int tile) {
-                    const int idx = tile * kPwKeys / p.block_size;
-                    return idx < p.bt_stride ? table[idx] : -1;
-                };
-                // a page outside of the pool gives rows of zeros (TMA fills what lies outside of the tensor)
-                auto slot_of = [&](int tile, int page) {
-                    return page >= 0 && page < p.num_blocks ? page * p.block_size + tile * kPwKeys % p.block_size : -kPwKeys;
-                };
-                // read by the softmax warps (and the converters) of tile j: released by the arrival that K's copy is armed with
-                auto put_ring = [&](int j, int key0, float ks, float vs) {
-                    volatile int* e = s_ring + (j % kPwRing) * 4;
-                    e[0] = key0;
-                    e[1] = __float_as_int(ks);
-                    e[2] = __float_as_int(vs);
-                };
-                if constexpr (FP8) {
-                    // order K0, K1, V0, K2, V1, ...: K of the next tile is needed before V of this one
-                    auto load_raw = [&](const CUtensorMap* map, uint32_t dst, uint32_t full, int slot) {
-                        mbar_expect_tx(full, kPwRaw);
-                        tma_load_3d(dst, map, full, 0, kvh, slot);
+                int item = 0, q_loads = 0, kc = 0, vc = 0;       // published row blocks, Q loads, K and V tiles
+                uint32_t claims = 0;
+                bool asked = false, stalled = false;             // asked: an answer is outstanding
+                int bx = blockIdx.x, by = blockIdx.y, b = blockIdx.z;
+                while (ok) {
+                    const int kvh = by / p.splits, split = by - kvh * p.splits;
+                    const int q0 = p.cu_q[b], lq = p.cu_q[b + 1] - q0, lk = p.cu_k[b + 1] - p.cu_k[b];
+                    const int shift = lk - lq;                              // position of the first query row
+                    const int tok0 = (int(gridDim.x) - 1 - bx) * 2 * p.tokens;     // longest rows first
+                    auto ask = [&] {
+                        fence_proxy_async();                                // the last answer has been read
+                        claim_request(base + C::claim, bar(PW_CLAIM));
+                        asked = true;
                     };
-                    int page = page_of(tile_at(0)), v_slot = 0;      // page of tile j, looked up one tile ahead
-                    int k_issued = 0, v_issued = 0;
-                    for (int j = 0; j <= n && ok; ++j) {
-                        int k_slot = 0;
-                        if (j < n) {
-                            const bool in = page >= 0 && page < p.num_blocks;
-                            const float ks = in ? p.k_scale[int64_t(page) * p.n_kv_heads + kvh] : 0.f;
-                            const float vs = in ? p.v_scale[int64_t(page) * p.n_kv_heads + kvh] : 0.f;
-                            const int s = j % C::k_stages;
-                            k_slot = slot_of(tile_at(j), page);
-                            if (j + 1 < n) page = page_of(tile_at(j + 1));
-                            put_ring(j, tile_at(j) * kPwKeys, ks, vs);
-                            if (tc_wait(bar(PW_K_EMPTY, s), ((j / C::k_stages) & 1) ^ 1, s_abort, p.wait_limit)) {
-                                load_raw(&map_k, base + C::k + s * kPwRaw, bar(PW_K_FULL, s), k_slot);
-                                ++k_issued;
-                            } else ok = false;
+                    if (tok0 < lq) {
+                        // key tiles: [0, n_sink) and [n_sink + skip, last]; list entry x is tile x below n_sink, x + skip behind
+                        const int pos_lo = shift + tok0, pos_hi = shift + min(lq, tok0 + 2 * p.tokens) - 1;
+                        const bool windowed = p.window < lk;
+                        const int first_key = windowed ? max(pos_lo - p.window + 1, 0) : 0;
+                        const int sinks = windowed ? min(p.sinks, lk) : 0;
+                        int n_sink = (sinks + kPwKeys - 1) / kPwKeys;
+                        const int skip = max(first_key / kPwKeys - n_sink, 0);
+                        if (skip == 0) n_sink = 0;
+                        const int n_all = pos_hi < 0 ? 0 : pos_hi / kPwKeys + 1 - skip;
+                        const int per_split = (n_all + p.splits - 1) / p.splits;
+                        const int x0 = min(n_all, split * per_split), n = min(n_all, x0 + per_split) - x0;
+                        auto tile_at = [&](int j) { return x0 + j < n_sink ? x0 + j : x0 + j + skip; };
+                        const bool two = tok0 + p.tokens < lq;
+                        if (!tc_wait(bar(PW_ITEM_EMPTY, item & 1), ((item >> 1) & 1) ^ 1, s_abort, p.wait_limit)) { ok = false; break; }
+                        volatile int* e = s_item + (item & 1) * PI_INTS;
+                        e[PI_TILES] = n;
+                        e[PI_TWO] = two;
+                        e[PI_Q0] = q0;
+                        e[PI_LQ] = lq;
+                        e[PI_SHIFT] = shift;
+                        e[PI_TOK0] = tok0;
+                        e[PI_KVH] = kvh;
+                        e[PI_SPLIT] = split;
+                        e[PI_WINDOWED] = windowed;
+                        mbar_arrive(bar(PW_ITEM_FULL, item & 1));
+                        ++item;
+                        if (n > 0 && p.stall_producer) {                    // self-test: nothing is loaded, every wait runs out
+                            stalled = true;
+                            break;
                         }
-                        if (j >= 1 && ok) {
-                            const int jv = j - 1, s = jv & 1;
-                            if (tc_wait(bar(PW_RAW_EMPTY, s), ((jv >> 1) & 1) ^ 1, s_abort, p.wait_limit)) {
-                                load_raw(&map_v, base + C::raw + s * kPwRaw, bar(PW_RAW_FULL, s), v_slot);
-                                ++v_issued;
-                            } else ok = false;
+                        if (n > 0) {
+                            if (!tc_wait(bar(PW_Q_EMPTY), (q_loads & 1) ^ 1, s_abort, p.wait_limit)) { ok = false; break; }
+                            const int n_q = two ? 2 : 1;
+                            mbar_expect_tx(bar(PW_Q_FULL), n_q * 2 * p.tokens * p.group * 128);
+                            for (int i = 0; i < n_q; ++i)
+                                for (int half = 0; half < 2; ++half)
+                                    tma_load_3d(base + C::q + i * kPwTile + half * kPwHalf, &map_q, bar(PW_Q_FULL), half * 64,
+                                                kvh * p.group, q0 + tok0 + i * p.tokens);
+                            ++q_loads;
+                            const int32_t* table = p.block_tables + int64_t(b) * p.bt_stride;
+                            auto page_of = [&](int j) {                     // -1: outside of the table or of the pool
+                                const int idx = j < n ? tile_at(j) * kPwKeys / p.block_size : 0;
+                                const int page = idx < p.bt_stride ? table[idx] : -1;
+                                return page >= 0 && page < p.num_blocks ? page : -1;
+                            };
+                            auto scale_of = [&](const float* scale, int page) {
+                                return FP8 && page >= 0 ? scale[int64_t(page) * p.n_kv_heads + kvh] : 0.f;
+                            };
+                            // a page is looked up two tiles ahead and its scales one tile ahead: neither load is waited for
+                            int page = page_of(0), page_next = page_of(1), v_slot = 0;
+                            float k_scale = scale_of(p.k_scale, page), v_scale = scale_of(p.v_scale, page);
+                            constexpr int lag = FP8 ? 0 : 1;
+                            float v_ref = 0.f;                              // e4m3: V scale that O is expressed in, 0 = none yet
+                            // order K0, K1, V0, K2, V1, ...: K of the next tile is needed before V of this one.  e4m3: K0, V0, K1,
+                            // V1, ...: V has the conversion in front of it
+                            for (int j = 0; j < n + lag && ok; ++j) {
+                                int slot = 0;
+                                if (j < n) {
+                                    const int tile = tile_at(j), key0 = tile * kPwKeys;
+                                    // a page outside of the pool gives rows of zeros (TMA fills what lies outside of the tensor)
+                                    slot = page >= 0 ? page * p.block_size + key0 % p.block_size : -kPwKeys;
+                                    page = page_next;
+                                    page_next = page_of(j + 2);
+                                    const float k_scale_next = scale_of(p.k_scale, page), v_scale_next = scale_of(p.v_scale, page);
+                                    volatile int* t = s_ring + (kc % kPwRing) * PT_INTS;     // released by the arrival K's copy is armed with
+                                    t[PT_KEY0] = key0;
+                                    t[PT_CUT] = key0 + kPwKeys - 1 > pos_lo || (windowed && key0 <= pos_hi - p.window && key0 + kPwKeys > sinks);
+                                    t[PT_SINK_END] = sinks - key0;
+                                    t[PT_BEGIN] = first_key - key0;
+                                    t[PT_END] = pos_hi + 1 - key0;
+                                    if constexpr (FP8) {
+                                        float o_factor = 1.f, ratio = 1.f;
+                                        if (j == 0) v_ref = 0.f;
+                                        if (v_ref == 0.f) v_ref = v_scale;              // O is 0 so far
+                                        else if (v_scale > 8.f * v_ref) {
+                                            o_factor = v_ref / v_scale;
+                                            v_ref = v_scale;
+                                        }
+                                        if (v_scale > 0.f) ratio = fmaxf(v_scale / v_ref, 1e-18f);
+                                        else t[PT_SINK_END] = t[PT_BEGIN] = t[PT_END] = 0;     // a scale of 0: values of 0
+                                        t[PT_K_SCALE] = __float_as_int(k_scale);
+                                        t[PT_UP] = __float_as_int(C::bias + log2f(ratio));
+                                        t[PT_DOWN] = __float_as_int(1.f / ratio);
+                                        t[PT_O_FACTOR] = __float_as_int(o_factor);
+                                        t[PT_V_REF] = __float_as_int(v_ref);
+                                    }
+                                    k_scale = k_scale_next;
+                                    v_scale = v_scale_next;
+                                    const int s = kc % C::k_stages;
+                                    if (tc_wait(bar(PW_K_EMPTY, s), ((kc / C::k_stages) & 1) ^ 1, s_abort, p.wait_limit)) {
+                                        const uint32_t dst = base + C::k + s * C::k_bytes;
+                                        mbar_expect_tx(bar(PW_K_FULL, s), C::k_bytes);
+                                        tma_load_3d(dst, &map_k, bar(PW_K_FULL, s), 0, kvh, slot);
+                                        if constexpr (!FP8) tma_load_3d(dst + kPwHalf, &map_k, bar(PW_K_FULL, s), 64, kvh, slot);
+                                        ++kc;
+                                    } else ok = false;
+                                }
+                                if (FP8) v_slot = slot;
+                                if (j >= lag && ok) {
+                                    const int s = vc % C::v_loads;
+                                    if (tc_wait(bar(FP8 ? PW_RAW_EMPTY : PW_V_EMPTY, s), ((vc / C::v_loads) & 1) ^ 1, s_abort, p.wait_limit)) {
+                                        const uint32_t full = bar(FP8 ? PW_RAW_FULL : PW_V_FULL, s);
+                                        const uint32_t dst = FP8 ? base + C::raw + s * kPwRaw : base + C::v + s * kPwTile;
+                                        mbar_expect_tx(full, C::k_bytes);
+                                        tma_load_3d(dst, &map_v, full, 0, kvh, v_slot);
+                                        if constexpr (!FP8) tma_load_3d(dst + kPwHalf, &map_v, full, 64, kvh, v_slot);
+                                        ++vc;
+                                    } else ok = false;
+                                }
+                                v_slot = slot;
+                                if (ok && !asked && j + 2 >= n) ask();      // two tiles before the last load: the answer is there in time
+                            }
                         }
-                        v_slot = k_slot;
                     }
-                    // never leave with a copy in flight: wait (bounded) for everything that was armed
-                    mbar_wait(bar(PW_Q_FULL), 0, p.wait_limit);
-                    for (int j = max(0, k_issued - C::k_stages); j < k_issued; ++j)
-                        mbar_wait(bar(PW_K_FULL, j % C::k_stages), (j / C::k_stages) & 1, p.wait_limit);
-                    for (int j = max(0, v_issued - 2); j < v_issued; ++j) mbar_wait(bar(PW_RAW_FULL, j & 1), (j >> 1) & 1, p.wait_limit);
-                } else {
-                    auto load_tile = [&](const CUtensorMap* map, uint32_t dst, uint32_t full, int slot) {
-                        mbar_expect_tx(full, kPwTile);
-                        tma_load_3d(dst, map, full, 0, kvh, slot);
-                        tma_load_3d(dst + kPwHalf, map, full, 64, kvh, slot);
-                    };
-                    int k_issued = 0, v_issued = 0, v_slot = 0;
-                    for (int j = 0; j <= n && ok; ++j) {
-                        int k_slot = 0;
-                        if (j < n) {
-                            const int s = j % C::k_stages, tile = tile_at(j);
-                            k_slot = slot_of(tile, page_of(tile));
-                            put_ring(j, tile * kPwKeys, 1.f, 1.f);
-                            if (tc_wait(bar(PW_K_EMPTY, s), ((j / C::k_stages) & 1) ^ 1, s_abort, p.wait_limit)) {
-                                load_tile(&map_k, base + C::k + s * kPwTile, bar(PW_K_FULL, s), k_slot);
-                                ++k_issued;
-                            } else ok = false;
-                        }
-                        if (j >= 1 && ok) {
-                            const int jv = j - 1, s = jv & 1;
-                            if (tc_wait(bar(PW_V_EMPTY, s), ((jv >> 1) & 1) ^ 1, s_abort, p.wait_limit)) {
-                                load_tile(&map_v, base + C::v + s * kPwTile, bar(PW_V_FULL, s), v_slot);
-                                ++v_issued;
-                            } else ok = false;
-                        }
-                        v_slot = k_slot;
-                    }
-                    mbar_wait(bar(PW_Q_FULL), 0, p.wait_limit);
-                    for (int j = max(0, k_issued - C::k_stages); j < k_issued; ++j)
-                        mbar_wait(bar(PW_K_FULL, j % C::k_stages), (j / C::k_stages) & 1, p.wait_limit);
-                    for (int j = max(0, v_issued - 2); j < v_issued; ++j) mbar_wait(bar(PW_V_FULL, j & 1), (j >> 1) & 1, p.wait_limit);
+                    if (!ok) break;
+                    if (!asked) ask();
+                    if (!tc_wait(bar(PW_CLAIM), claims & 1, s_abort, p.wait_limit)) { ok = false; break; }
+                    ++claims;
+                    asked = false;
+                    if (!claim_result(base + C::claim, bx, by, b)) break;
                 }
+                if (ok && !stalled) {
+                    if (tc_wait(bar(PW_ITEM_EMPTY, item & 1), ((item >> 1) & 1) ^ 1, s_abort, p.wait_limit)) {
+                        s_item[(item & 1) * PI_INTS + PI_TILES] = -1;
+                        mbar_arrive(bar(PW_ITEM_FULL, item & 1));
+                    }
+                }
+                // never leave with a copy (or an answer) in flight: wait (bounded) for everything that was armed
+                if (asked) mbar_wait(bar(PW_CLAIM), claims & 1, p.wait_limit);
+                if (q_loads > 0) mbar_wait(bar(PW_Q_FULL), (q_loads - 1) & 1, p.wait_limit);
+                for (int j = max(0, kc - C::k_stages); j < kc; ++j)
+                    mbar_wait(bar(PW_K_FULL, j % C::k_stages), (j / C::k_stages) & 1, p.wait_limit);
+                for (int j = max(0, vc - C::v_loads); j < vc; ++j)
+                    mbar_wait(bar(FP8 ? PW_RAW_FULL : PW_V_FULL, j % C::v_loads), (j / C::v_loads) & 1, p.wait_limit);
             }
         } else if (warp == kPwIssueS) {
             // ============================================================= MMA issue: the S products
@@ -316,16 +459,31 @@ __global__ void __launch_bounds__(PwCfg<FP8>::threads, 1) prefill_window_kernel(
                 }
                 __syncwarp();
             };
-            if (!tc_wait(bar(FP8 ? PW_Q_READY : PW_Q_FULL), 0, s_abort, p.wait_limit)) ok = false;
-            int ks = 0, kph = 0;                                           // stage and phase of K_j
-            for (int j = 0; j < n && ok; ++j) {
-                if (!tc_wait(bar(PW_K_FULL, ks), kph, s_abort, p.wait_limit)) { ok = false; break; }
-                issue_s(0, ks);
-                if (ok && two) issue_s(1, ks);
+            int q_uses = 0, q1_uses = 0, ks = 0, kph = 0;                               // stage and phase of the next K tile
+            for (int item = 0; ok; ++item) {
+                const volatile int* e = item_wait(item);
                 if (!ok) break;
-                if (elect_one()) tc_commit(bar(PW_K_EMPTY, ks));              // all S(j) are issued
-                __syncwarp();
-                if (++ks == C::k_stages) { ks = 0; kph ^= 1; }
+                const int n = e[PI_TILES];
+                const bool two = e[PI_TWO] != 0;
+                if (n < 0) break;
+                if (n > 0) {
+                    if (!tc_wait(bar(FP8 ? PW_Q_READY : PW_Q_FULL), q_uses & 1, s_abort, p.wait_limit)) { ok = false; break; }
+                    for (int j = 0; j < n && ok; ++j) {
+                        if (!tc_wait(bar(PW_K_FULL, ks), kph, s_abort, p.wait_limit)) { ok = false; break; }
+                        issue_s(0, ks);
+                        if (FP8 && j == 0 && ok && two && !tc_wait(bar(PW_Q_READY, 1), q1_uses++ & 1, s_abort, p.wait_limit)) ok = false;
+                        if (ok && two) issue_s(1, ks);
+                        if (!ok) break;
+                        if (elect_one()) {                                    // all S(j) are issued
+                            tc_commit(bar(PW_K_EMPTY, ks));
+                            if (j == n - 1) tc_commit(bar(PW_Q_EMPTY));
+                        }
+                        __syncwarp();
+                        if (++ks == C::k_stages) { ks = 0; kph ^= 1; }
+                    }
+                    ++q_uses;
+                }
+                item_done(item);
             }
             // all tensor-core work issued by this warp must have retired before TMEM is freed
             if (elect_one()) tc_commit(bar(PW_DRAIN, 0));
@@ -335,8 +493,10 @@ __global__ void __launch_bounds__(PwCfg<FP8>::threads, 1) prefill_window_kernel(
             // ============================================================= MMA issue: the P V products
             constexpr uint32_t idesc_pv = tc_idesc(true, FP8);
             const uint64_t v_desc0 = tc_desc(base + C::v, kPwHalf);
-            auto issue_pv = [&](int i, int stage, int j) {   // O_i += P_i V  (V_FULL of that stage already awaited)
-                if (!tc_wait(bar(PW_P_FULL, i), j & 1, s_abort, p.wait_limit)) { ok = false; return; }
+            int uses0 = 0, uses1 = 0;                        // products of either query tile so far
+            auto issue_pv = [&](int i, int stage, int j, int& uses) {   // O_i += P_i V  (V_FULL of that stage already awaited)
+                if (!tc_wait(bar(PW_P_FULL, i), uses & 1, s_abort, p.wait_limit)) { ok = false; return; }
+                ++uses;
                 tc_fence_after();
                 if (elect_one()) {
                     const uint64_t vd = v_desc0 + uint64_t(stage * (kPwTile >> 4));
@@ -349,173 +509,164 @@ __global__ void __launch_bounds__(PwCfg<FP8>::threads, 1) prefill_window_kernel(
                 }
                 __syncwarp();
             };
-            for (int j = 0; j < n && ok; ++j) {
-                const int vs = j & 1;
-                if (!tc_wait(bar(PW_V_FULL, vs), (j >> 1) & 1, s_abort, p.wait_limit)) { ok = false; break; }
-                if constexpr (!FP8) {
-                    // clear the rows that nobody sees (e4m3: the converters did)
-                    int sink_end, begin, end;
-                    seen_rows(tile_at(j), sink_end, begin, end);
-                    if (end < kPwKeys || begin > sink_end) {
-                        uint8_t* vt = smem + C::v + vs * kPwTile;
-                        for (int x = lane; x < kPwKeys * 8; x += 32) {
-                            const int r = x >> 3;
-                            if (r < sink_end || (r >= begin && r < end)) continue;
-                            *reinterpret_cast<uint4*>(vt + x * 16) = make_uint4(0, 0, 0, 0);
-                            *reinterpret_cast<uint4*>(vt + kPwHalf + x * 16) = make_uint4(0, 0, 0, 0);
-                        }
-                        fence_proxy_async();
-                        __syncwarp();
-                    }
-                }
-                issue_pv(0, vs, j);
-                if (ok && two) issue_pv(1, vs, j);
+            int vc = 0, vs = 0, vph = 0;                     // V tiles so far, stage and phase of the next
+            for (int item = 0; ok; ++item) {
+                const volatile int* e = item_wait(item);
                 if (!ok) break;
-                if (elect_one()) tc_commit(bar(PW_V_EMPTY, vs));              // all products with V_j are issued
-                __syncwarp();
+                const int n = e[PI_TILES];
+                const bool two = e[PI_TWO] != 0;
+                if (n < 0) break;
+                for (int j = 0; j < n && ok; ++j, ++vc) {
+                    if (!tc_wait(bar(PW_V_FULL, vs), vph, s_abort, p.wait_limit)) { ok = false; break; }
+                    if constexpr (!FP8) {
+                        // clear the rows that nobody sees (e4m3: the converters did)
+                        const volatile int* t = s_ring + (vc % kPwRing) * PT_INTS;
+                        const int sink_end = t[PT_SINK_END], begin = t[PT_BEGIN], end = t[PT_END];
+                        if (end < kPwKeys || begin > max(sink_end, 0)) {
+                            uint8_t* vt = smem + C::v + vs * kPwTile;
+                            for (int x = lane; x < kPwKeys * 8; x += 32) {
+                                const int r = x >> 3;
+                                if (r < sink_end || (r >= begin && r < end)) continue;
+                                *reinterpret_cast<uint4*>(vt + x * 16) = make_uint4(0, 0, 0, 0);
+                                *reinterpret_cast<uint4*>(vt + kPwHalf + x * 16) = make_uint4(0, 0, 0, 0);
+                            }
+                            fence_proxy_async();
+                            __syncwarp();
+                        }
+                    }
+                    issue_pv(0, vs, j, uses0);
+                    if (ok && two) issue_pv(1, vs, j, uses1);
+                    if (!ok) break;
+                    if (elect_one()) tc_commit(bar(PW_V_EMPTY, vs));              // all products with V_j are issued
+                    __syncwarp();
+                    if (++vs == C::v_stages) { vs = 0; vph ^= 1; }
+                }
+                item_done(item);
             }
             if (elect_one()) tc_commit(bar(PW_DRAIN, 1));
             __syncwarp();
             mbar_wait(bar(PW_DRAIN, 1), 0, p.wait_limit);
         }
     } else if (FP8 && hw >= 12) {
-        // ================================================================= converters: e4m3 bytes -> f16 operand tiles
+        // ================================================================= converters: V bytes -> f16
         if constexpr (FP8) {
-            asm volatile("setmaxnreg.dec.sync.aligned.u32 48;" ::: "memory");
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 56;" ::: "memory");
             const int t = int(threadIdx.x) - 12 * 32;                         // 0 .. 127
-            if (!tc_wait(bar(PW_Q_FULL), 0, s_abort, p.wait_limit)) ok = false;
-            if (ok) {
-                // Q in place, one row per thread: chunk x (of 16) holds eight bf16; result c (of 8) is the first parts of
-                // chunks 2c and 2c + 1, stored over chunk c, and their second parts, stored over chunk 8 + c.  Chunks that a
-                // store covers before their turn are read ahead.  A thread alone touches its row; the eight rows of a phase
-                // have a chunk at eight different banks.
-#pragma unroll 1
-                for (int i = 0; i < (two ? 2 : 1); ++i) {
-                    const uint32_t row = base + C::q + i * kPwTile;
-                    auto chunk = [&](int x) { return row + (x >> 3) * kPwHalf + swz128(t, x & 7); };
-                    uint32_t top = 0;                                         // largest magnitude, as bf16 bits
-#pragma unroll 2
-                    for (int x = 0; x < 16; ++x) {
-                        const uint4 w = ld_shared_v4(chunk(x));
-                        const uint32_t v[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) top = max(top, max(v[k] & 0x7fffu, (v[k] >> 16) & 0x7fffu));
+            // A thread's chunk of V: 16 dims (4 bytes of the lane number, low bits) of rows row0, row0 + 16, ...; the eight lanes
+            // of a phase take four chunks of one half of the dims in rows m and m ^ 5, whose swizzles put them at eight
+            // different banks both where they are read and where they are written.
+            const int row0 = (t >> 6) * 8 + (((t >> 4) & 3) ^ (t & 4 ? 5 : 0)), c0 = ((t >> 3) & 1) * 4 + (t & 3);
+            const uint32_t src0 = base + C::raw + swz128(row0, c0);
+            const uint32_t dst0 = base + C::v + (c0 >> 2) * kPwHalf + swz128(row0, (c0 & 3) * 2);
+            int vc = 0, vs = 0, vph = 0;
+            for (int item = 0; ok; ++item) {
+                const volatile int* ie = item_wait(item);
+                if (!ok) break;
+                const int n = ie[PI_TILES];
+                if (n < 0) break;
+                for (int j = 0; j < n && ok; ++j, ++vc) {
+                    const int s = vc % C::raw_slots;
+                    if (!tc_wait_idle(bar(PW_RAW_FULL, s), (vc / C::raw_slots) & 1, s_abort, p.wait_limit) ||
+                        !tc_wait_idle(bar(PW_V_EMPTY, vs), vph ^ 1, s_abort, p.wait_limit)) {
+                        ok = false;
+                        break;
                     }
-                    const int e = min(max(int(top >> 7) - 127 - 7, -126), 126);
-                    const float down = __uint_as_float(uint32_t(127 - e) << 23);
-                    // (a row that holds an infinity or a NaN gives NaN)
-                    s_qscale[i * kPwRows + t] = __uint_as_float(top < 0x7f80u ? uint32_t(127 + e) << 23 : 0x7fffffffu);
-                    auto split8 = [&](const uint4& w, uint32_t& h0, uint32_t& h1, uint32_t& l0, uint32_t& l1) {
-                        const uint32_t v[4] = {w.x, w.y, w.z, w.w};
-                        uint32_t h[4], l[4];
+                    const volatile int* e = s_ring + (vc % kPwRing) * PT_INTS;
+                    const int sink_end = e[PT_SINK_END], begin = e[PT_BEGIN], end = e[PT_END];
+                    const uint32_t src = src0 + s * kPwRaw, dst = dst0 + vs * kPwTile;
+                    const bool partly = end < kPwKeys || begin > max(sink_end, 0);
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            const float2 f = make_float2(__uint_as_float(v[k] << 16) * down, __uint_as_float(v[k] & 0xffff0000u) * down);
-                            h[k] = __nv_cvt_float2_to_fp8x2(f, __NV_SATFINITE, __NV_E4M3);
-                            const uint32_t back = e4m3x2_to_f16x2(h[k]);
-                            const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&back));
-                            l[k] = __nv_cvt_float2_to_fp8x2(make_float2(f.x - y.x, f.y - y.y), __NV_SATFINITE, __NV_E4M3);
+                    for (int h = 0; h < 2; ++h) {
+                        uint4 w[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) w[i] = ld_shared_v4(src + (h * 4 + i) * 16 * 128);
+                        if (partly) {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const int r = row0 + (h * 4 + i) * 16;
+                                if (!(r < sink_end || (r >= begin && r < end))) w[i] = make_uint4(0, 0, 0, 0);
+                            }
                         }
-                        h0 = h[0] | h[1] << 16;
-                        h1 = h[2] | h[3] << 16;
-                        l0 = l[0] | l[1] << 16;
-                        l1 = l[2] | l[3] << 16;
-                    };
-                    auto result = [&](int c, const uint4& wa, const uint4& wb) {
-                        uint4 h, l;
-                        split8(wa, h.x, h.y, l.x, l.y);
-                        split8(wb, h.z, h.w, l.z, l.w);
-                        st_shared_v4(chunk(c), h);
-                        st_shared_v4(chunk(8 + c), l);
-                    };
-                    const uint4 w8 = ld_shared_v4(chunk(8)), w9 = ld_shared_v4(chunk(9));
-                    const uint4 w10 = ld_shared_v4(chunk(10)), w11 = ld_shared_v4(chunk(11));
-#pragma unroll 1
-                    for (int c = 0; c < 4; ++c) {
-                        const uint4 wa = ld_shared_v4(chunk(2 * c)), wb = ld_shared_v4(chunk(2 * c + 1));
-                        result(c, wa, wb);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            uint4 lo, hi;                                    // sixteen dims: two chunks of eight f16
+                            e4m3x4_to_f16x2x2(w[i].x, lo.x, lo.y);
+                            e4m3x4_to_f16x2x2(w[i].y, lo.z, lo.w);
+                            e4m3x4_to_f16x2x2(w[i].z, hi.x, hi.y);
+                            e4m3x4_to_f16x2x2(w[i].w, hi.z, hi.w);
+                            st_shared_v4(dst + (h * 4 + i) * 16 * 128, lo);
+                            st_shared_v4((dst ^ 16) + (h * 4 + i) * 16 * 128, hi);
+                        }
                     }
-                    const uint4 w12 = ld_shared_v4(chunk(12)), w13 = ld_shared_v4(chunk(13));
-                    result(4, w8, w9);
-                    result(5, w10, w11);
-                    const uint4 w14 = ld_shared_v4(chunk(14)), w15 = ld_shared_v4(chunk(15));
-                    result(6, w12, w13);
-                    result(7, w14, w15);
-                }
-                fence_proxy_async();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(bar(PW_Q_READY));
-            }
-            for (int j = 0; j < n && ok; ++j) {
-                const int s = j & 1;
-                if (!tc_wait(bar(PW_RAW_FULL, s), (j >> 1) & 1, s_abort, p.wait_limit) ||
-                    !tc_wait(bar(PW_V_EMPTY, s), ((j >> 1) & 1) ^ 1, s_abort, p.wait_limit)) {
-                    ok = false;
-                    break;
-                }
-                int sink_end, begin, end;
-                seen_rows(tile_at(j), sink_end, begin, end);
-                if (__int_as_float(s_ring[(j % kPwRing) * 4 + 2]) == 0.f) sink_end = 0, end = 0;       // a scale of 0: values of 0
-                const uint32_t src = base + C::raw + s * kPwRaw, dst = base + C::v + s * kPwTile;
-                const int c = t & 7;
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    uint4 w[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) w[i] = ld_shared_v4(src + swz128((h * 4 + i) * 16 + (t >> 3), c));
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int r = (h * 4 + i) * 16 + (t >> 3);
-                        if (!(r < sink_end || (r >= begin && r < end))) w[i] = make_uint4(0, 0, 0, 0);
-                        uint4 lo, hi;
-                        e4m3x4_to_f16x2x2(w[i].x, lo.x, lo.y);
-                        e4m3x4_to_f16x2x2(w[i].y, lo.z, lo.w);
-                        e4m3x4_to_f16x2x2(w[i].z, hi.x, hi.y);
-                        e4m3x4_to_f16x2x2(w[i].w, hi.z, hi.w);
-                        // sixteen dims become two chunks; lanes 4-7 of a row store the second one first, so that the eight
-                        // lanes of a phase (whose two halves of the dims share banks) hit eight different chunks
-                        const uint32_t half = dst + (c >> 2) * kPwHalf;
-                        const bool swap = c >= 4;
-                        st_shared_v4(half + swz128(r, (c & 3) * 2 + (swap ? 1 : 0)), swap ? hi : lo);
-                        st_shared_v4(half + swz128(r, (c & 3) * 2 + (swap ? 0 : 1)), swap ? lo : hi);
+                    fence_proxy_async();
+                    __syncwarp();
+                    if (lane == 0) {
+                        mbar_arrive(bar(PW_V_FULL, vs));
+                        mbar_arrive(bar(PW_RAW_EMPTY, s));
                     }
+                    if (++vs == C::v_stages) { vs = 0; vph ^= 1; }
                 }
-                fence_proxy_async();
-                __syncwarp();
-                if (lane == 0) {
-                    mbar_arrive(bar(PW_V_FULL, s));
-                    mbar_arrive(bar(PW_RAW_EMPTY, s));
-                }
+                item_done(item);
             }
         }
     } else {
         // ================================================================= softmax, one row per thread
-        if constexpr (FP8) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;" ::: "memory");
+        if constexpr (FP8) asm volatile("setmaxnreg.inc.sync.aligned.u32 200;" ::: "memory");
         else asm volatile("setmaxnreg.inc.sync.aligned.u32 216;" ::: "memory");
         const int g = warp >> 2;                                   // query tile of this warpgroup
         const int r = (warp & 3) * 32 + lane;                      // row in the tile == TMEM lane
         const uint32_t lane_sel = uint32_t((warp & 3) * 32) << 16;
-        const int n_kt = g == 0 || two ? n : 0;
-        const int tile_tok = tok0 + g * p.tokens;                  // first token of the tile
-        const int tok = tile_tok + r / p.group;
-        const bool live = r < p.tokens * p.group && tok < lq;      // rows behind the tokens of the tile or the sequence hold anything
-        const int pos = shift + min(tok, min(lq, tile_tok + p.tokens) - 1);
-        const int start = windowed ? pos - p.window + 1 : -0x40000000;      // first key of the row's window
         const uint32_t s_addr = tmem + lane_sel;                   // the S buffer is shared by the two tiles
         const uint32_t p_addr = tmem + lane_sel + kPwTmemP + g * 64;
         const uint32_t o_addr = tmem + lane_sel + kPwTmemO + g * 128;
+        int tiles = 0, uses = 0, q_uses = 0;                       // key tiles so far: of the CTA, of this query tile; Q loads so far
+
+        for (int item = 0; ok; ++item) {
+        const volatile int* ie = item_wait(item);
+        if (!ok) break;
+        const int n_all = ie[PI_TILES];
+        if (n_all < 0) break;
+        if (n_all == 0) {
+            // nothing is visible here: zeros, or an empty part
+            const int tok0 = ie[PI_TOK0], q0 = ie[PI_Q0], head0 = ie[PI_KVH] * p.group;
+            const int rows = min(ie[PI_LQ] - tok0, 2 * p.tokens) * p.group;
+            for (int i = warp * 32 + lane; i < rows * 16; i += kPwSoftmaxWarps * 32) {
+                const int x = i >> 4;
+                const int64_t row = int64_t(q0 + tok0 + x / p.group) * p.n_q_heads + head0 + x % p.group;
+                if (p.splits == 1) {
+                    reinterpret_cast<uint4*>(p.out + row * kHeadDim)[i & 15] = make_uint4(0, 0, 0, 0);
+                } else if ((i & 15) == 0) {
+                    reinterpret_cast<float2*>(p.part_ml)[int64_t(ie[PI_SPLIT]) * p.total_q * p.n_q_heads + row] = make_float2(-INFINITY, 0.f);
+                }
+            }
+        }
         float m_ref = -INFINITY, l_run = 0.f;                      // reference maximum (log2 domain), row sum
-        float v_ref = 0.f;                                         // e4m3: V scale that O is expressed in, 0 = none yet
+        float unit = 1.f;                                          // e4m3: V scale that O is expressed in
         float c_row = p.scale_log2;
-        if (FP8 && n_kt > 0) {
-            if (!tc_wait(bar(PW_Q_READY), 0, s_abort, p.wait_limit)) ok = false;
-            c_row *= s_qscale[g * kPwRows + r];
+        int left = g == 0 || ie[PI_TWO] ? n_all : 0;
+        if (left == 0) tiles += n_all;                             // this query tile has no rows
+        const bool any_tile = left > 0;
+        if (FP8 && any_tile) {
+            // this thread's row of Q: one row block's tiles take 256 threads about a microsecond; by the converters, four warps
+            // that also yield to these, they took six
+            if (!tc_wait(bar(PW_Q_FULL), q_uses & 1, s_abort, p.wait_limit)) ok = false;
+            if (ok) {
+                c_row = p.scale_log2 * split_q_row(base + C::q + g * kPwTile, r);
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(PW_Q_READY, g));
+            }
         }
 
-        for (int j = 0; j < n_kt; ++j) {
-            if (ok && !tc_wait(bar(PW_S_FULL, g), j & 1, s_abort, p.wait_limit)) ok = false;
+        for (; left > 0; --left, ++uses, ++tiles) {
+            if (ok && !tc_wait(bar(PW_S_FULL, g), uses & 1, s_abort, p.wait_limit)) ok = false;
             if (!ok) continue;
             tc_fence_after();
+            const bool first = left == ie[PI_TILES];
+            // the tile's entry, early: its latency passes under the loads of S
+            const volatile int* e = s_ring + (tiles % kPwRing) * PT_INTS;
+            const uint4 head = ld_shared_v4(base + C::ring + (tiles % kPwRing) * (PT_INTS * 4));      // CUT, KEY0, K_SCALE, O_FACTOR
+            float c_tile = FP8 ? c_row * __uint_as_float(head.z) : c_row;
             uint32_t sv[128];                                      // the whole row of S in registers
             tc_ld32(s_addr, *reinterpret_cast<uint32_t(*)[32]>(&sv[0]));
             tc_ld32(s_addr + 32, *reinterpret_cast<uint32_t(*)[32]>(&sv[32]));
@@ -525,25 +676,20 @@ __global__ void __launch_bounds__(PwCfg<FP8>::threads, 1) prefill_window_kernel(
             // the row is in registers: the tensor core may overwrite the S buffer
             tc_fence_before();
             mbar_arrive(bar(PW_S_FREE));
-            const volatile int* e = s_ring + (j % kPwRing) * 4;
-            const int kb = e[0];
-            float c_tile = c_row, v_scale = 1.f;
-            if constexpr (FP8) {
-                c_tile *= __int_as_float(e[1]);
-                v_scale = __int_as_float(e[2]);
-            }
-            // keys behind a row's own position, or in front of its window and behind the sinks: -infinity
-            const bool cut = kb + kPwKeys - 1 > pos || (kb < start && kb + kPwKeys > p.sinks);
-            if (__any_sync(0xffffffffu, cut || (FP8 && c_tile == 0.f))) {
+            if (__any_sync(0xffffffffu, head.x != 0 || (FP8 && c_tile == 0.f))) {
                 if (FP8 && c_tile == 0.f) {                        // a K scale of 0: scores of 0
 #pragma unroll
                     for (int i = 0; i < 128; ++i) sv[i] = 0u;
                     c_tile = 1.f;
                 }
+                // keys behind a row's own position, or in front of its window and behind the sinks: -infinity
+                const int tile_tok = ie[PI_TOK0] + g * p.tokens;   // first token of the query tile
+                const int pos = ie[PI_SHIFT] + min(tile_tok + r / p.group, min(ie[PI_LQ], tile_tok + p.tokens) - 1);
+                const int start = ie[PI_WINDOWED] ? pos - p.window + 1 : -0x40000000;
                 auto low_bits = [](int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; };
 #pragma unroll
                 for (int w = 0; w < 4; ++w) {
-                    const int k0 = kb + w * 32;
+                    const int k0 = int(head.y) + w * 32;
                     const uint32_t seen = low_bits(pos + 1 - k0) & (~low_bits(start - k0) | low_bits(p.sinks - k0));
 #pragma unroll
                     for (int i = 0; i < 32; ++i)
@@ -561,30 +707,23 @@ __global__ void __launch_bounds__(PwCfg<FP8>::threads, 1) prefill_window_kernel(
             const float mx = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)) * c_tile;    // -inf: this row sees none of the tile
             // move the reference only when the maximum outgrew it by more than 2^lazy
             const bool move = mx > m_ref + C::lazy || (m_ref == -INFINITY && mx > -INFINITY);
-            float v_factor = 1.f;                                  // what a larger V scale makes of O
-            if constexpr (FP8) {
-                if (v_ref == 0.f) v_ref = v_scale;                 // O is 0 so far
-                else if (v_scale > 8.f * v_ref) {
-                    v_factor = v_ref / v_scale;
-                    v_ref = v_scale;
-                }
-            }
-            if (__any_sync(0xffffffffu, move || v_factor != 1.f)) {
+            const float o_factor = FP8 ? __uint_as_float(head.w) : 1.f;
+            if (__any_sync(0xffffffffu, move || (FP8 && o_factor != 1.f))) {
                 const float m_new = move ? mx : m_ref;
                 const float alpha = m_ref == -INFINITY ? 0.f : fast_exp2(m_ref - m_new);
-                if (j > 0) {
-                    // O holds tiles < j once P V_{j-1} has retired; P V_j cannot start before P_FULL below
-                    if (!tc_wait(bar(PW_PV_DONE, g), (j - 1) & 1, s_abort, p.wait_limit)) { ok = false; continue; }
+                if (!first) {
+                    // O is whole once the P V product of the previous tile has retired; the next cannot start before P_FULL below
+                    if (!tc_wait(bar(PW_PV_DONE, g), (uses - 1) & 1, s_abort, p.wait_limit)) { ok = false; continue; }
                     tc_fence_after();
-                    const float f = alpha * v_factor;
+                    const float f = alpha * o_factor;
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        uint32_t v[32];
-                        tc_ld32(o_addr + c * 32, v);
+                    for (int c = 0; c < 8; ++c) {                  // sixteen columns at a time: S is still in registers
+                        uint32_t v[16];
+                        tc_ld16(o_addr + c * 16, v);
                         tc_wait_ld();
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
-                        tc_st32(o_addr + c * 32, v);
+                        for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
+                        tc_st16(o_addr + c * 16, v);
                     }
                     tc_wait_st();
                 }
@@ -592,53 +731,47 @@ __global__ void __launch_bounds__(PwCfg<FP8>::threads, 1) prefill_window_kernel(
                 m_ref = m_new;
             }
             float up = m_ref == -INFINITY ? 0.f : -m_ref;          // added to the exponent
-            float down = 1.f;                                      // takes the V scale out of the row sum
-            if constexpr (FP8) {
-                up += C::bias;
-                if (v_scale > 0.f && v_scale != v_ref) {
-                    const float ratio = fmaxf(__fdividef(v_scale, v_ref), 1e-18f);
-                    up += __log2f(ratio);
-                    down = __fdividef(1.f, ratio);
-                }
-            }
+            if constexpr (FP8) up += __int_as_float(e[PT_UP]);
             // the tensor core must be done reading P of the previous key tile (long since, as a rule)
-            if (j > 0 && !tc_wait(bar(PW_PV_DONE, g), (j - 1) & 1, s_abort, p.wait_limit)) { ok = false; continue; }
+            if (!first && !tc_wait(bar(PW_PV_DONE, g), (uses - 1) & 1, s_abort, p.wait_limit)) { ok = false; continue; }
             // P = exp2(S * c + up) as packed 16-bit values
             uint64_t rsa = pk2(0.f, 0.f), rsb = pk2(0.f, 0.f);
             const uint64_t c2 = pk2(c_tile, c_tile), up2 = pk2(up, up);
+            auto pair = [&](int c, uint64_t& sum) {
+                const uint64_t x2 = ffma2(pk2(__uint_as_float(sv[c]), __uint_as_float(sv[c + 1])), c2, up2);
+                float e0, e1;
+                upk2(x2, e0, e1);
+                e0 = fast_exp2(e0);
+                e1 = fast_exp2(e1);
+                sum = fadd2(sum, pk2(e0, e1));
+                return FP8 ? pack_f16(e0, e1) : pack_bf16(e0, e1);
+            };
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 uint32_t pk[32];
 #pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    const int c = h * 64 + 2 * i;
-                    const uint64_t x2 = ffma2(pk2(__uint_as_float(sv[c]), __uint_as_float(sv[c + 1])), c2, up2);
-                    float e0, e1;
-                    upk2(x2, e0, e1);
-                    e0 = fast_exp2(e0);
-                    e1 = fast_exp2(e1);
-                    if (i & 1) rsb = fadd2(rsb, pk2(e0, e1)); else rsa = fadd2(rsa, pk2(e0, e1));
-                    pk[i] = FP8 ? pack_f16(e0, e1) : pack_bf16(e0, e1);
-                }
+                for (int i = 0; i < 32; ++i) pk[i] = pair(h * 64 + 2 * i, i & 1 ? rsb : rsa);
                 tc_st32(p_addr + h * 32, pk);
             }
             float rs0, rs1, rs2, rs3;
             upk2(rsa, rs0, rs1);
             upk2(rsb, rs2, rs3);
-            l_run = fmaf((rs0 + rs1) + (rs2 + rs3), down, l_run);
+            l_run = fmaf((rs0 + rs1) + (rs2 + rs3), FP8 ? __int_as_float(e[PT_DOWN]) : 1.f, l_run);
+            if constexpr (FP8) unit = __int_as_float(e[PT_V_REF]);
             tc_wait_st();
             tc_fence_before();
-            mbar_arrive(bar(PW_P_FULL, g));
+            mbar_arrive(bar(PW_P_FULL, g));                        // (the tile's entry may be gone from here on)
         }
         // O is complete once the last P V has retired
-        if (n_kt > 0 && ok && !tc_wait(bar(PW_PV_DONE, g), (n_kt - 1) & 1, s_abort, p.wait_limit)) ok = false;
-        if (n_kt > 0 && ok) {
+        if (any_tile && ok && !tc_wait(bar(PW_PV_DONE, g), (uses - 1) & 1, s_abort, p.wait_limit)) ok = false;
+        if (any_tile && ok) {
             tc_fence_after();
-            const float unit = FP8 ? v_ref : 1.f;
             const bool any = l_run != 0.f;                          // a row that sees nothing gives zeros
             const float f = p.splits > 1 ? unit : unit / l_run;
-            const int64_t row = int64_t(q0 + tok) * p.n_q_heads + kvh * p.group + r % p.group;
-            const int64_t part = int64_t(split) * p.total_q * p.n_q_heads + row;
+            const int tok = ie[PI_TOK0] + g * p.tokens + r / p.group;
+            const bool live = r < p.tokens * p.group && tok < ie[PI_LQ];      // rows behind the tokens of the tile or the sequence hold anything
+            const int64_t row = int64_t(ie[PI_Q0] + tok) * p.n_q_heads + ie[PI_KVH] * p.group + r % p.group;
+            const int64_t part = int64_t(ie[PI_SPLIT]) * p.total_q * p.n_q_heads + row;
             if (p.splits > 1 && live) reinterpret_cast<float2*>(p.part_ml)[part] = make_float2(any ? m_ref : -INFINITY, l_run);
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
@@ -666,6 +799,9 @@ __global__ void __launch_bounds__(PwCfg<FP8>::threads, 1) prefill_window_kernel(
                 }
             }
             tc_fence_before();
+        }
+        q_uses += ie[PI_TILES] > 0;
+        item_done(item);
         }
     }
 
