@@ -210,17 +210,12 @@ INFER_API int infer_paged_prefill(const infer_kv_pool_t* pool, void* out, const 
  * effect).  The alignment of queries and keys is that of infer_paged_prefill; a query that sees no key (a sequence with
  * fewer keys than queries) gives zeros, rows of out that belong to no sequence are left alone, and block-table entries
  * of pages without a visible key are not read.  Up to 128 query heads per kv head.  max_seqlen_q has to cover the longest
- * chunk, max_seqlen_k (the longest context) only guides the split.  softmax_scale: a positive finite number.
- * workspace: when few rows meet many keys, the keys are split over thread blocks and the parts joined through
- * infer_paged_prefill_window_workspace_bytes() of 16-byte aligned device memory (0 when there is nothing to split); it
- * needs no initialisation and is free again when the call has run.  NULL, or fewer bytes: fewer parts, same result up to
- * rounding. */
+ * chunk; max_seqlen_k (the longest context) only guides over how many thread blocks few rows' keys are split.
+ * softmax_scale: a positive finite number. */
 INFER_API int infer_paged_prefill_window(const infer_kv_pool_t* pool, void* out, const void* q, int64_t total_q,
                         const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, const int32_t* block_tables,
                         int64_t bt_stride, int batch, int max_seqlen_q, int max_seqlen_k, int n_q_heads,
-                        float softmax_scale, int window, int sinks, void* workspace, size_t workspace_bytes, void* stream);
-INFER_API size_t infer_paged_prefill_window_workspace_bytes(const infer_kv_pool_t* pool, int64_t total_q, int batch,
-                        int max_seqlen_q, int max_seqlen_k, int n_q_heads, int window, int sinks);
+                        float softmax_scale, int window, int sinks, void* stream);
 
 /* Dense causal attention.  Replaces flash_attn_prefill_impl
  * (src/operators/flashattn/flashattn.cu:269-328; schema src/bindings.cpp:9):

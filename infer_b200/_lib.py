@@ -42,8 +42,7 @@ SIGNATURES = {
     "infer_paged_decode_noalloc": (_i32, [_vp, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _f32, _vp]),
     "infer_paged_prefill": (_i32, [_vp, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _f32, _vp]),
     "infer_paged_prefill_window": (_i32, [_vp, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _f32, _i32, _i32,
-                                          _vp, _sz, _vp]),
-    "infer_paged_prefill_window_workspace_bytes": (_sz, [_vp, _i64, _i32, _i32, _i32, _i32, _i32, _i32]),
+                                          _vp]),
     "infer_flash_attn_prefill": (_i32, [_vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _vp]),
     "infer_paged_decode_status": (_i32, [_vp, _vp]),
     "infer_prefill_status": (_i32, [_vp]),
@@ -74,7 +73,7 @@ SELFTEST_SIGNATURES = {
     "infer_selftest_paged_prefill": (_i32, [_vp, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _f32, _vp,
                                             _i32, _u32, _i32]),
     "infer_selftest_paged_prefill_window": (_i32, [_vp, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _f32, _i32,
-                                                   _i32, _vp, _sz, _vp, _u32, _i32]),
+                                                   _i32, _vp, _u32, _i32]),
     "infer_selftest_flash_attn_prefill": (_i32, [_vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _vp, _i32]),
 }
 

@@ -18,8 +18,10 @@
 //   memory and roles stay, and the Q and first K tiles of the next row block are loaded (and converted) while the softmax
 //   warps finish the current one.  Launched one by one, a CTA cost about 6 us beyond its tiles, a third of the time of a
 //   window of 1024 keys.
-// Few rows.  When the (row block, kv head, sequence) triples do not fill the GPU, the key tiles of a CTA are split over
-//   several, each leaving maximum, sum and accumulator per row in 32 bits, and a second kernel joins them.
+// Few rows.  When the (row block, kv head, sequence) triples do not fill the GPU, the key tiles of a row block are split over
+//   the CTAs of a cluster (up to 16), which join their parts through distributed shared memory: maxima and sums first, then
+//   every CTA scales its accumulator and leaves it in shared memory, and the rows are summed in turn.  No scratch in global
+//   memory, no second kernel.
 // e4m3.  S = Q K^T runs on the raw bytes of K (kind::f8f6f4, no conversion): a bf16 value has 8 significant bits, so it is
 //   the exact sum of two e4m3 values, its rounding to 4 bits and the rest.  The softmax warps split Q once per row block,
 //   each row scaled by a power of two that puts its largest value into [2^7, 2^8); values 2^-10 below that lose bits of the
@@ -37,6 +39,7 @@
 // Every wait is bounded; one that runs out raises the abort flag, every role drains to the common epilogue, tensor memory
 // is freed and the status word of the prefill kernels is set.
 #include <atomic>
+#include <mutex>
 
 #include "prefill.cuh"
 #include "tcgen05.cuh"
@@ -126,10 +129,7 @@ struct PwParams {
     int block_size, num_blocks;
     int window, sinks;       // window: 0x7fffffff = none
     float scale_log2;
-    int splits;              // CTAs that share the key tiles of a row block
-    int64_t total_q;
-    float* part_ml;          // splits > 1: [splits][total_q * n_q_heads][2] maximum (log2), sum
-    float* part_o;           // [splits][total_q * n_q_heads][128]
+    int splits;              // CTAs (of one cluster) that share the key tiles of a row block
     int* status;             // may be null
     uint32_t wait_limit;
     int stall_producer;
@@ -145,6 +145,28 @@ __device__ __forceinline__ bool tc_wait_idle(uint32_t bar, uint32_t parity, vola
     }
     *abort_flag = 1;
     return false;
+}
+
+// All threads of all CTAs of the cluster.  (No bound on the wait: every thread comes here whatever happened before, since the
+// waits in front of it are bounded, and the CTAs of a cluster are resident together.)
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+// The place in the shared memory of CTA `rank` of the cluster that corresponds to `addr` in this one's.
+__device__ __forceinline__ uint32_t cluster_addr(uint32_t addr, int rank) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ float2 ld_cluster_f2(uint32_t addr) {
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+    return v;
 }
 
 // Row t of a Q tile, 128 bf16 in two halves of 64 dims, becomes two rows of 128 e4m3 values in the same place whose sum it is
@@ -410,11 +432,11 @@ __global__ void __launch_bounds__(PwCfg<FP8>::threads, 1) prefill_window_kernel(
                                     } else ok = false;
                                 }
                                 v_slot = slot;
-                                if (ok && !asked && j + 2 >= n) ask();      // two tiles before the last load: the answer is there in time
+                                if (ok && !asked && p.splits == 1 && j + 2 >= n) ask();      // two tiles before the last load: the answer is there in time
                             }
                         }
                     }
-                    if (!ok) break;
+                    if (!ok || p.splits > 1) break;                         // (a cluster stays with its one row block)
                     if (!asked) ask();
                     if (!tc_wait(bar(PW_CLAIM), claims & 1, s_abort, p.wait_limit)) { ok = false; break; }
                     ++claims;
@@ -620,28 +642,26 @@ __global__ void __launch_bounds__(PwCfg<FP8>::threads, 1) prefill_window_kernel(
         const uint32_t p_addr = tmem + lane_sel + kPwTmemP + g * 64;
         const uint32_t o_addr = tmem + lane_sel + kPwTmemO + g * 128;
         int tiles = 0, uses = 0, q_uses = 0;                       // key tiles so far: of the CTA, of this query tile; Q loads so far
+        float m_ref = -INFINITY, l_run = 0.f;                      // reference maximum (log2 domain), row sum
+        float unit = 1.f;                                          // e4m3: V scale that O is expressed in
+        int blocks = 0;                                            // row blocks so far
 
         for (int item = 0; ok; ++item) {
         const volatile int* ie = item_wait(item);
         if (!ok) break;
         const int n_all = ie[PI_TILES];
         if (n_all < 0) break;
-        if (n_all == 0) {
-            // nothing is visible here: zeros, or an empty part
+        if (n_all == 0 && p.splits == 1) {                         // nothing is visible here: zeros
             const int tok0 = ie[PI_TOK0], q0 = ie[PI_Q0], head0 = ie[PI_KVH] * p.group;
             const int rows = min(ie[PI_LQ] - tok0, 2 * p.tokens) * p.group;
             for (int i = warp * 32 + lane; i < rows * 16; i += kPwSoftmaxWarps * 32) {
                 const int x = i >> 4;
                 const int64_t row = int64_t(q0 + tok0 + x / p.group) * p.n_q_heads + head0 + x % p.group;
-                if (p.splits == 1) {
-                    reinterpret_cast<uint4*>(p.out + row * kHeadDim)[i & 15] = make_uint4(0, 0, 0, 0);
-                } else if ((i & 15) == 0) {
-                    reinterpret_cast<float2*>(p.part_ml)[int64_t(ie[PI_SPLIT]) * p.total_q * p.n_q_heads + row] = make_float2(-INFINITY, 0.f);
-                }
+                reinterpret_cast<uint4*>(p.out + row * kHeadDim)[i & 15] = make_uint4(0, 0, 0, 0);
             }
         }
-        float m_ref = -INFINITY, l_run = 0.f;                      // reference maximum (log2 domain), row sum
-        float unit = 1.f;                                          // e4m3: V scale that O is expressed in
+        m_ref = -INFINITY;
+        l_run = 0.f;
         float c_row = p.scale_log2;
         int left = g == 0 || ie[PI_TWO] ? n_all : 0;
         if (left == 0) tiles += n_all;                             // this query tile has no rows
@@ -764,15 +784,13 @@ __global__ void __launch_bounds__(PwCfg<FP8>::threads, 1) prefill_window_kernel(
         }
         // O is complete once the last P V has retired
         if (any_tile && ok && !tc_wait(bar(PW_PV_DONE, g), (uses - 1) & 1, s_abort, p.wait_limit)) ok = false;
-        if (any_tile && ok) {
+        if (any_tile && ok && p.splits == 1) {
             tc_fence_after();
             const bool any = l_run != 0.f;                          // a row that sees nothing gives zeros
-            const float f = p.splits > 1 ? unit : unit / l_run;
+            const float f = unit / l_run;
             const int tok = ie[PI_TOK0] + g * p.tokens + r / p.group;
             const bool live = r < p.tokens * p.group && tok < ie[PI_LQ];      // rows behind the tokens of the tile or the sequence hold anything
             const int64_t row = int64_t(ie[PI_Q0] + tok) * p.n_q_heads + ie[PI_KVH] * p.group + r % p.group;
-            const int64_t part = int64_t(ie[PI_SPLIT]) * p.total_q * p.n_q_heads + row;
-            if (p.splits > 1 && live) reinterpret_cast<float2*>(p.part_ml)[part] = make_float2(any ? m_ref : -INFINITY, l_run);
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
                 uint32_t v[32];
@@ -781,28 +799,95 @@ __global__ void __launch_bounds__(PwCfg<FP8>::threads, 1) prefill_window_kernel(
                 if (!live) continue;
 #pragma unroll
                 for (int i = 0; i < 32; ++i) v[i] = any ? __float_as_uint(__uint_as_float(v[i]) * f) : 0u;
-                if (p.splits > 1) {
-                    uint4* dst = reinterpret_cast<uint4*>(p.part_o + part * kHeadDim + c * 32);
+                uint4* dst = reinterpret_cast<uint4*>(p.out + row * kHeadDim + c * 32);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) dst[i] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-                } else {
-                    uint4* dst = reinterpret_cast<uint4*>(p.out + row * kHeadDim + c * 32);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        uint4 w;
-                        w.x = pack_bf16(__uint_as_float(v[8 * i]), __uint_as_float(v[8 * i + 1]));
-                        w.y = pack_bf16(__uint_as_float(v[8 * i + 2]), __uint_as_float(v[8 * i + 3]));
-                        w.z = pack_bf16(__uint_as_float(v[8 * i + 4]), __uint_as_float(v[8 * i + 5]));
-                        w.w = pack_bf16(__uint_as_float(v[8 * i + 6]), __uint_as_float(v[8 * i + 7]));
-                        dst[i] = w;
-                    }
+                for (int i = 0; i < 4; ++i) {
+                    uint4 w;
+                    w.x = pack_bf16(__uint_as_float(v[8 * i]), __uint_as_float(v[8 * i + 1]));
+                    w.y = pack_bf16(__uint_as_float(v[8 * i + 2]), __uint_as_float(v[8 * i + 3]));
+                    w.z = pack_bf16(__uint_as_float(v[8 * i + 4]), __uint_as_float(v[8 * i + 5]));
+                    w.w = pack_bf16(__uint_as_float(v[8 * i + 6]), __uint_as_float(v[8 * i + 7]));
+                    dst[i] = w;
                 }
             }
             tc_fence_before();
         }
+        ++blocks;
         q_uses += ie[PI_TILES] > 0;
         item_done(item);
         }
+
+        if (p.splits > 1) {
+            // ------------------------------------------------------------- joins the parts of the cluster's row block
+            // maximum and sum of a row: over this query tile's Q, which no product needs any more
+            const uint32_t ml = base + C::q + g * kPwTile + r * 8;
+            asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(ml), "f"(m_ref), "f"(l_run) : "memory");
+            cluster_sync();                                        // (and every product of this CTA has retired)
+            const volatile int* ie = s_item;
+            const int tile_rows = p.tokens * p.group;
+            int tok0 = 0, rank = 0, rows = 0;                      // a cluster whose row block lies behind its sequence joins nothing
+            if (blocks > 0) {
+                tok0 = ie[PI_TOK0];
+                rank = ie[PI_SPLIT];
+                rows = min(ie[PI_LQ] - tok0, 2 * p.tokens) * p.group;
+            }
+            const uint32_t o_part = base + C::k;                   // [256][128] f32, 16-byte chunks swizzled by the row
+            if (r < tile_rows && g * tile_rows + r < rows) {
+                float m_all = -INFINITY, l_all = 0.f;
+                for (int k = 0; k < p.splits; ++k) {
+                    const float2 x = ld_cluster_f2(cluster_addr(ml, k));
+                    if (x.y != 0.f) m_all = fmaxf(m_all, x.x);     // a sum of 0: this part of the keys is hidden from the row
+                }
+                for (int k = 0; k < p.splits; ++k) {
+                    const float2 x = ld_cluster_f2(cluster_addr(ml, k));
+                    if (x.y != 0.f) l_all = fmaf(x.y, fast_exp2(x.x - m_all), l_all);
+                }
+                m_ref = l_run != 0.f ? fast_exp2(m_ref - m_all) * unit / l_all : 0.f;      // factor of this part
+            }
+            __syncwarp();
+            tc_fence_after();
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                uint32_t v[32];
+                tc_ld32(o_addr + c * 32, v);
+                tc_wait_ld();
+                if (r >= tile_rows || g * tile_rows + r >= rows) continue;
+                const uint32_t dst = o_part + (g * kPwRows + r) * 512;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    uint4 w;
+                    w.x = l_run != 0.f ? __float_as_uint(__uint_as_float(v[4 * i]) * m_ref) : 0u;
+                    w.y = l_run != 0.f ? __float_as_uint(__uint_as_float(v[4 * i + 1]) * m_ref) : 0u;
+                    w.z = l_run != 0.f ? __float_as_uint(__uint_as_float(v[4 * i + 2]) * m_ref) : 0u;
+                    w.w = l_run != 0.f ? __float_as_uint(__uint_as_float(v[4 * i + 3]) * m_ref) : 0u;
+                    st_shared_v4(dst + (((c * 8 + i) ^ (r & 31)) << 4), w);
+                }
+            }
+            tc_fence_before();
+            cluster_sync();
+            // rows in turn over the CTAs and their warps, four dims per lane
+            for (int x = rank + p.splits * warp; x < rows; x += p.splits * kPwSoftmaxWarps) {
+                const int t = x / tile_rows, xr = x - t * tile_rows;
+                const uint32_t src = o_part + (t * kPwRows + xr) * 512 + ((lane ^ (xr & 31)) << 4);
+                float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+                for (int k = 0; k < p.splits; ++k) {
+                    const float4 v = ld_cluster_f4(cluster_addr(src, k));
+                    o.x += v.x;
+                    o.y += v.y;
+                    o.z += v.z;
+                    o.w += v.w;
+                }
+                const int64_t row = int64_t(ie[PI_Q0] + tok0 + x / p.group) * p.n_q_heads + ie[PI_KVH] * p.group + x % p.group;
+                *reinterpret_cast<uint2*>(p.out + row * kHeadDim + lane * 4) = make_uint2(pack_bf16(o.x, o.y), pack_bf16(o.z, o.w));
+            }
+            cluster_sync();                                        // nobody leaves while another CTA reads its shared memory
+        }
+    }
+    if (p.splits > 1 && (hw < 4 || hw >= 12)) {                    // the other warps' share of the three barriers
+        __syncwarp();
+        cluster_sync();
+        cluster_sync();
+        cluster_sync();
     }
 
     // ===================================================================== common epilogue
@@ -815,71 +900,95 @@ __global__ void __launch_bounds__(PwCfg<FP8>::threads, 1) prefill_window_kernel(
     if (threadIdx.x == 0 && *s_abort && p.status) atomicExch(p.status, 0x5AFE0006);
 }
 
-// Joins the parts of every (token, head): a warp per row.  Rows outside of the sequences are left alone.
-__global__ void __launch_bounds__(256) prefill_join_kernel(__nv_bfloat16* out, const float* part_ml, const float* part_o,
-                                                           const int32_t* cu_q, int batch, int64_t rows, int n_q_heads, int splits) {
-    const int64_t row = (int64_t(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
-    const int lane = threadIdx.x & 31;
-    if (row < int64_t(cu_q[0]) * n_q_heads || row >= min(int64_t(cu_q[batch]) * n_q_heads, rows)) return;
-    const float2* ml = reinterpret_cast<const float2*>(part_ml) + row;
-    float m = -INFINITY;
-    for (int s = 0; s < splits; ++s) m = fmaxf(m, ml[s * rows].x);
-    float l = 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int s = 0; s < splits; ++s) {
-        const float2 x = ml[s * rows];
-        if (x.y == 0.f) continue;                       // saw nothing of this part; its accumulator is not written
-        const float a = exp2f(x.x - m);
-        const float4 v = reinterpret_cast<const float4*>(part_o + (s * rows + row) * kHeadDim)[lane];
-        l = fmaf(x.y, a, l);
-        o.x = fmaf(v.x, a, o.x);
-        o.y = fmaf(v.y, a, o.y);
-        o.z = fmaf(v.z, a, o.z);
-        o.w = fmaf(v.w, a, o.w);
+// What a launch over clusters needs to know of a device: how many clusters of 2, 4, 8 and 16 CTAs fit at a time.
+struct PwDevice {
+    std::atomic<bool> ready{false};
+    int clusters[4] = {0, 0, 0, 0};
+};
+
+// The launch configuration; attr has to outlive it.
+static cudaLaunchConfig_t prefill_config(dim3 grid, int threads, int smem, int splits, cudaStream_t st, cudaLaunchAttribute* attr) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    if (splits > 1) {
+        attr->id = cudaLaunchAttributeClusterDimension;
+        attr->val.clusterDim.x = 1;
+        attr->val.clusterDim.y = splits;
+        attr->val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
     }
-    const float f = l != 0.f ? 1.f / l : 0.f;
-    uint2 w;
-    w.x = pack_bf16(o.x * f, o.y * f);
-    w.y = pack_bf16(o.z * f, o.w * f);
-    *reinterpret_cast<uint2*>(out + row * kHeadDim + lane * 4) = w;
+    return cfg;
 }
 
-// Over how many CTAs the key tiles of a row block are spread: as many as keep every SM at one CTA, when a CTA has at
-// least four tiles to give away (one tile costs about 1.5 us, setting a CTA up and joining the parts about 5).
-static int prefill_splits(const infer_kv_pool* pool, int batch, int max_q, int max_k, int n_q_heads, int window, int sinks) {
-    const int group = n_q_heads / pool->n_kv_heads, tokens = kPwRows / group;
-    const int64_t blocks = int64_t((max_q + 2 * tokens - 1) / (2 * tokens)) * pool->n_kv_heads * batch;
-    int64_t tiles = (int64_t(max_k) + kPwKeys - 1) / kPwKeys;
+// Shared-memory limit and cluster counts of the current device, looked up once.
+template <bool FP8>
+static int prefill_device(const PwDevice** out) {
+    static PwDevice devices[64];
+    static std::mutex mutex;
+    int dev = 0;
+    IB_CUDA(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64) {
+        set_cuda_error(cudaErrorInvalidDevice);
+        return INFER_ERR_CUDA;
+    }
+    PwDevice& d = devices[dev];
+    *out = &d;
+    if (d.ready.load(std::memory_order_acquire)) return INFER_OK;
+    std::lock_guard<std::mutex> lock(mutex);
+    const int smem = PwCfg<FP8>::total + 1024;
+    IB_CUDA(cudaFuncSetAttribute(prefill_window_kernel<FP8>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    IB_CUDA(cudaFuncSetAttribute(prefill_window_kernel<FP8>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    for (int i = 0; i < 4; ++i) {
+        cudaLaunchAttribute attr;
+        const int size = 2 << i;
+        const cudaLaunchConfig_t cfg = prefill_config(dim3(1, size, 1), PwCfg<FP8>::threads, smem, size, nullptr, &attr);
+        int n = 0;
+        if (cudaOccupancyMaxActiveClusters(&n, prefill_window_kernel<FP8>, &cfg) != cudaSuccess) {
+            (void)cudaGetLastError();
+            n = 0;
+        }
+        d.clusters[i] = n;
+    }
+    d.ready.store(true, std::memory_order_release);
+    return INFER_OK;
+}
+
+// Over how many CTAs the key tiles of a row block are spread: the largest cluster size of which all row blocks run at the
+// same time and that leaves every CTA three tiles or more (a tile takes about 1.6 us, the join 4).
+static int prefill_splits(const PwDevice& d, int64_t blocks, int64_t max_k, int tokens, int window, int sinks) {
+    int64_t tiles = (max_k + kPwKeys - 1) / kPwKeys;
     if (window > 0) {
         const int64_t seen = (int64_t(window) + 2 * tokens + kPwKeys - 1) / kPwKeys + 1 + (int64_t(sinks) + kPwKeys - 1) / kPwKeys;
         if (seen < tiles) tiles = seen;
     }
-    int64_t splits = blocks > 0 ? pool->sm_count / blocks : 1;
-    if (splits > tiles / 2) splits = tiles / 2;
-    return splits < 1 ? 1 : int(splits);
+    for (int i = 3; i >= 0; --i)
+        if (blocks <= d.clusters[i] && tiles >= int64_t(3) * (2 << i)) return 2 << i;
+    return 1;
 }
 
-static size_t prefill_part_bytes(int splits, int64_t rows) { return size_t(splits) * rows * (2 + kHeadDim) * sizeof(float); }
-
 template <bool FP8>
-static int launch_prefill_window(const PwParams& p, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, dim3 grid,
-                                 cudaStream_t st) {
-    const int smem = PwCfg<FP8>::total + 1024;
-    static std::atomic<bool> prepared[64];     // the shared-memory limit is raised once per device
-    int dev = 0;
-    IB_CUDA(cudaGetDevice(&dev));
-    if (dev < 0 || dev >= 64 || !prepared[dev].load(std::memory_order_acquire)) {
-        IB_CUDA(cudaFuncSetAttribute(prefill_window_kernel<FP8>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-        if (dev >= 0 && dev < 64) prepared[dev].store(true, std::memory_order_release);
-    }
-    prefill_window_kernel<FP8><<<grid, PwCfg<FP8>::threads, smem, st>>>(p, mq, mk, mv);
+static int launch_prefill_window(PwParams& p, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, int max_q, int max_k,
+                                 int window, int batch, cudaStream_t st) {
+    const PwDevice* d = nullptr;
+    const int rc = prefill_device<FP8>(&d);
+    if (rc != INFER_OK) return rc;
+    const int64_t row_blocks = (int64_t(max_q) + 2 * p.tokens - 1) / (2 * p.tokens);
+    p.splits = prefill_splits(*d, row_blocks * p.n_kv_heads * batch, max_k, p.tokens, window, p.sinks);
+    cudaLaunchAttribute attr;
+    const cudaLaunchConfig_t cfg = prefill_config(dim3(unsigned(row_blocks), p.n_kv_heads * p.splits, batch), PwCfg<FP8>::threads,
+                                                  PwCfg<FP8>::total + 1024, p.splits, st, &attr);
+    IB_CUDA(cudaLaunchKernelEx(&cfg, prefill_window_kernel<FP8>, PwParams(p), mq, mk, mv));
     return check_launch();
 }
 
 static int paged_prefill_window(const infer_kv_pool_t* pool, void* out, const void* q, int64_t total_q, const int32_t* cu_seqlens_q,
                                 const int32_t* cu_seqlens_k, const int32_t* block_tables, int64_t bt_stride, int batch,
-                                int max_seqlen_q, int max_seqlen_k, int n_q_heads, float softmax_scale, int window, int sinks,
-                                void* workspace, size_t workspace_bytes, cudaStream_t st, uint32_t wait_limit, int stall_producer) {
+                                int max_seqlen_q, int max_seqlen_k, int n_q_heads, float softmax_scale, int window, int sinks, cudaStream_t st,
+                                uint32_t wait_limit, int stall_producer) {
     if (!(softmax_scale > 0.f) || !(softmax_scale < INFINITY) || window < 0 || sinks < 0) return INFER_ERR_GEOMETRY;
     if (!pool || !out || !q || !cu_seqlens_q || !cu_seqlens_k || !block_tables) return INFER_ERR_NULL;
     if (batch < 0 || n_q_heads <= 0 || n_q_heads % pool->n_kv_heads != 0 || n_q_heads / pool->n_kv_heads > kPwRows || bt_stride <= 0 ||
@@ -887,11 +996,7 @@ static int paged_prefill_window(const infer_kv_pool_t* pool, void* out, const vo
         total_q > int64_t(batch) * max_seqlen_q || total_q >= (int64_t(1) << 31))
         return INFER_ERR_GEOMETRY;
     if (!aligned16(out) || !aligned16(q)) return INFER_ERR_ALIGN;
-    if (workspace && !aligned16(workspace)) return INFER_ERR_WORKSPACE;
     if (total_q == 0 || batch == 0) return INFER_OK;
-    const int64_t rows = total_q * n_q_heads;
-    int splits = prefill_splits(pool, batch, max_seqlen_q, max_seqlen_k, n_q_heads, window, sinks);
-    while (splits > 1 && (!workspace || prefill_part_bytes(splits, rows) > workspace_bytes)) --splits;
     PwParams p{};
     p.out = static_cast<__nv_bfloat16*>(out);
     p.cu_q = cu_seqlens_q;
@@ -909,12 +1014,6 @@ static int paged_prefill_window(const infer_kv_pool_t* pool, void* out, const vo
     p.window = window > 0 ? window : 0x7fffffff;
     p.sinks = sinks;
     p.scale_log2 = softmax_scale * 1.4426950408889634f;
-    p.splits = splits;
-    p.total_q = total_q;
-    if (splits > 1) {
-        p.part_o = static_cast<float*>(workspace);
-        p.part_ml = p.part_o + size_t(splits) * rows * kHeadDim;
-    }
     p.status = prefill_status_word();
     p.wait_limit = wait_limit;
     p.stall_producer = stall_producer;
@@ -922,45 +1021,32 @@ static int paged_prefill_window(const infer_kv_pool_t* pool, void* out, const vo
     int rc = encode_map_3d(&mq, q, 2, kHeadDim, uint64_t(n_q_heads), uint64_t(total_q), 256, uint64_t(n_q_heads) * 256, 64,
                            uint32_t(p.group), uint32_t(p.tokens));
     if (rc != INFER_OK) return rc;
-    const dim3 grid((max_seqlen_q + 2 * p.tokens - 1) / (2 * p.tokens), pool->n_kv_heads * splits, batch);
-    if (pool->dtype == INFER_KV_E4M3) rc = launch_prefill_window<true>(p, mq, pool->maps[3].k, pool->maps[3].v, grid, st);
-    else rc = launch_prefill_window<false>(p, mq, pool->maps[3].k, pool->maps[3].v, grid, st);
-    if (rc != INFER_OK || splits == 1) return rc;
-    prefill_join_kernel<<<unsigned((rows + 7) / 8), 256, 0, st>>>(p.out, p.part_ml, p.part_o, cu_seqlens_q, batch, rows, n_q_heads,
-                                                                  splits);
-    return check_launch();
+    if (pool->dtype == INFER_KV_E4M3)
+        return launch_prefill_window<true>(p, mq, pool->maps[3].k, pool->maps[3].v, max_seqlen_q, max_seqlen_k, window, batch, st);
+    return launch_prefill_window<false>(p, mq, pool->maps[3].k, pool->maps[3].v, max_seqlen_q, max_seqlen_k, window, batch, st);
 }
 
 }  // namespace ib
 
 extern "C" {
 
-size_t infer_paged_prefill_window_workspace_bytes(const infer_kv_pool_t* pool, int64_t total_q, int batch, int max_seqlen_q,
-                                                  int max_seqlen_k, int n_q_heads, int window, int sinks) {
-    if (!pool || total_q <= 0 || batch <= 0 || n_q_heads <= 0 || n_q_heads % pool->n_kv_heads != 0 ||
-        n_q_heads / pool->n_kv_heads > ib::kPwRows || max_seqlen_q < 0 || max_seqlen_k < 0 || window < 0 || sinks < 0)
-        return 0;
-    const int splits = ib::prefill_splits(pool, batch, max_seqlen_q, max_seqlen_k, n_q_heads, window, sinks);
-    return splits > 1 ? ib::prefill_part_bytes(splits, total_q * n_q_heads) : 0;
-}
-
 int infer_paged_prefill_window(const infer_kv_pool_t* pool, void* out, const void* q, int64_t total_q, const int32_t* cu_seqlens_q,
                                const int32_t* cu_seqlens_k, const int32_t* block_tables, int64_t bt_stride, int batch,
                                int max_seqlen_q, int max_seqlen_k, int n_q_heads, float softmax_scale, int window, int sinks,
-                               void* workspace, size_t workspace_bytes, void* stream_) {
+                               void* stream_) {
     return ib::paged_prefill_window(pool, out, q, total_q, cu_seqlens_q, cu_seqlens_k, block_tables, bt_stride, batch, max_seqlen_q,
-                                    max_seqlen_k, n_q_heads, softmax_scale, window, sinks, workspace, workspace_bytes,
-                                    static_cast<cudaStream_t>(stream_), ib::kDefaultWaitLimit, 0);
+                                    max_seqlen_k, n_q_heads, softmax_scale, window, sinks, static_cast<cudaStream_t>(stream_),
+                                    ib::kDefaultWaitLimit, 0);
 }
 
 int infer_selftest_paged_prefill_window(const infer_kv_pool_t* pool, void* out, const void* q, int64_t total_q,
                                         const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, const int32_t* block_tables,
                                         int64_t bt_stride, int batch, int max_seqlen_q, int max_seqlen_k, int n_q_heads,
-                                        float softmax_scale, int window, int sinks, void* workspace, size_t workspace_bytes,
-                                        void* stream_, uint32_t wait_limit, int stall_producer) {
+                                        float softmax_scale, int window, int sinks, void* stream_, uint32_t wait_limit,
+                                        int stall_producer) {
     return ib::paged_prefill_window(pool, out, q, total_q, cu_seqlens_q, cu_seqlens_k, block_tables, bt_stride, batch, max_seqlen_q,
-                                    max_seqlen_k, n_q_heads, softmax_scale, window, sinks, workspace, workspace_bytes,
-                                    static_cast<cudaStream_t>(stream_), wait_limit ? wait_limit : ib::kDefaultWaitLimit, stall_producer);
+                                    max_seqlen_k, n_q_heads, softmax_scale, window, sinks, static_cast<cudaStream_t>(stream_),
+                                    wait_limit ? wait_limit : ib::kDefaultWaitLimit, stall_producer);
 }
 
 }  // extern "C"

@@ -463,14 +463,13 @@ def paged_attn_decode_append(q, key, value, k_cache, v_cache, cache_seqlens, blo
 
 # --------------------------------------------------------------------------- prefill
 def paged_attn_prefill(q, k_cache, v_cache, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k,
-                       softmax_scale, block_table, out=None, k_scale=None, v_scale=None, window=None, sinks=0, workspace=None):
+                       softmax_scale, block_table, out=None, k_scale=None, v_scale=None, window=None, sinks=0):
     """q [total_q, Hq, 128]; keys come from the pools through block_table; causal,
     bottom-right aligned (the flash_attn_varlen_func convention).
 
     e4m3 pools come with their ``k_scale`` / ``v_scale``.  ``window`` / ``sinks``: a query sees the ``window`` keys up to its
     own position and the first ``sinks`` of its sequence; entries of ``block_table`` for pages without a visible key are not
-    read.  With either, a query that sees no key gives zeros.  ``workspace``: uint8 scratch for chunks of few rows over many
-    keys (see ``infer_paged_prefill_window``); by default it comes from the allocator of the current stream, call by call."""
+    read.  With either, a query that sees no key gives zeros."""
     if q.dtype != torch.bfloat16 or not q.is_contiguous() or q.dim() != 3:
         raise RuntimeError("paged_attn_prefill: q must be contiguous bf16 [total_q, Hq, 128]")
     for name, t in (("cu_seqlens_q", cu_seqlens_q), ("cu_seqlens_k", cu_seqlens_k), ("block_table", block_table)):
@@ -483,11 +482,7 @@ def paged_attn_prefill(q, k_cache, v_cache, cu_seqlens_q, cu_seqlens_k, max_seql
     batch, args = cu_seqlens_q.numel() - 1, ()
     if pool.fp8 or window:
         _check_prefill_window(q, o, cu_seqlens_q, cu_seqlens_k, block_table, batch, pool)
-        need = lib.infer_paged_prefill_window_workspace_bytes(pool.handle, q.shape[0], batch, int(max_seqlen_q), int(max_seqlen_k),
-                                                              q.shape[1], window, sinks)
-        if workspace is None and need:
-            workspace = torch.empty(need, dtype=torch.uint8, device=pool.device)
-        args = (window, sinks, _ptr(workspace), workspace.numel() if workspace is not None else 0)
+        args = (window, sinks)
     with _on_device(pool.device):
         rc = (_call_prefill_window if args else _call_prefill)(
             lib, pool.handle, _ptr(o), _ptr(q), q.shape[0], _ptr(cu_seqlens_q), _ptr(cu_seqlens_k), _ptr(block_table),
