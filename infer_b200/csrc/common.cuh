@@ -128,6 +128,36 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, uint32_
     return false;
 }
 
+// Thirty-two bytes of global memory per lane.
+struct Bytes32 {
+    uint4 lo, hi;
+};
+// 32 bytes at once (WIDE: the address is a multiple of 32), or twice 16
+template <bool WIDE>
+__device__ __forceinline__ Bytes32 load32(const void* p) {
+    Bytes32 v;
+    if constexpr (WIDE) {
+        asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=r"(v.lo.x), "=r"(v.lo.y), "=r"(v.lo.z), "=r"(v.lo.w), "=r"(v.hi.x), "=r"(v.hi.y), "=r"(v.hi.z), "=r"(v.hi.w)
+                     : "l"(p));
+    } else {
+        v.lo = static_cast<const uint4*>(p)[0];
+        v.hi = static_cast<const uint4*>(p)[1];
+    }
+    return v;
+}
+template <bool WIDE>
+__device__ __forceinline__ void store32(void* p, const Bytes32& v) {
+    if constexpr (WIDE) {
+        asm volatile("st.global.v8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};"
+                     ::"r"(v.lo.x), "r"(v.lo.y), "r"(v.lo.z), "r"(v.lo.w), "r"(v.hi.x), "r"(v.hi.y), "r"(v.hi.z), "r"(v.hi.w), "l"(p)
+                     : "memory");
+    } else {
+        static_cast<uint4*>(p)[0] = v.lo;
+        static_cast<uint4*>(p)[1] = v.hi;
+    }
+}
+
 // 3-D tiled TMA load global -> shared of this CTA, completion on an mbarrier.
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x,
                                             int y, int z) {

@@ -12,8 +12,10 @@
 //
 // Bound by HBM: (Hq + 2 Hkv) rows of 256 bytes read, as many written.  Eight lanes per head, two 16-byte chunks of
 // eight dims per lane, chosen so that a pair never leaves its lane: in the half layout lane s < rot_dim / 16 owns chunks
-// s and s + rot_dim / 16, the other lanes two adjacent chunks of the untouched tail; in the interleaved layout every
-// chunk holds whole pairs and lane s owns chunks s and s + 8.
+// s and s + rot_dim / 16, the other lanes two adjacent chunks of the untouched tail; in the interleaved layout lane s owns
+// the adjacent chunks 2s and 2s + 1, which it moves with 32-byte loads and stores where the addresses allow.
+// Measured (32q/8kv heads): 32768 tokens half layout 125-128 us (6.3-6.4 TB/s of the bytes that have to move, 0.97 of the copy
+// peak); 5001 tokens of 64q/8kv heads interleaved, half a head rotated: see kRotQuads.
 #include "common.cuh"
 
 namespace ib {
@@ -37,20 +39,25 @@ struct RotaryArgs {
     float factor;
 };
 
-constexpr int kRotQuads = 6;         // heads of one work item: four per load instruction, six instructions
-
+// Heads of one work item: four per load instruction, six or four instructions.  Swept, us at 6 / 5 / 4 / 3: half layout,
+// 32768 tokens of 48 heads 128 / 139 / 137 / 132; interleaved, 5001 tokens of 80 heads 40.2 / 38.9 / 35.9 / 38.2 (four loads
+// leave room for three blocks per SM).
 template <bool INTERLEAVED>
-__global__ void __launch_bounds__(256) rotary_append_kernel(RotaryArgs a) {
+constexpr int kRotQuads = INTERLEAVED ? 4 : 6;
+
+template <bool INTERLEAVED, bool WIDE>
+__global__ void __launch_bounds__(256, INTERLEAVED ? 3 : 2) rotary_append_kernel(RotaryArgs a) {
+    constexpr int Q = kRotQuads<INTERLEAVED>;
     const bool append = a.v != nullptr;
     const int qk_heads = a.n_q_heads + a.n_kv_heads;
     const int heads = append ? qk_heads + a.n_kv_heads : qk_heads;
-    const int batches = (heads + 4 * kRotQuads - 1) / (4 * kRotQuads);
+    const int batches = (heads + 4 * Q - 1) / (4 * Q);
     const int lane = threadIdx.x & 31, sub = lane & 7, grp = lane >> 3;
     const int m = a.rot_chunks;
     // the two chunks of eight dims of this lane, and whether they are rotated
-    const int c0 = INTERLEAVED || sub < m ? sub : 2 * sub;
-    const int c1 = INTERLEAVED ? sub + 8 : sub < m ? sub + m : 2 * sub + 1;
-    const bool rot0 = INTERLEAVED ? c0 < 2 * m : sub < m, rot1 = INTERLEAVED ? c1 < 2 * m : sub < m;
+    const bool rotated = sub < m;
+    const int c0 = !INTERLEAVED && rotated ? sub : 2 * sub;
+    const int c1 = !INTERLEAVED && rotated ? sub + m : 2 * sub + 1;
     const int64_t n_items = a.n_tokens * batches;
     const int64_t n_warps = (int64_t(gridDim.x) * blockDim.x) >> 5;
     // turns per position of pairs `lane` and `lane + 32`
@@ -58,24 +65,30 @@ __global__ void __launch_bounds__(256) rotary_append_kernel(RotaryArgs a) {
     const double turns1 = lane + 32 < 8 * m ? a.inv_freq[lane + 32] * 0.15915494309189535 : 0.0;
     for (int64_t item = (int64_t(blockIdx.x) * blockDim.x + threadIdx.x) >> 5; item < n_items; item += n_warps) {
         const int64_t tok = item / batches;
-        const int h0 = int(item - tok * batches) * 4 * kRotQuads;
+        const int h0 = int(item - tok * batches) * 4 * Q;
         const int64_t slot = append ? int64_t(a.slot_mapping[tok]) : tok;
         const bool slot_ok = !append || (slot >= 0 && slot < a.num_slots);     // false: padding row of a captured batch
         const double pos = double(a.positions[tok]);
         // every load of the item before any arithmetic
-        uint4 x[kRotQuads], y[kRotQuads];
-        int h[kRotQuads];
+        uint4 x[Q], y[Q];
+        int h[Q];
 #pragma unroll
-        for (int j = 0; j < kRotQuads; ++j) {
+        for (int j = 0; j < Q; ++j) {
             h[j] = h0 + 4 * j + grp;
             const int hh = min(h[j], heads - 1);                   // a lane group past the last head re-reads it and stores nothing
             const __nv_bfloat16* src = hh < a.n_q_heads ? a.q + tok * a.q_pitch + hh * kHeadDim
                                      : hh < qk_heads    ? a.k + tok * a.k_pitch + (hh - a.n_q_heads) * kHeadDim
                                                         : a.v + tok * a.v_pitch + (hh - qk_heads) * kHeadDim;
-            x[j] = *reinterpret_cast<const uint4*>(src + 8 * c0);
-            y[j] = *reinterpret_cast<const uint4*>(src + 8 * c1);
+            if constexpr (INTERLEAVED) {
+                const Bytes32 w = load32<WIDE>(src + 8 * c0);
+                x[j] = w.lo;
+                y[j] = w.hi;
+            } else {
+                x[j] = *reinterpret_cast<const uint4*>(src + 8 * c0);
+                y[j] = *reinterpret_cast<const uint4*>(src + 8 * c1);
+            }
         }
-        // the token's angles: pairs lane and lane + 32, then pair 8 s + i (half) or 4 c + i (interleaved) by shuffle
+        // the token's angles: pairs lane and lane + 32; this lane's eight pairs are 8 sub .. 8 sub + 7 in either layout
         float cs[8], sn[8];
         {
             const double t0 = pos * turns0, t1 = pos * turns1;
@@ -85,19 +98,17 @@ __global__ void __launch_bounds__(256) rotary_append_kernel(RotaryArgs a) {
             s0 *= a.factor; co0 *= a.factor; s1 *= a.factor; co1 *= a.factor;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                // interleaved: chunk c0 = sub holds pairs 4 sub .. 4 sub + 3 (below 32), chunk c1 pairs 32 + 4 sub ..
-                const int pair = INTERLEAVED ? 4 * sub + (i & 3) : 8 * sub + i;
+                const int pair = 8 * sub + i;
                 const float clo = __shfl_sync(0xffffffffu, co0, pair & 31), chi = __shfl_sync(0xffffffffu, co1, pair & 31);
                 const float slo = __shfl_sync(0xffffffffu, s0, pair & 31), shi = __shfl_sync(0xffffffffu, s1, pair & 31);
-                const bool high = INTERLEAVED ? i >= 4 : pair >= 32;
-                cs[i] = high ? chi : clo;
-                sn[i] = high ? shi : slo;
+                cs[i] = pair >= 32 ? chi : clo;
+                sn[i] = pair >= 32 ? shi : slo;
             }
         }
 #pragma unroll
-        for (int j = 0; j < kRotQuads; ++j) {
+        for (int j = 0; j < Q; ++j) {
             if (h[j] >= heads) continue;                           // uniform over the 8 lanes of a group
-            if (h[j] < qk_heads) {
+            if (h[j] < qk_heads && rotated) {
                 uint32_t* xr = reinterpret_cast<uint32_t*>(&x[j]);
                 uint32_t* yr = reinterpret_cast<uint32_t*>(&y[j]);
 #pragma unroll
@@ -105,9 +116,9 @@ __global__ void __launch_bounds__(256) rotary_append_kernel(RotaryArgs a) {
                     const float2 u = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&xr[i]));
                     const float2 w = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&yr[i]));
                     if (INTERLEAVED) {
-                        if (rot0) xr[i] = pack_bf16(u.x * cs[i] - u.y * sn[i], u.y * cs[i] + u.x * sn[i]);
-                        if (rot1) yr[i] = pack_bf16(w.x * cs[4 + i] - w.y * sn[4 + i], w.y * cs[4 + i] + w.x * sn[4 + i]);
-                    } else if (rot0) {
+                        xr[i] = pack_bf16(u.x * cs[i] - u.y * sn[i], u.y * cs[i] + u.x * sn[i]);
+                        yr[i] = pack_bf16(w.x * cs[4 + i] - w.y * sn[4 + i], w.y * cs[4 + i] + w.x * sn[4 + i]);
+                    } else {
                         xr[i] = pack_bf16(u.x * cs[2 * i] - w.x * sn[2 * i], u.y * cs[2 * i + 1] - w.y * sn[2 * i + 1]);
                         yr[i] = pack_bf16(w.x * cs[2 * i] + u.x * sn[2 * i], w.y * cs[2 * i + 1] + u.y * sn[2 * i + 1]);
                     }
@@ -121,8 +132,12 @@ __global__ void __launch_bounds__(256) rotary_append_kernel(RotaryArgs a) {
                 dst = h[j] < qk_heads ? a.k_out + slot * a.k_out_pitch + (h[j] - a.n_q_heads) * kHeadDim
                                       : a.v_out + slot * a.k_out_pitch + (h[j] - qk_heads) * kHeadDim;
             }
-            *reinterpret_cast<uint4*>(dst + 8 * c0) = x[j];
-            *reinterpret_cast<uint4*>(dst + 8 * c1) = y[j];
+            if constexpr (INTERLEAVED) {
+                store32<WIDE>(dst + 8 * c0, Bytes32{x[j], y[j]});
+            } else {
+                *reinterpret_cast<uint4*>(dst + 8 * c0) = x[j];
+                *reinterpret_cast<uint4*>(dst + 8 * c1) = y[j];
+            }
         }
     }
 }
@@ -144,12 +159,18 @@ static int rotary(RotaryArgs& a, const void* q_out, int64_t q_out_stride, const 
     a.rot_chunks = rot_dim / 16;
     a.factor = factor;
     const int heads = n_q_heads + (a.v ? 2 : 1) * n_kv_heads;
-    const int64_t items = n_tokens * ((heads + 4 * kRotQuads - 1) / (4 * kRotQuads));      // one warp each
+    const int per = 4 * (interleaved ? kRotQuads<true> : kRotQuads<false>);
+    const int64_t items = n_tokens * ((heads + per - 1) / per);                            // one warp each
     int64_t blocks = (items + 7) / 8;
     const int64_t cap = int64_t(sm_count) * 16;                                            // grid-stride beyond that
     if (blocks > cap) blocks = cap;
-    if (interleaved) rotary_append_kernel<true><<<unsigned(blocks), 256, 0, st>>>(a);
-    else rotary_append_kernel<false><<<unsigned(blocks), 256, 0, st>>>(a);
+    // 32-byte accesses of the interleaved layout: every row at a multiple of 32 bytes
+    auto at32 = [](const void* p, int64_t stride) { return (reinterpret_cast<uintptr_t>(p) & 31) == 0 && stride % 16 == 0; };
+    const bool wide = at32(a.q, a.q_pitch) && at32(a.k, a.k_pitch) && at32(a.v, a.v_pitch) && at32(a.q_out, a.q_out_pitch) &&
+                      at32(a.k_out, a.k_out_pitch) && at32(a.v_out, a.k_out_pitch);
+    if (!interleaved) rotary_append_kernel<false, false><<<unsigned(blocks), 256, 0, st>>>(a);
+    else if (wide) rotary_append_kernel<true, true><<<unsigned(blocks), 256, 0, st>>>(a);
+    else rotary_append_kernel<true, false><<<unsigned(blocks), 256, 0, st>>>(a);
     return check_launch();
 }
 

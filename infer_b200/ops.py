@@ -55,6 +55,15 @@ class _on_device:
             self.guard.__exit__(*exc)
 
 
+def _call(device, fn, *args):
+    """``fn(*args, stream)`` on ``device`` and its current stream."""
+    index = device.index
+    if _current_device() == index:
+        return fn(*args, _raw_stream(index))
+    with torch.cuda.device(device):
+        return fn(*args, _raw_stream(index))
+
+
 # The attention entry points are reached through these one-line functions so that the test
 # suite can route a call to the library's self-test entry points (infer_b200/selftest.py).
 def _call_decode(lib, *args):
@@ -280,10 +289,10 @@ def load_kvcache(k_cache, v_cache, slot_mapping, k_scale=None, v_scale=None, k_o
     if v_out is None:
         v_out = k_cache.new_empty(shape, dtype=torch.bfloat16)
     k_pitch, v_pitch = _rows("load_kvcache", "k_out", k_out, dev, shape), _rows("load_kvcache", "v_out", v_out, dev, shape)
-    with _on_device(pool.device):
-        rc = _lib.load().infer_kv_load(pool.handle, k_out.data_ptr(), v_out.data_ptr(), k_pitch, v_pitch, slot_mapping.data_ptr(), n,
-                                       _stream())
-    _lib.check(rc, "load_kvcache")
+    rc = _call(pool.device, _lib.load().infer_kv_load, pool.handle, k_out.data_ptr(), v_out.data_ptr(), k_pitch, v_pitch,
+               slot_mapping.data_ptr(), n)
+    if rc:
+        _lib.check(rc, "load_kvcache")
     return k_out, v_out
 
 
@@ -296,7 +305,7 @@ def _rotary_args(what, q, k, positions, inv_freq, q_out, dev):
     pairs = inv_freq.numel()
     _vector(what, "inv_freq", inv_freq, pairs, torch.float64, dev)
     if q_out is None:
-        q_out = q.new_empty(q.shape)
+        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
         return q_out, q_pitch, k_pitch, q.shape[1] * 128, t, 2 * pairs
     return q_out, q_pitch, k_pitch, _rows(what, "q_out", q_out, dev, q.shape), t, 2 * pairs
 
@@ -318,11 +327,11 @@ def rotary_append(q, k, v, positions, inv_freq, k_cache, v_cache, slot_mapping, 
     if v.shape != k.shape or k.shape[1] != pool.n_kv_heads:
         raise RuntimeError("rotary_append: k and v must have q's rows and the pool's heads")
     _vector("rotary_append", "slot_mapping", slot_mapping, t, torch.int32, dev)
-    with _on_device(pool.device):
-        rc = _lib.load().infer_rotary_append(pool.handle, q_out.data_ptr(), q_out_pitch, q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                                             q_pitch, k_pitch, v_pitch, positions.data_ptr(), inv_freq.data_ptr(), rot,
-                                             bool(interleaved), float(attention_factor), slot_mapping.data_ptr(), t, q.shape[1], _stream())
-    _lib.check(rc, "rotary_append")
+    rc = _call(pool.device, _lib.load().infer_rotary_append, pool.handle, q_out.data_ptr(), q_out_pitch, q.data_ptr(), k.data_ptr(),
+               v.data_ptr(), q_pitch, k_pitch, v_pitch, positions.data_ptr(), inv_freq.data_ptr(), rot, bool(interleaved),
+               float(attention_factor), slot_mapping.data_ptr(), t, q.shape[1])
+    if rc:
+        _lib.check(rc, "rotary_append")
     return q_out
 
 
@@ -332,13 +341,13 @@ def rotary_embedding(q, k, positions, inv_freq, interleaved=False, attention_fac
     dev = q.get_device()
     q_out, q_pitch, k_pitch, q_out_pitch, t, rot = _rotary_args("rotary_embedding", q, k, positions, inv_freq, q_out, dev)
     if k_out is None:
-        k_out = k.new_empty(k.shape)
+        k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
     k_out_pitch = _rows("rotary_embedding", "k_out", k_out, dev, k.shape)
-    with _on_device(q.device):
-        rc = _lib.load().infer_rotary_embed(q_out.data_ptr(), k_out.data_ptr(), q_out_pitch, k_out_pitch, q.data_ptr(), k.data_ptr(),
-                                            q_pitch, k_pitch, positions.data_ptr(), inv_freq.data_ptr(), rot, bool(interleaved),
-                                            float(attention_factor), t, q.shape[1], k.shape[1], _stream())
-    _lib.check(rc, "rotary_embedding")
+    rc = _call(q.device, _lib.load().infer_rotary_embed, q_out.data_ptr(), k_out.data_ptr(), q_out_pitch, k_out_pitch, q.data_ptr(),
+               k.data_ptr(), q_pitch, k_pitch, positions.data_ptr(), inv_freq.data_ptr(), rot, bool(interleaved),
+               float(attention_factor), t, q.shape[1], k.shape[1])
+    if rc:
+        _lib.check(rc, "rotary_embedding")
     return q_out, k_out
 
 
@@ -470,40 +479,58 @@ def paged_attn_prefill(q, k_cache, v_cache, cu_seqlens_q, cu_seqlens_k, max_seql
     e4m3 pools come with their ``k_scale`` / ``v_scale``.  ``window`` / ``sinks``: a query sees the ``window`` keys up to its
     own position and the first ``sinks`` of its sequence; entries of ``block_table`` for pages without a visible key are not
     read.  With either, a query that sees no key gives zeros."""
+    if window is not None or sinks or k_scale is not None:
+        return _prefill_window(q, k_cache, v_cache, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, softmax_scale,
+                               block_table, out, k_scale, v_scale, window, sinks)
     if q.dtype != torch.bfloat16 or not q.is_contiguous() or q.dim() != 3:
         raise RuntimeError("paged_attn_prefill: q must be contiguous bf16 [total_q, Hq, 128]")
     for name, t in (("cu_seqlens_q", cu_seqlens_q), ("cu_seqlens_k", cu_seqlens_k), ("block_table", block_table)):
         if t.dtype != torch.int32 or not t.is_cuda:
             raise RuntimeError(f"paged_attn_prefill: {name} must be an int32 CUDA tensor")
-    window, sinks = _window("paged_attn_prefill", window, sinks)
-    pool = pool_of(k_cache, v_cache, k_scale, v_scale)
+    pool = pool_of(k_cache, v_cache)
     o = torch.empty_like(q) if out is None else out
     lib = _lib.load()
-    batch, args = cu_seqlens_q.numel() - 1, ()
-    if pool.fp8 or window:
-        _check_prefill_window(q, o, cu_seqlens_q, cu_seqlens_k, block_table, batch, pool)
-        args = (window, sinks)
     with _on_device(pool.device):
-        rc = (_call_prefill_window if args else _call_prefill)(
-            lib, pool.handle, _ptr(o), _ptr(q), q.shape[0], _ptr(cu_seqlens_q), _ptr(cu_seqlens_k), _ptr(block_table),
-            block_table.stride(0), batch, int(max_seqlen_q), int(max_seqlen_k), q.shape[1], float(softmax_scale), *args, _stream())
+        rc = _call_prefill(lib, pool.handle, _ptr(o), _ptr(q), q.shape[0], _ptr(cu_seqlens_q), _ptr(cu_seqlens_k),
+                                     _ptr(block_table), block_table.stride(0), cu_seqlens_q.numel() - 1,
+                                     int(max_seqlen_q), int(max_seqlen_k), q.shape[1], float(softmax_scale),
+                                     _stream())
         _lib.check(rc, "paged_attn_prefill")
         _check_prefill_status(lib, "paged_attn_prefill")
     return o
 
 
-def _check_prefill_window(q, out, cu_seqlens_q, cu_seqlens_k, block_table, batch, pool):
-    """What the windowed and the e4m3 form check beyond the plain one."""
-    for name, t in (("q", q), ("out", out), ("cu_seqlens_q", cu_seqlens_q), ("cu_seqlens_k", cu_seqlens_k),
-                    ("block_table", block_table)):
-        if t.device != pool.device:
-            raise RuntimeError(f"paged_attn_prefill: {name} must be on the pools' device")
-    if q.shape[2] != 128 or out.shape != q.shape or out.dtype != torch.bfloat16 or not out.is_contiguous():
-        raise RuntimeError("paged_attn_prefill: out must be contiguous bf16 in the shape of q, [total_q, Hq, 128]")
-    if cu_seqlens_k.numel() != batch + 1 or not cu_seqlens_q.is_contiguous() or not cu_seqlens_k.is_contiguous():
+def _prefill_window(q, k_cache, v_cache, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, softmax_scale, block_table, out,
+                    k_scale, v_scale, window, sinks):
+    """The windowed and the e4m3 form of ``paged_attn_prefill``."""
+    window, sinks = _window("paged_attn_prefill", window, sinks)
+    pool = pool_of(k_cache, v_cache, k_scale, v_scale)
+    dev, shape = pool.device.index, q.shape
+    if q.dtype is not torch.bfloat16 or len(shape) != 3 or shape[2] != 128 or not q.is_contiguous() or q.get_device() != dev:
+        raise RuntimeError(f"paged_attn_prefill: q must be contiguous bf16 [total_q, Hq, 128] on the pools' device, cuda:{dev}")
+    if out is None:
+        out = torch.empty_like(q)
+    elif out.dtype is not torch.bfloat16 or out.shape != shape or not out.is_contiguous() or out.get_device() != dev:
+        raise RuntimeError("paged_attn_prefill: out must be contiguous bf16 in the shape of q and on its device")
+    for name, t in (("cu_seqlens_q", cu_seqlens_q), ("cu_seqlens_k", cu_seqlens_k), ("block_table", block_table)):
+        if t.dtype is not torch.int32 or t.get_device() != dev:
+            raise RuntimeError(f"paged_attn_prefill: {name} must be an int32 CUDA tensor on cuda:{dev}")
+    batch = cu_seqlens_q.numel() - 1
+    if batch < 0 or cu_seqlens_k.numel() != batch + 1 or not cu_seqlens_q.is_contiguous() or not cu_seqlens_k.is_contiguous():
         raise RuntimeError("paged_attn_prefill: cu_seqlens_q and cu_seqlens_k must be contiguous, batch + 1 values each")
-    if block_table.dim() != 2 or block_table.shape[0] < batch or block_table.stride(1) != 1:
+    pitch = block_table.stride()
+    if len(pitch) != 2 or block_table.shape[0] < batch or pitch[1] != 1:
         raise RuntimeError("paged_attn_prefill: block_table must have a row of contiguous entries per sequence")
+    lib = _lib.load()
+    rc = _call(pool.device, _call_prefill_window, lib, pool.handle, out.data_ptr(), q.data_ptr(), shape[0], cu_seqlens_q.data_ptr(),
+               cu_seqlens_k.data_ptr(), block_table.data_ptr(), pitch[0], batch, int(max_seqlen_q), int(max_seqlen_k), shape[1],
+               float(softmax_scale), window, sinks)
+    if rc:
+        _lib.check(rc, "paged_attn_prefill")
+    if _CHECK:
+        with _on_device(pool.device):
+            _check_prefill_status(lib, "paged_attn_prefill")
+    return out
 
 
 def _check_prefill_status(lib, what):
