@@ -84,7 +84,8 @@ struct TmaSmem {
     static constexpr int pages = bars + 2 * kStages * 8 + 16;      // page of the tile in each stage (fused append)
     static constexpr int patch = pages + 16;                        // 512 bytes per consumer warp: a new k row and v row
     static constexpr int rem = patch + kConsumerWarps * 512;        // tokens in every sequence's last tile, one byte each
-    static constexpr int total = rem + kMaxBatch;
+    static constexpr int tile = rem + kMaxBatch;                    // tile of the sequence in each stage (window)
+    static constexpr int total = tile + 16;
 };
 
 // Tensor maps with boxes of 16, 32, 64 and 128 token rows: the last tile of a sequence is copied with the smallest
@@ -143,6 +144,7 @@ __global__ void __launch_bounds__(kTmaThreads, 1) decode_tma_kernel(DecodeParams
     volatile int* s_flag = s_scan + 32;             // "this CTA drew the last ticket" (the scan only uses 32 words)
     uint64_t* s_bar = reinterpret_cast<uint64_t*>(smem + TmaSmem::bars);
     volatile int* s_page = reinterpret_cast<volatile int*>(smem + TmaSmem::pages);
+    volatile int* s_tile = reinterpret_cast<volatile int*>(smem + TmaSmem::tile);
     const uint32_t tiles_u32 = smem_u32(smem);
     const uint32_t full0 = smem_u32(s_bar), empty0 = full0 + kStages * 8;
 
@@ -198,6 +200,7 @@ __global__ void __launch_bounds__(kTmaThreads, 1) decode_tma_kernel(DecodeParams
                 const uint32_t bar = full0 + s * 8;
                 const uint32_t kdst = tiles_u32 + s * (2 * kTileBytes), vdst = kdst + kTileBytes;
                 if (p.stall_producer) continue;          // self-test: nothing is armed, every wait on this stage runs out
+                if constexpr (WINDOW) s_tile[s] = tile;
                 s_page[s] = page;                         // for the warp that appends into this tile; released by the arrival below
                 // a sequence's last tile: only the rows that exist (in boxes of 16, 32 or 64 rows); what the stage
                 // holds behind them is masked by the consumers like any row past the context's end
@@ -264,8 +267,7 @@ __global__ void __launch_bounds__(kTmaThreads, 1) decode_tma_kernel(DecodeParams
             continue;
         }
         const int ctx = p.context_lens[sg.b];
-        WindowTiles win;
-        if constexpr (WINDOW) win = window_tiles(ctx, TT, p.window, p.sinks);
+        const int start = ctx - p.window;          // first key of the window, if positive
         const int head = sg.hg * HPC + hl;
         // Query fragments: rows 0..group-1 of the 16-row A operand, zero elsewhere.
         uint32_t qa[8][2];
@@ -304,12 +306,12 @@ __global__ void __launch_bounds__(kTmaThreads, 1) decode_tma_kernel(DecodeParams
         for (int t = sg.t0; t < sg.t1; ++t, ++it) {
             const uint32_t s = it % kStages, ph = (it / kStages) & 1;
             if (ok && !mbar_wait(full0 + s * 8, ph, p.wait_limit)) ok = false;
-            const int tok_w = (WINDOW ? tile_of(win, t) : t) * TT + tw * 16;   // first token of this warp's 16
+            const int tok_w = (WINDOW ? s_tile[s] : t) * TT + tw * 16;   // first token of this warp's 16
             const int valid = ctx - tok_w;                  // tokens of the 16 that exist
-            auto seen = [&](int i) { return WINDOW ? key_visible(win, ctx, tok_w + i) : i < valid; };
+            auto seen = [&](int i) { return i < valid && (!WINDOW || tok_w + i >= start || tok_w + i < p.sinks); };
             // some of the 16 are visible / not all of them are
-            auto some = [&] { return valid > 0 && (!WINDOW || tok_w + 16 > win.start || tok_w < win.sinks); };
-            auto partly = [&] { return valid < 16 || (WINDOW && tok_w < win.start && tok_w + 16 > win.sinks); };
+            auto some = [&] { return valid > 0 && (!WINDOW || tok_w + 16 > start || tok_w < p.sinks); };
+            auto partly = [&] { return valid < 16 || (WINDOW && tok_w < start && tok_w + 16 > p.sinks); };
             if (ok && some()) {
                 const uint32_t kbase = tiles_u32 + s * (2 * kTileBytes) + (hl * 2) * SUB;
                 const uint32_t vbase = kbase + kTileBytes;
@@ -486,7 +488,8 @@ struct Fp8Smem {
     static constexpr int bars = scan + threads * 4;
     static constexpr int meta = bars + 2 * kStages * 8 + 16;      // [kStages][HPC][2] floats: k scale, v scale
     static constexpr int rem = meta + kStages * HPC * 8;           // tokens in every sequence's last tile, one byte each
-    static constexpr int total = rem + kMaxBatch;
+    static constexpr int tile = rem + kMaxBatch;                   // tile of the sequence in each stage (window)
+    static constexpr int total = tile + 16;
 };
 
 template <int HPC, bool WINDOW>
@@ -511,6 +514,7 @@ __global__ void __launch_bounds__(kTmaThreads, 1) decode_tma_fp8_kernel(DecodePa
     volatile int* s_flag = s_scan + 32;             // "this CTA drew the last ticket" (the scan only uses 32 words)
     uint64_t* s_bar = reinterpret_cast<uint64_t*>(smem + L::bars);
     volatile float* s_meta = reinterpret_cast<volatile float*>(smem + L::meta);
+    volatile int* s_tile = reinterpret_cast<volatile int*>(smem + L::tile);
     const uint32_t tiles_u32 = smem_u32(smem);
     const uint32_t full0 = smem_u32(s_bar), empty0 = full0 + kStages * 8;
 
@@ -568,6 +572,7 @@ __global__ void __launch_bounds__(kTmaThreads, 1) decode_tma_fp8_kernel(DecodePa
                     s_meta[(s * HPC + hl) * 2 + 0] = ks[hl];
                     s_meta[(s * HPC + hl) * 2 + 1] = vs[hl];
                 }
+                if constexpr (WINDOW) s_tile[s] = tile;
                 const uint32_t bar = full0 + s * 8;
                 const uint32_t kdst = tiles_u32 + s * (2 * kTileBytes), vdst = kdst + kTileBytes;
                 if (p.stall_producer) continue;          // self-test: nothing is armed, every wait on this stage runs out
@@ -633,8 +638,7 @@ __global__ void __launch_bounds__(kTmaThreads, 1) decode_tma_fp8_kernel(DecodePa
             continue;
         }
         const int ctx = p.context_lens[sg.b];
-        WindowTiles win;
-        if constexpr (WINDOW) win = window_tiles(ctx, TT, p.window, p.sinks);
+        const int start = ctx - p.window;          // first key of the window, if positive
         const int head = sg.hg * HPC + hl;
         // B fragments of Q^T in f16: column gid is query head gid of the group.  MMA k-slots
         // (2t, 2t+1, 2t+8, 2t+9) of a 16-dim chunk carry dims (4t, 4t+1, 4t+2, 4t+3): the order in
@@ -666,10 +670,10 @@ __global__ void __launch_bounds__(kTmaThreads, 1) decode_tma_fp8_kernel(DecodePa
             const float c_k = s_meta[(s * HPC + hl) * 2 + 0] * p.scale_log2;
             const float vs = s_meta[(s * HPC + hl) * 2 + 1];
             const int row0 = tw * TPW;                      // this warp's tokens of the tile
-            const int tok_w = (WINDOW ? tile_of(win, t) : t) * TT + row0;
+            const int tok_w = (WINDOW ? s_tile[s] : t) * TT + row0;
             const int valid = ctx - tok_w;
-            auto some = [&] { return valid > 0 && (!WINDOW || tok_w + TPW > win.start || tok_w < win.sinks); };
-            auto seen = [&](int i) { return WINDOW ? key_visible(win, ctx, tok_w + i) : i < valid; };
+            auto some = [&] { return valid > 0 && (!WINDOW || tok_w + TPW > start || tok_w < p.sinks); };
+            auto seen = [&](int i) { return i < valid && (!WINDOW || tok_w + i >= start || tok_w + i < p.sinks); };
             if (ok && some()) {
                 const uint32_t kbase = tiles_u32 + s * (2 * kTileBytes) + hl * kHeadBytes;
                 const uint32_t vbase = kbase + kTileBytes;
@@ -752,7 +756,7 @@ __global__ void __launch_bounds__(kTmaThreads, 1) decode_tma_fp8_kernel(DecodePa
                     const uint32_t pb0 = movmatrix_trans(pp[h][0]), pb1 = movmatrix_trans(pp[h][1]);
                     const int vh = valid - h * 16;          // tokens of this half that exist
                     auto partly = [&] {
-                        return vh < 16 || (WINDOW && tok_w + h * 16 < win.start && tok_w + h * 16 + 16 > win.sinks);
+                        return vh < 16 || (WINDOW && tok_w + h * 16 < start && tok_w + h * 16 + 16 > p.sinks);
                     };
 #pragma unroll
                     for (int c2 = 0; c2 < 4; ++c2) {

@@ -100,9 +100,6 @@ __device__ __forceinline__ WindowTiles window_tiles(int len, int tile_tokens, in
     return w;
 }
 __device__ __forceinline__ int tile_of(const WindowTiles& w, int t) { return t < w.n_sink ? t : t + w.skip; }
-__device__ __forceinline__ bool key_visible(const WindowTiles& w, int len, int key) {
-    return key < len && (key >= w.start || key < w.sinks);
-}
 
 // Exclusive prefix of tiles per sequence into shared memory (s_tp[batch] = total).
 // Every thread of the CTA must call it (blockDim.x a multiple of 32, at most 1024); ends with
