@@ -130,6 +130,7 @@ struct PwParams {
     int window, sinks;       // window: 0x7fffffff = none
     float scale_log2;
     int splits;              // CTAs (of one cluster) that share the key tiles of a row block
+    int out_at32;            // out is a multiple of 32
     int* status;             // may be null
     uint32_t wait_limit;
     int stall_producer;
@@ -174,9 +175,8 @@ __device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
 // no room for the power).  Chunk x (of 16) holds eight bf16; result c (of 8) is the first parts of chunks 2c and 2c + 1,
 // stored over chunk c, and their second parts, stored over chunk 8 + c.  The eight rows of a phase have a chunk at eight
 // different banks.
-// The split is arithmetic on f16 bits: y = q * 2^-e * 2^-8 has the exponents of e4m3 (subnormal ones too) in its upper bits,
-// so the first part is y cut to three bits of mantissa, the second the difference, and the byte of either its sign and the
-// seven bits below bit 14.
+// The split is arithmetic on bf16 bits: y = q * 2^-e * 2^-120 has the exponents of e4m3 (subnormal ones too), so the first part
+// is y cut to three bits of mantissa, the second the difference, and the byte of either its sign and bits 10 .. 4.
 __device__ __forceinline__ float split_q_row(uint32_t tile, int t) {
     auto chunk = [&](int x) { return tile + (x >> 3) * kPwHalf + swz128(t, x & 7); };
     uint4 w[16];
@@ -195,21 +195,22 @@ __device__ __forceinline__ float split_q_row(uint32_t tile, int t) {
     const __nv_bfloat162 all = __hmax2_nan(__hmax2_nan(top2[0], top2[1]), __hmax2_nan(top2[2], top2[3]));
     const uint32_t top = __bfloat16_as_ushort(__hmax_nan(__low2bfloat16(all), __high2bfloat16(all))) & 0x7fffu;
     const int e = min(max(int(top >> 7) - 127 - 7, -118), 118);
-    const float down = __uint_as_float(uint32_t(127 - e - 8) << 23);
-    auto bytes = [](uint32_t y0, uint32_t y1) {            // e4m3 of four f16 scaled by 2^-8
-        const uint32_t b0 = (y0 & 0x80008000u) | ((y0 << 1) & 0x7fff7fffu);
-        const uint32_t b1 = (y1 & 0x80008000u) | ((y1 << 1) & 0x7fff7fffu);
+    const uint32_t down = uint32_t(127 - e) << 7 | uint32_t(127 - e) << 23, tiny = 0x03800380u;      // 2^-e and 2^-120, twice
+    auto bytes = [](uint32_t y0, uint32_t y1) {            // e4m3 of four bf16 scaled by 2^-120
+        const uint32_t b0 = (y0 & 0x80008000u) | ((y0 << 4) & 0x7fff7fffu);
+        const uint32_t b1 = (y1 & 0x80008000u) | ((y1 << 4) & 0x7fff7fffu);
         return __byte_perm(b0, b1, 0x7531);
     };
+    auto as2 = [](const uint32_t& v) { return *reinterpret_cast<const __nv_bfloat162*>(&v); };
+    auto bits = [](const __nv_bfloat162& v) { return *reinterpret_cast<const uint32_t*>(&v); };
     auto split8 = [&](const uint4& q, uint32_t& h0, uint32_t& h1, uint32_t& l0, uint32_t& l1) {
         const uint32_t v[4] = {q.x, q.y, q.z, q.w};
         uint32_t y[4], l[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            y[k] = pack_f16(__uint_as_float(v[k] << 16) * down, __uint_as_float(v[k] & 0xffff0000u) * down);
-            const uint32_t h = y[k] & 0xff80ff80u;
-            const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&y[k]), *reinterpret_cast<const __half2*>(&h));
-            l[k] = *reinterpret_cast<const uint32_t*>(&d);
+            y[k] = bits(__hmul2_rn(__hmul2_rn(as2(v[k]), as2(down)), as2(tiny)));
+            const uint32_t h = y[k] & 0xfff0fff0u;
+            l[k] = bits(__hsub2_rn(as2(y[k]), as2(h)));
         }
         h0 = bytes(y[0], y[1]);
         h1 = bytes(y[2], y[3]);
@@ -386,7 +387,17 @@ __global__ void __launch_bounds__(PwCfg<FP8>::threads, 1) prefill_window_kernel(
                                     page = page_next;
                                     page_next = page_of(j + 2);
                                     const float k_scale_next = scale_of(p.k_scale, page), v_scale_next = scale_of(p.v_scale, page);
-                                    volatile int* t = s_ring + (kc % kPwRing) * PT_INTS;     // released by the arrival K's copy is armed with
+                                    const int s = kc % C::k_stages;
+                                    if (!tc_wait(bar(PW_K_EMPTY, s), ((kc / C::k_stages) & 1) ^ 1, s_abort, p.wait_limit)) {
+                                        ok = false;
+                                        break;
+                                    }
+                                    // the copy first; the tile's entry is written while it runs and released by the arrival below,
+                                    // without which the barrier cannot complete
+                                    const uint32_t dst = base + C::k + s * C::k_bytes;
+                                    tma_load_3d(dst, &map_k, bar(PW_K_FULL, s), 0, kvh, slot);
+                                    if constexpr (!FP8) tma_load_3d(dst + kPwHalf, &map_k, bar(PW_K_FULL, s), 64, kvh, slot);
+                                    volatile int* t = s_ring + (kc % kPwRing) * PT_INTS;
                                     t[PT_KEY0] = key0;
                                     t[PT_CUT] = key0 + kPwKeys - 1 > pos_lo || (windowed && key0 <= pos_hi - p.window && key0 + kPwKeys > sinks);
                                     t[PT_SINK_END] = sinks - key0;
@@ -410,14 +421,8 @@ __global__ void __launch_bounds__(PwCfg<FP8>::threads, 1) prefill_window_kernel(
                                     }
                                     k_scale = k_scale_next;
                                     v_scale = v_scale_next;
-                                    const int s = kc % C::k_stages;
-                                    if (tc_wait(bar(PW_K_EMPTY, s), ((kc / C::k_stages) & 1) ^ 1, s_abort, p.wait_limit)) {
-                                        const uint32_t dst = base + C::k + s * C::k_bytes;
-                                        mbar_expect_tx(bar(PW_K_FULL, s), C::k_bytes);
-                                        tma_load_3d(dst, &map_k, bar(PW_K_FULL, s), 0, kvh, slot);
-                                        if constexpr (!FP8) tma_load_3d(dst + kPwHalf, &map_k, bar(PW_K_FULL, s), 64, kvh, slot);
-                                        ++kc;
-                                    } else ok = false;
+                                    mbar_expect_tx(bar(PW_K_FULL, s), C::k_bytes);
+                                    ++kc;
                                 }
                                 if (FP8) v_slot = slot;
                                 if (j >= lag && ok) {
@@ -782,32 +787,34 @@ __global__ void __launch_bounds__(PwCfg<FP8>::threads, 1) prefill_window_kernel(
             tc_fence_before();
             mbar_arrive(bar(PW_P_FULL, g));                        // (the tile's entry may be gone from here on)
         }
+        // where the row goes (worked out while the last P V product runs)
+        const int tok = ie[PI_TOK0] + g * p.tokens + r / p.group;
+        const bool live = r < p.tokens * p.group && tok < ie[PI_LQ];      // rows behind the tokens of the tile or the sequence hold anything
+        const int64_t row = int64_t(ie[PI_Q0] + tok) * p.n_q_heads + ie[PI_KVH] * p.group + r % p.group;
+        const bool any = l_run != 0.f;                              // a row that sees nothing gives zeros
+        const float f = any ? unit / l_run : 0.f;
         // O is complete once the last P V has retired
         if (any_tile && ok && !tc_wait(bar(PW_PV_DONE, g), (uses - 1) & 1, s_abort, p.wait_limit)) ok = false;
         if (any_tile && ok && p.splits == 1) {
             tc_fence_after();
-            const bool any = l_run != 0.f;                          // a row that sees nothing gives zeros
-            const float f = unit / l_run;
-            const int tok = ie[PI_TOK0] + g * p.tokens + r / p.group;
-            const bool live = r < p.tokens * p.group && tok < ie[PI_LQ];      // rows behind the tokens of the tile or the sequence hold anything
-            const int64_t row = int64_t(ie[PI_Q0] + tok) * p.n_q_heads + ie[PI_KVH] * p.group + r % p.group;
+            uint32_t v[128];
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                uint32_t v[32];
-                tc_ld32(o_addr + c * 32, v);
-                tc_wait_ld();
-                if (!live) continue;
+            for (int c = 0; c < 4; ++c) tc_ld32(o_addr + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&v[c * 32]));
+            tc_wait_ld();
+            if (live) {
+                __nv_bfloat16* dst = p.out + row * kHeadDim;
+                if (!any) {
 #pragma unroll
-                for (int i = 0; i < 32; ++i) v[i] = any ? __float_as_uint(__uint_as_float(v[i]) * f) : 0u;
-                uint4* dst = reinterpret_cast<uint4*>(p.out + row * kHeadDim + c * 32);
+                    for (int i = 0; i < 128; ++i) v[i] = 0u;
+                }
+                auto two = [&](int i) { return pack_bf16(__uint_as_float(v[i]) * f, __uint_as_float(v[i + 1]) * f); };
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    uint4 w;
-                    w.x = pack_bf16(__uint_as_float(v[8 * i]), __uint_as_float(v[8 * i + 1]));
-                    w.y = pack_bf16(__uint_as_float(v[8 * i + 2]), __uint_as_float(v[8 * i + 3]));
-                    w.z = pack_bf16(__uint_as_float(v[8 * i + 4]), __uint_as_float(v[8 * i + 5]));
-                    w.w = pack_bf16(__uint_as_float(v[8 * i + 6]), __uint_as_float(v[8 * i + 7]));
-                    dst[i] = w;
+                for (int i = 0; i < 128; i += 16) {
+                    const Bytes32 w = {make_uint4(two(i), two(i + 2), two(i + 4), two(i + 6)),
+                                       make_uint4(two(i + 8), two(i + 10), two(i + 12), two(i + 14))};
+                    // a lane's row is 256 bytes away from its neighbour's: whole 32-byte sectors halve what the stores take
+                    if (p.out_at32) store32<true>(dst + i, w);
+                    else store32<false>(dst + i, w);
                 }
             }
             tc_fence_before();
@@ -999,6 +1006,7 @@ static int paged_prefill_window(const infer_kv_pool_t* pool, void* out, const vo
     if (total_q == 0 || batch == 0) return INFER_OK;
     PwParams p{};
     p.out = static_cast<__nv_bfloat16*>(out);
+    p.out_at32 = (reinterpret_cast<uintptr_t>(out) & 31) == 0;
     p.cu_q = cu_seqlens_q;
     p.cu_k = cu_seqlens_k;
     p.block_tables = block_tables;
