@@ -78,10 +78,11 @@ SELFTEST_SIGNATURES = {
 }
 
 _lib = None
+host_ops = None            # the module of csrc/host_ops.cpp, bound to the loaded library
 
 
 def load() -> C.CDLL:
-    global _lib
+    global _lib, host_ops
     if _lib is not None:
         return _lib
     if not LIB_PATH.exists():
@@ -92,6 +93,13 @@ def load() -> C.CDLL:
     for name, (res, args) in {**SIGNATURES, **SELFTEST_SIGNATURES}.items():
         fn = getattr(lib, name)
         fn.restype, fn.argtypes = res, args
+    try:
+        from . import _host_ops
+    except ImportError as e:
+        raise ImportError(f"infer_b200/_host_ops.so is missing or does not fit this PyTorch: build it with "
+                          f"`python -m infer_b200.build` ({e})") from e
+    _host_ops.bind_library({name: C.cast(getattr(lib, name), C.c_void_p).value for name in {**SIGNATURES, **SELFTEST_SIGNATURES}})
+    host_ops = _host_ops
     _lib = lib
     return lib
 

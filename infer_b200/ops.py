@@ -28,9 +28,7 @@ _POOLS: dict = {}
 _CHECK = os.environ.get("INFER_B200_CHECK") == "1"    # debugging: read the device status word after each call
 
 
-# What a call costs the host counts as much as the kernel when a step is small: the lean accessors below (the raw stream
-# instead of a Stream object, addresses as plain integers, get_device() for both "on the GPU" and "on which") brought a
-# call of load_kvcache from 19 to 8 us.
+# The raw stream and addresses as plain integers: a Stream object costs 3 us, a c_void_p per pointer 0.1.
 _raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 
 
@@ -55,16 +53,7 @@ class _on_device:
             self.guard.__exit__(*exc)
 
 
-def _call(device, fn, *args):
-    """``fn(*args, stream)`` on ``device`` and its current stream."""
-    index = device.index
-    if _current_device() == index:
-        return fn(*args, _raw_stream(index))
-    with torch.cuda.device(device):
-        return fn(*args, _raw_stream(index))
-
-
-# The attention entry points are reached through these one-line functions so that the test
+# The three attention entry points are reached through these one-line functions so that the test
 # suite can route a call to the library's self-test entry points (infer_b200/selftest.py).
 def _call_decode(lib, *args):
     return lib.infer_paged_decode(*args)
@@ -72,10 +61,6 @@ def _call_decode(lib, *args):
 
 def _call_prefill(lib, *args):
     return lib.infer_paged_prefill(*args)
-
-
-def _call_prefill_window(lib, *args):
-    return lib.infer_paged_prefill_window(*args)
 
 
 def _call_dense(lib, *args):
@@ -155,7 +140,7 @@ class KVPool:
                                           self.num_blocks, self.block_size, self.n_kv_heads, self.head_dim,
                                           _lib.KV_E4M3 if fp8 else _lib.KV_BF16)
         _lib.check(rc, "infer_kv_pool_create")
-        self.handle = handle
+        self.handle, self.address = handle, handle.value
         self._decode_ws_bytes: dict = {}      # n_q_heads -> bytes, asked of the library once
         # e4m3 append scratch: its layout follows the pool's geometry and every call leaves it in the state
         # the next call on the SAME pool expects, so each pool owns one (sized here, never re-allocated)
@@ -259,21 +244,11 @@ def qk_norm_rope_append(q, k, v, q_norm_weight, k_norm_weight, eps, positions, c
     return q_out
 
 
-def _rows(what, name, x, device, shape=None):
-    """Checks that ``x`` is rows [T, H, 128] of bf16 with contiguous heads on GPU ``device``; their pitch in elements."""
-    size, stride = x.shape, x.stride()
-    if x.dtype is not torch.bfloat16 or len(size) != 3 or size[2] != 128 or x.get_device() != device:
-        raise RuntimeError(f"{what}: {name} must be a bf16 CUDA tensor [T, H, 128] on cuda:{device}")
-    if stride[2] != 1 or (size[1] > 1 and stride[1] != 128):
-        raise RuntimeError(f"{what}: {name} must have contiguous heads")
-    if shape is not None and size != shape:
-        raise RuntimeError(f"{what}: {name} must be {list(shape)}")
-    return stride[0] if size[0] > 1 else size[1] * 128
-
-
-def _vector(what, name, x, n, dtype, device):
-    if x.dtype is not dtype or x.get_device() != device or x.numel() != n or not x.is_contiguous():
-        raise RuntimeError(f"{what}: {name} must be a contiguous {str(dtype)[6:]} tensor of {n} values on cuda:{device}")
+def _host_ops():
+    """The module of csrc/host_ops.cpp: argument checks and launches of the ops below."""
+    if _lib.host_ops is None:
+        _lib.load()
+    return _lib.host_ops
 
 
 def load_kvcache(k_cache, v_cache, slot_mapping, k_scale=None, v_scale=None, k_out=None, v_out=None):
@@ -281,33 +256,7 @@ def load_kvcache(k_cache, v_cache, slot_mapping, k_scale=None, v_scale=None, k_o
     the inverse of ``store_kvcache``.  e4m3 pools: byte * scale of its page and head, in fp32, rounded once.  Slots
     outside the pool (-1: padding) give rows of zeros.  ``k_out`` / ``v_out`` may be column slices of a wider row."""
     pool = pool_of(k_cache, v_cache, k_scale, v_scale)
-    dev, n = pool.device.index, slot_mapping.numel()
-    _vector("load_kvcache", "slot_mapping", slot_mapping, n, torch.int32, dev)
-    shape = torch.Size((n, pool.n_kv_heads, pool.head_dim))
-    if k_out is None:
-        k_out = k_cache.new_empty(shape, dtype=torch.bfloat16)
-    if v_out is None:
-        v_out = k_cache.new_empty(shape, dtype=torch.bfloat16)
-    k_pitch, v_pitch = _rows("load_kvcache", "k_out", k_out, dev, shape), _rows("load_kvcache", "v_out", v_out, dev, shape)
-    rc = _call(pool.device, _lib.load().infer_kv_load, pool.handle, k_out.data_ptr(), v_out.data_ptr(), k_pitch, v_pitch,
-               slot_mapping.data_ptr(), n)
-    if rc:
-        _lib.check(rc, "load_kvcache")
-    return k_out, v_out
-
-
-def _rotary_args(what, q, k, positions, inv_freq, q_out, dev):
-    t = q.shape[0]
-    q_pitch, k_pitch = _rows(what, "q", q, dev), _rows(what, "k", k, dev)
-    if k.shape[0] != t:
-        raise RuntimeError(f"{what}: q and k must have the same number of rows")
-    _vector(what, "positions", positions, t, torch.int64, dev)
-    pairs = inv_freq.numel()
-    _vector(what, "inv_freq", inv_freq, pairs, torch.float64, dev)
-    if q_out is None:
-        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        return q_out, q_pitch, k_pitch, q.shape[1] * 128, t, 2 * pairs
-    return q_out, q_pitch, k_pitch, _rows(what, "q_out", q_out, dev, q.shape), t, 2 * pairs
+    return _host_ops().load_kvcache(pool.address, pool.device.index, pool.n_kv_heads, slot_mapping, k_out, v_out)
 
 
 def rotary_append(q, k, v, positions, inv_freq, k_cache, v_cache, slot_mapping, interleaved=False, attention_factor=1.0,
@@ -321,57 +270,14 @@ def rotary_append(q, k, v, positions, inv_freq, k_cache, v_cache, slot_mapping, 
     (column slices of the fused qkv output are fine); returns the rotated q, contiguous, or in ``q_out`` (may be ``q``).
     Rows with a slot outside the pool are not stored."""
     pool = pool_of(k_cache, v_cache)
-    dev = pool.device.index
-    q_out, q_pitch, k_pitch, q_out_pitch, t, rot = _rotary_args("rotary_append", q, k, positions, inv_freq, q_out, dev)
-    v_pitch = _rows("rotary_append", "v", v, dev)
-    if v.shape != k.shape or k.shape[1] != pool.n_kv_heads:
-        raise RuntimeError("rotary_append: k and v must have q's rows and the pool's heads")
-    _vector("rotary_append", "slot_mapping", slot_mapping, t, torch.int32, dev)
-    rc = _call(pool.device, _lib.load().infer_rotary_append, pool.handle, q_out.data_ptr(), q_out_pitch, q.data_ptr(), k.data_ptr(),
-               v.data_ptr(), q_pitch, k_pitch, v_pitch, positions.data_ptr(), inv_freq.data_ptr(), rot, bool(interleaved),
-               float(attention_factor), slot_mapping.data_ptr(), t, q.shape[1])
-    if rc:
-        _lib.check(rc, "rotary_append")
-    return q_out
+    return _host_ops().rotary_append(pool.address, pool.device.index, pool.n_kv_heads, q, k, v, positions, inv_freq, slot_mapping,
+                                     interleaved, attention_factor, q_out)
 
 
 def rotary_embedding(q, k, positions, inv_freq, interleaved=False, attention_factor=1.0, q_out=None, k_out=None):
     """``rotary_append`` without the append -> (q, k) rotated; in front of ``store_kvcache`` for an e4m3 pool.
     ``q_out`` / ``k_out`` may be ``q`` / ``k``."""
-    dev = q.get_device()
-    q_out, q_pitch, k_pitch, q_out_pitch, t, rot = _rotary_args("rotary_embedding", q, k, positions, inv_freq, q_out, dev)
-    if k_out is None:
-        k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
-    k_out_pitch = _rows("rotary_embedding", "k_out", k_out, dev, k.shape)
-    rc = _call(q.device, _lib.load().infer_rotary_embed, q_out.data_ptr(), k_out.data_ptr(), q_out_pitch, k_out_pitch, q.data_ptr(),
-               k.data_ptr(), q_pitch, k_pitch, positions.data_ptr(), inv_freq.data_ptr(), rot, bool(interleaved),
-               float(attention_factor), t, q.shape[1], k.shape[1])
-    if rc:
-        _lib.check(rc, "rotary_embedding")
-    return q_out, k_out
-
-
-def _window(what, window, sinks):
-    """``window`` and ``sinks`` as the library takes them: 0 = no window."""
-    if window is None:
-        if sinks:
-            raise RuntimeError(f"{what}: sinks without a window (every key is visible)")
-        return 0, 0
-    window, sinks = int(window), int(sinks)
-    if window < 1 or sinks < 0:
-        raise RuntimeError(f"{what}: window must be at least 1 and sinks at least 0")
-    return min(window, 0x7fffffff), min(sinks, 0x7fffffff)
-
-
-def _check_decode_window(what, q3, o, lens, table, pool):
-    """What the windowed form checks beyond the plain one."""
-    b = q3.shape[0]
-    if q3.shape[2] != 128 or o.dtype is not torch.bfloat16 or not o.is_contiguous():
-        raise RuntimeError(f"{what}: q and out must be contiguous bf16 [B, Hq, 128]")
-    if lens.device != pool.device or table.device != pool.device:
-        raise RuntimeError(f"{what}: cache_seqlens and block_table must be on the pools' device")
-    if lens.numel() != b or not lens.is_contiguous() or table.dim() != 2 or table.shape[0] < b or table.stride(1) != 1:
-        raise RuntimeError(f"{what}: cache_seqlens must hold a length, block_table a row of contiguous entries per sequence")
+    return _host_ops().rotary_embedding(q, k, positions, inv_freq, interleaved, attention_factor, q_out, k_out)
 
 
 # --------------------------------------------------------------------------- decode
@@ -389,6 +295,9 @@ def paged_attn_decode(q, k_cache, v_cache, cache_seqlens, block_table, softmax_s
     ``workspace``: a zero-initialised uint8 tensor of at least
     ``pool.decode_workspace_bytes(B, Hq)`` bytes reserved for this caller's stream; by default the
     per-device scratch is used (see ``_Scratch``: one stream per device)."""
+    if window is not None or sinks:
+        return _decode_window(q, None, None, k_cache, v_cache, cache_seqlens, block_table, softmax_scale, out, k_scale, v_scale,
+                              workspace, window, sinks)
     shape = q.shape
     q3 = q if len(shape) == 3 else q.reshape(shape[0], shape[-2], shape[-1])
     if q3.dtype != torch.bfloat16 or not q3.is_contiguous():
@@ -401,21 +310,14 @@ def paged_attn_decode(q, k_cache, v_cache, cache_seqlens, block_table, softmax_s
             raise RuntimeError(f"paged_attn_decode: {name} must be an int32 CUDA tensor")
     if block_table.stride(-1) != 1:
         raise RuntimeError("paged_attn_decode: block_table rows must be contiguous")
-    window, sinks = _window("paged_attn_decode", window, sinks)
     pool = pool_of(k_cache, v_cache, k_scale, v_scale)
     o = torch.empty(q3.shape, dtype=q3.dtype, device=pool.device) if out is None else out if out.shape == q3.shape else out.view(q3.shape)
     lib = _lib.load()
     b, hq, _ = q3.shape
     ws = workspace if workspace is not None else _SCRATCH.get(pool.device, "decode", pool.decode_workspace_bytes(b, hq))
     with _on_device(pool.device):
-        if window:
-            _check_decode_window("paged_attn_decode", q3, o, cache_seqlens, block_table, pool)
-            rc = lib.infer_paged_decode_window(pool.handle, _ptr(o), _ptr(q3), _ptr(cache_seqlens), _ptr(block_table),
-                                               block_table.stride(0), b, hq, float(softmax_scale), window, sinks, _ptr(ws),
-                                               ws.numel(), _stream())
-        else:
-            rc = _call_decode(lib, pool.handle, _ptr(o), _ptr(q3), _ptr(cache_seqlens), _ptr(block_table),
-                              block_table.stride(0), b, hq, float(softmax_scale), _ptr(ws), ws.numel(), _stream())
+        rc = _call_decode(lib, pool.handle, _ptr(o), _ptr(q3), _ptr(cache_seqlens), _ptr(block_table),
+                          block_table.stride(0), b, hq, float(softmax_scale), _ptr(ws), ws.numel(), _stream())
         _lib.check(rc, "paged_attn_decode")
         if _CHECK and not torch.cuda.is_current_stream_capturing():
             _lib.check(lib.infer_paged_decode_status(_ptr(ws), _stream()), "paged_attn_decode (device status)")
@@ -430,7 +332,9 @@ def paged_attn_decode_append(q, key, value, k_cache, v_cache, cache_seqlens, blo
     ``cache_seqlens[b] - 1`` of sequence b; the slot is read off ``block_table``, so no ``slot_mapping`` is
     needed.  The pools end up as after ``store_kvcache``.  ``q``, ``key``, ``value`` and ``out`` may be pinned
     host tensors, ``window`` and ``sinks`` limit the visible keys (see ``paged_attn_decode``)."""
-    window, sinks = _window("paged_attn_decode_append", window, sinks)
+    if window is not None or sinks:
+        return _decode_window(q, key, value, k_cache, v_cache, cache_seqlens, block_table, softmax_scale, out, None, None, workspace,
+                              window, sinks)
     shape = q.shape
     q3 = q if len(shape) == 3 else q.reshape(shape[0], shape[-2], shape[-1])
     if q3.dtype != torch.bfloat16 or not q3.is_contiguous():
@@ -457,17 +361,29 @@ def paged_attn_decode_append(q, key, value, k_cache, v_cache, cache_seqlens, blo
     v_pitch = value.stride(0) if b > 1 else row
     ws = workspace if workspace is not None else _SCRATCH.get(pool.device, "decode", pool.decode_workspace_bytes(b, hq))
     with _on_device(pool.device):
-        args = (pool.handle, _ptr(o), _ptr(q3), _ptr(key), _ptr(value), k_pitch, v_pitch, _ptr(cache_seqlens),
-                _ptr(block_table), block_table.stride(0), b, hq, float(softmax_scale))
-        if window:
-            _check_decode_window("paged_attn_decode_append", q3, o, cache_seqlens, block_table, pool)
-            rc = lib.infer_paged_decode_append_window(*args, window, sinks, _ptr(ws), ws.numel(), _stream())
-        else:
-            rc = lib.infer_paged_decode_append(*args, _ptr(ws), ws.numel(), _stream())
+        rc = lib.infer_paged_decode_append(pool.handle, _ptr(o), _ptr(q3), _ptr(key), _ptr(value), k_pitch, v_pitch,
+                                           _ptr(cache_seqlens), _ptr(block_table), block_table.stride(0), b, hq,
+                                           float(softmax_scale), _ptr(ws), ws.numel(), _stream())
         _lib.check(rc, "paged_attn_decode_append")
         if _CHECK and not torch.cuda.is_current_stream_capturing():
             _lib.check(lib.infer_paged_decode_status(_ptr(ws), _stream()), "paged_attn_decode_append (device status)")
     return o if o.shape == shape else o.view(shape)
+
+
+def _decode_window(q, key, value, k_cache, v_cache, cache_seqlens, block_table, softmax_scale, out, k_scale, v_scale, workspace,
+                   window, sinks):
+    """The windowed forms of the two ops above."""
+    pool = pool_of(k_cache, v_cache, k_scale, v_scale)
+    if key is not None and (pool.fp8 or value is None):
+        raise RuntimeError("paged_attn_decode_append: bf16 pools only (store_kvcache + paged_attn_decode for e4m3 pools), key and value")
+    if workspace is None:
+        workspace = _SCRATCH.get(pool.device, "decode", pool.decode_workspace_bytes(q.shape[0], q.shape[-2]))
+    out = _host_ops().decode_window(pool.address, pool.device.index, pool.n_kv_heads, q, key, value, cache_seqlens, block_table,
+                                    softmax_scale, out, workspace, window, sinks)
+    if _CHECK and not torch.cuda.is_current_stream_capturing():
+        with _on_device(pool.device):
+            _lib.check(_lib.load().infer_paged_decode_status(_ptr(workspace), _stream()), "paged_attn_decode (device status)")
+    return out
 
 
 # --------------------------------------------------------------------------- prefill
@@ -503,33 +419,12 @@ def paged_attn_prefill(q, k_cache, v_cache, cu_seqlens_q, cu_seqlens_k, max_seql
 def _prefill_window(q, k_cache, v_cache, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, softmax_scale, block_table, out,
                     k_scale, v_scale, window, sinks):
     """The windowed and the e4m3 form of ``paged_attn_prefill``."""
-    window, sinks = _window("paged_attn_prefill", window, sinks)
     pool = pool_of(k_cache, v_cache, k_scale, v_scale)
-    dev, shape = pool.device.index, q.shape
-    if q.dtype is not torch.bfloat16 or len(shape) != 3 or shape[2] != 128 or not q.is_contiguous() or q.get_device() != dev:
-        raise RuntimeError(f"paged_attn_prefill: q must be contiguous bf16 [total_q, Hq, 128] on the pools' device, cuda:{dev}")
-    if out is None:
-        out = torch.empty_like(q)
-    elif out.dtype is not torch.bfloat16 or out.shape != shape or not out.is_contiguous() or out.get_device() != dev:
-        raise RuntimeError("paged_attn_prefill: out must be contiguous bf16 in the shape of q and on its device")
-    for name, t in (("cu_seqlens_q", cu_seqlens_q), ("cu_seqlens_k", cu_seqlens_k), ("block_table", block_table)):
-        if t.dtype is not torch.int32 or t.get_device() != dev:
-            raise RuntimeError(f"paged_attn_prefill: {name} must be an int32 CUDA tensor on cuda:{dev}")
-    batch = cu_seqlens_q.numel() - 1
-    if batch < 0 or cu_seqlens_k.numel() != batch + 1 or not cu_seqlens_q.is_contiguous() or not cu_seqlens_k.is_contiguous():
-        raise RuntimeError("paged_attn_prefill: cu_seqlens_q and cu_seqlens_k must be contiguous, batch + 1 values each")
-    pitch = block_table.stride()
-    if len(pitch) != 2 or block_table.shape[0] < batch or pitch[1] != 1:
-        raise RuntimeError("paged_attn_prefill: block_table must have a row of contiguous entries per sequence")
-    lib = _lib.load()
-    rc = _call(pool.device, _call_prefill_window, lib, pool.handle, out.data_ptr(), q.data_ptr(), shape[0], cu_seqlens_q.data_ptr(),
-               cu_seqlens_k.data_ptr(), block_table.data_ptr(), pitch[0], batch, int(max_seqlen_q), int(max_seqlen_k), shape[1],
-               float(softmax_scale), window, sinks)
-    if rc:
-        _lib.check(rc, "paged_attn_prefill")
+    out = _host_ops().prefill_window(pool.address, pool.device.index, q, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k,
+                                     softmax_scale, block_table, out, window, sinks)
     if _CHECK:
         with _on_device(pool.device):
-            _check_prefill_status(lib, "paged_attn_prefill")
+            _check_prefill_status(_lib.load(), "paged_attn_prefill")
     return out
 
 

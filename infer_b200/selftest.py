@@ -13,12 +13,12 @@ from __future__ import annotations
 
 from contextlib import contextmanager
 
-from . import ops
+from . import _lib, ops
 
 
 @contextmanager
 def variant(decode_heads_per_tile: int = 0, prefill_kernel: int = 0, wait_limit: int = 0, stall_producer: int = 0):
-    saved = ops._call_decode, ops._call_prefill, ops._call_prefill_window, ops._call_dense
+    saved = ops._call_decode, ops._call_prefill, ops._call_dense
 
     def decode(lib, *args):
         return lib.infer_selftest_paged_decode(*args, decode_heads_per_tile, wait_limit, stall_producer)
@@ -26,14 +26,14 @@ def variant(decode_heads_per_tile: int = 0, prefill_kernel: int = 0, wait_limit:
     def prefill(lib, *args):
         return lib.infer_selftest_paged_prefill(*args, prefill_kernel, wait_limit, stall_producer)
 
-    def prefill_window(lib, *args):
-        return lib.infer_selftest_paged_prefill_window(*args, wait_limit, stall_producer)
-
     def dense(lib, *args):
         return lib.infer_selftest_flash_attn_prefill(*args, prefill_kernel)
 
-    ops._call_decode, ops._call_prefill, ops._call_prefill_window, ops._call_dense = decode, prefill, prefill_window, dense
+    ops._call_decode, ops._call_prefill, ops._call_dense = decode, prefill, dense
+    _lib.load()
+    _lib.host_ops.set_prefill_test(wait_limit, stall_producer)          # the windowed prefill call
     try:
         yield
     finally:
-        ops._call_decode, ops._call_prefill, ops._call_prefill_window, ops._call_dense = saved
+        ops._call_decode, ops._call_prefill, ops._call_dense = saved
+        _lib.host_ops.set_prefill_test(0, 0)
