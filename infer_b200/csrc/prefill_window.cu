@@ -246,7 +246,13 @@ __global__ void __launch_bounds__(PwCfg<FP8>::threads, 1) prefill_window_kernel(
     const int hw = int(threadIdx.x >> 5), lane = threadIdx.x & 31;
     const int warp = hw < 4 ? hw + kPwSoftmaxWarps : hw < 12 ? hw - 4 : hw;
 
+    // the producer's first look-ups, under the set-up below (thread 0 is the producer)
+    int seq_q0 = 0, seq_q1 = 0, seq_k0 = 0, seq_k1 = 0;
     if (threadIdx.x == 0) {
+        seq_q0 = p.cu_q[blockIdx.z];
+        seq_q1 = p.cu_q[blockIdx.z + 1];
+        seq_k0 = p.cu_k[blockIdx.z];
+        seq_k1 = p.cu_k[blockIdx.z + 1];
         mbar_init(bar(PW_Q_FULL), 1);
         mbar_init(bar(PW_Q_READY, 0), 4);
         mbar_init(bar(PW_Q_READY, 1), 4);
@@ -314,7 +320,7 @@ __global__ void __launch_bounds__(PwCfg<FP8>::threads, 1) prefill_window_kernel(
                 int bx = blockIdx.x, by = blockIdx.y, b = blockIdx.z;
                 while (ok) {
                     const int kvh = by / p.splits, split = by - kvh * p.splits;
-                    const int q0 = p.cu_q[b], lq = p.cu_q[b + 1] - q0, lk = p.cu_k[b + 1] - p.cu_k[b];
+                    const int q0 = seq_q0, lq = seq_q1 - q0, lk = seq_k1 - seq_k0;
                     const int shift = lk - lq;                              // position of the first query row
                     const int tok0 = (int(gridDim.x) - 1 - bx) * 2 * p.tokens;     // longest rows first
                     auto ask = [&] {
@@ -336,6 +342,16 @@ __global__ void __launch_bounds__(PwCfg<FP8>::threads, 1) prefill_window_kernel(
                         const int x0 = min(n_all, split * per_split), n = min(n_all, x0 + per_split) - x0;
                         auto tile_at = [&](int j) { return x0 + j < n_sink ? x0 + j : x0 + j + skip; };
                         const bool two = tok0 + p.tokens < lq;
+                        if (n > 0 && !p.stall_producer) {
+                            if (!tc_wait(bar(PW_Q_EMPTY), (q_loads & 1) ^ 1, s_abort, p.wait_limit)) { ok = false; break; }
+                            const int n_q = two ? 2 : 1;
+                            mbar_expect_tx(bar(PW_Q_FULL), n_q * 2 * p.tokens * p.group * 128);
+                            for (int i = 0; i < n_q; ++i)
+                                for (int half = 0; half < 2; ++half)
+                                    tma_load_3d(base + C::q + i * kPwTile + half * kPwHalf, &map_q, bar(PW_Q_FULL), half * 64,
+                                                kvh * p.group, q0 + tok0 + i * p.tokens);
+                            ++q_loads;
+                        }
                         if (!tc_wait(bar(PW_ITEM_EMPTY, item & 1), ((item >> 1) & 1) ^ 1, s_abort, p.wait_limit)) { ok = false; break; }
                         volatile int* e = s_item + (item & 1) * PI_INTS;
                         e[PI_TILES] = n;
@@ -354,14 +370,6 @@ __global__ void __launch_bounds__(PwCfg<FP8>::threads, 1) prefill_window_kernel(
                             break;
                         }
                         if (n > 0) {
-                            if (!tc_wait(bar(PW_Q_EMPTY), (q_loads & 1) ^ 1, s_abort, p.wait_limit)) { ok = false; break; }
-                            const int n_q = two ? 2 : 1;
-                            mbar_expect_tx(bar(PW_Q_FULL), n_q * 2 * p.tokens * p.group * 128);
-                            for (int i = 0; i < n_q; ++i)
-                                for (int half = 0; half < 2; ++half)
-                                    tma_load_3d(base + C::q + i * kPwTile + half * kPwHalf, &map_q, bar(PW_Q_FULL), half * 64,
-                                                kvh * p.group, q0 + tok0 + i * p.tokens);
-                            ++q_loads;
                             const int32_t* table = p.block_tables + int64_t(b) * p.bt_stride;
                             auto page_of = [&](int j) {                     // -1: outside of the table or of the pool
                                 const int idx = j < n ? tile_at(j) * kPwKeys / p.block_size : 0;
@@ -447,6 +455,10 @@ __global__ void __launch_bounds__(PwCfg<FP8>::threads, 1) prefill_window_kernel(
                     ++claims;
                     asked = false;
                     if (!claim_result(base + C::claim, bx, by, b)) break;
+                    seq_q0 = p.cu_q[b];
+                    seq_q1 = p.cu_q[b + 1];
+                    seq_k0 = p.cu_k[b];
+                    seq_k1 = p.cu_k[b + 1];
                 }
                 if (ok && !stalled) {
                     if (tc_wait(bar(PW_ITEM_EMPTY, item & 1), ((item >> 1) & 1) ^ 1, s_abort, p.wait_limit)) {
