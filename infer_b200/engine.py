@@ -101,7 +101,8 @@ class AttentionLayerModel(torch.nn.Module):
     weights from a seeded generator."""
 
     def __init__(self, hidden: int, n_q_heads: int, n_kv_heads: int, vocab: int, max_position: int, device, seed: int = 0,
-                 eps: float = 1e-6):
+                 eps: float = 1e-6, window: int | None = None, sinks: int = 0):
+        """``window`` / ``sinks``: a sliding-window layer (see ``Attention``)."""
         super().__init__()
         d = 128
         gen = torch.Generator().manual_seed(seed)
@@ -116,7 +117,7 @@ class AttentionLayerModel(torch.nn.Module):
         inv_freq = 1.0 / (10000.0 ** (torch.arange(0, d, 2).float() / d))
         ang = torch.arange(max_position).float()[:, None] * inv_freq[None]
         self.cos, self.sin = ang.cos().bfloat16().to(device), ang.sin().bfloat16().to(device)
-        self.attn = Attention(n_q_heads, d, d ** -0.5, n_kv_heads)
+        self.attn = Attention(n_q_heads, d, d ** -0.5, n_kv_heads, window, sinks)
         self.tap = None            # when a dict: receives the tensors handed to / returned by the attention path
 
     def _norm_rope(self, x, weight, positions):
@@ -149,8 +150,11 @@ class LayerRunner:
     prefill, decode through per-bucket CUDA graphs over static buffers."""
 
     def __init__(self, model: AttentionLayerModel, num_blocks: int, block_size: int, max_num_seqs: int, max_model_len: int,
-                 device, enforce_eager: bool = False, device_metadata: bool = False):
-        """``device_metadata``: keep the decode step's metadata on the GPU (``metadata.DecodeState``): while the
+                 device, enforce_eager: bool = False, device_metadata: bool = False, kv_dtype: str = "bf16"):
+        """``kv_dtype``: "bf16", or "e4m3" for pools of 8-bit values with a scale per page and KV head; a page that a
+        sequence gets anew starts with scale 0, as if it had never been written.
+
+        ``device_metadata``: keep the decode step's metadata on the GPU (``metadata.DecodeState``): while the
         batch keeps its composition a step costs one small kernel (lengths + 1, slots and positions from the block
         tables already on the device) and the upload of newly allocated page ids, instead of the reference's
         per-step rebuild and upload (infer/engine/model_runner.py:110-126); the graphs read the state's tensors."""
@@ -161,8 +165,15 @@ class LayerRunner:
             self.state = metadata.DecodeState(min(max_num_seqs, 512), self.max_pages, block_size, self.device)
             self._state_ids, self._state_lens = None, None
         # one zero-filled tensor [2, num_blocks, block_size, Hkv, 128]; the layer gets its two halves
-        self.kv_cache = torch.zeros(2, num_blocks, block_size, model.n_kv_heads, 128, dtype=torch.bfloat16, device=device)
+        if kv_dtype not in ("bf16", "e4m3"):
+            raise ValueError(f"LayerRunner: kv_dtype must be 'bf16' or 'e4m3', not {kv_dtype!r}")
+        self.kv_cache = torch.zeros(2, num_blocks, block_size, model.n_kv_heads, 128, device=device,
+                                    dtype=torch.bfloat16 if kv_dtype == "bf16" else torch.uint8)
         model.attn.k_cache, model.attn.v_cache = self.kv_cache[0], self.kv_cache[1]
+        self.kv_scale = None
+        if kv_dtype == "e4m3":
+            self.kv_scale = torch.zeros(2, num_blocks, model.n_kv_heads, device=device)
+            model.attn.k_scale, model.attn.v_scale = self.kv_scale[0], self.kv_scale[1]
         self.graphs, self.graph_taps, self.graph_bs = {}, {}, []
         self.last_tap, self.last_bucket = None, None
         if not enforce_eager:
@@ -231,9 +242,20 @@ class LayerRunner:
         self.last_tap, self.last_bucket = self.graph_taps[bs], bs
         return self.model.compute_logits(v["outputs"][:n])
 
+    def _start_pages(self, seqs, is_prefill: bool):
+        """The scales that the last owners of this step's new pages left behind go back to zero."""
+        if is_prefill:
+            pages = [p for s in seqs for p in s.block_table[s.num_cached_blocks:]]
+        else:
+            pages = [s.block_table[-1] for s in seqs if len(s) % self.block_size == 1]
+        if pages:
+            self.kv_scale[:, torch.tensor(pages, dtype=torch.int64).to(self.device)] = 0
+
     def run(self, seqs, is_prefill: bool):
         """-> sampled token ids (greedy).  Prefill always publishes block tables: the keys are read from
         the pools, also when no prefix is cached."""
+        if self.kv_scale is not None:
+            self._start_pages(seqs, is_prefill)
         if is_prefill:
             input_ids, positions = metadata.prepare_prefill(seqs, self.block_size, self.device)
             ctx = get_context()

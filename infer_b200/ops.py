@@ -467,6 +467,26 @@ def register_torch_ops():
                "Tensor block_table, float softmax_scale) -> ()")
     lib.define("paged_attn_prefill(Tensor! out, Tensor q, Tensor k_cache, Tensor v_cache, Tensor cu_seqlens_q, "
                "Tensor cu_seqlens_k, int max_seqlen_q, int max_seqlen_k, float softmax_scale, Tensor block_table) -> ()")
+    lib.define("paged_attn_decode_window(Tensor! out, Tensor q, Tensor k_cache, Tensor v_cache, Tensor cache_seqlens, "
+               "Tensor block_table, float softmax_scale, int window, int sinks, Tensor? k_scale=None, Tensor? v_scale=None) -> ()")
+    lib.define("paged_attn_prefill_window(Tensor! out, Tensor q, Tensor k_cache, Tensor v_cache, Tensor cu_seqlens_q, "
+               "Tensor cu_seqlens_k, int max_seqlen_q, int max_seqlen_k, float softmax_scale, Tensor block_table, int? window, "
+               "int sinks, Tensor? k_scale=None, Tensor? v_scale=None) -> ()")
+    lib.define("load_kvcache(Tensor! k_out, Tensor! v_out, Tensor k_cache, Tensor v_cache, Tensor slot_mapping, "
+               "Tensor? k_scale=None, Tensor? v_scale=None) -> ()")
+    lib.define("rotary_append(Tensor! q_out, Tensor q, Tensor k, Tensor v, Tensor positions, Tensor inv_freq, Tensor! k_cache, "
+               "Tensor! v_cache, Tensor slot_mapping, bool interleaved, float attention_factor) -> ()")
+    lib.impl("paged_attn_decode_window",
+             lambda out, q, kc, vc, sl, bt, sc, w, sk, ks=None, vs=None:
+             (paged_attn_decode(q, kc, vc, sl, bt, sc, out=out, k_scale=ks, v_scale=vs, window=w, sinks=sk), None)[1], "CUDA")
+    lib.impl("paged_attn_prefill_window",
+             lambda out, q, kc, vc, cq, ck, mq, mk, sc, bt, w, sk, ks=None, vs=None:
+             (paged_attn_prefill(q, kc, vc, cq, ck, mq, mk, sc, bt, out=out, k_scale=ks, v_scale=vs, window=w, sinks=sk), None)[1],
+             "CUDA")
+    lib.impl("load_kvcache", lambda ko, vo, kc, vc, sm, ks=None, vs=None:
+             (load_kvcache(kc, vc, sm, k_scale=ks, v_scale=vs, k_out=ko, v_out=vo), None)[1], "CUDA")
+    lib.impl("rotary_append", lambda qo, q, k, v, p, f, kc, vc, sm, il, af:
+             (rotary_append(q, k, v, p, f, kc, vc, sm, interleaved=il, attention_factor=af, q_out=qo), None)[1], "CUDA")
     lib.impl("flash_attn_prefill", lambda Q, K, V, O: flash_attn_prefill(Q, K, V, O), "CUDA")
     lib.impl("store_kvcache", lambda k, v, kc, vc, sm: store_kvcache(k, v, kc, vc, sm), "CUDA")
     lib.impl("paged_attn_decode",
