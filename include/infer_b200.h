@@ -209,7 +209,9 @@ INFER_API int infer_paged_prefill(const infer_kv_pool_t* pool, void* out, const 
  * its sequence sees key j <= i when i - j < window or j < sinks.  window = 0: every key j <= i (sinks is then without
  * effect).  The alignment of queries and keys is that of infer_paged_prefill; a query that sees no key (a sequence with
  * fewer keys than queries) gives zeros, rows of out that belong to no sequence are left alone, and block-table entries
- * of pages without a visible key are not read.  Up to 128 query heads per kv head.  max_seqlen_q has to cover the longest
+ * of pages without a visible key are not read; a page id outside of the pool, or a key behind the table's columns, counts
+ * as rows of zeros.  Values that no query of a sequence sees may be anything; a NaN or an infinity that only some of a
+ * chunk's queries see may reach the others (0 times it is NaN).  Up to 128 query heads per kv head.  max_seqlen_q has to cover the longest
  * chunk; max_seqlen_k (the longest context) only guides over how many thread blocks few rows' keys are split.
  * softmax_scale: a positive finite number. */
 INFER_API int infer_paged_prefill_window(const infer_kv_pool_t* pool, void* out, const void* q, int64_t total_q,

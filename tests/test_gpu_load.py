@@ -51,6 +51,19 @@ def test_load_into_slices_of_a_wider_row_and_large_pages():
     assert bool((wide[:, :256] == 7.0).all())
 
 
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+def test_load_into_rows_at_sixteen_bytes(kind):
+    gen = torch.Generator().manual_seed(13)
+    k, v, ks, vs = _pool(kind, 3, 256, 2, gen)
+    slots = torch.randperm(3 * 256, generator=gen)[:77].to(torch.int32).cuda()
+    want = ops.load_kvcache(k, v, slots, k_scale=ks, v_scale=vs)
+    wide = torch.zeros(77, 2 * 256 + 24, dtype=torch.bfloat16, device="cuda")
+    k_out, v_out = wide[:, 8:264].view(77, 2, 128), wide[:, 264:520].view(77, 2, 128)
+    assert k_out.data_ptr() % 32 == 16
+    ops.load_kvcache(k, v, slots, k_scale=ks, v_scale=vs, k_out=k_out, v_out=v_out)
+    assert torch.equal(k_out, want[0]) and torch.equal(v_out, want[1])
+
+
 def test_store_then_load_round_trip():
     """bf16: the stored bits; e4m3: within half a step of the format (2^-4) of the row, or of its subnormals."""
     gen = torch.Generator().manual_seed(6)

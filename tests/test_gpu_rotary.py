@@ -85,6 +85,25 @@ def test_rotary_in_place_and_through_an_8_bit_cache():
     assert bool(((back.double() - x).abs() <= (2.0 ** -4 + 2.0 ** -7) * x.abs() + 2.0 ** -10 * ks[0][:, None].double()).all())
 
 
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rotary_on_rows_at_sixteen_bytes(interleaved):
+    """Columns and pitches that are multiples of 16 bytes but not of 32 take the narrow accesses, with the same result."""
+    gen = torch.Generator().manual_seed(12)
+    hq, hkv, t = 6, 2, 50
+    wide = torch.randn(t, (hq + 2 * hkv) * 128 + 24, generator=gen).bfloat16().cuda()
+    q, k, v = (x.view(t, -1, 128) for x in wide[:, 8:8 + (hq + 2 * hkv) * 128].split([hq * 128, hkv * 128, hkv * 128], dim=1))
+    assert q.data_ptr() % 32 == 16 and q.stride(0) % 16 == 8
+    positions = torch.arange(t, device="cuda") * 37
+    inv_freq, _ = rotary_frequencies(96, device="cuda")
+    want = ops.rotary_embedding(q.contiguous(), k.contiguous(), positions, inv_freq, interleaved=interleaved)
+    got = ops.rotary_embedding(q, k, positions, inv_freq, interleaved=interleaved)
+    assert bits_equal(got[0], want[0]) and bits_equal(got[1], want[1])
+    kc, vc = (torch.zeros(1, 256, hkv, 128, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    slots = torch.arange(t, dtype=torch.int32, device="cuda")
+    assert bits_equal(ops.rotary_append(q, k, v, positions, inv_freq, kc, vc, slots, interleaved=interleaved), want[0])
+    assert bits_equal(kc[0, :t], want[1]) and bits_equal(vc[0, :t], v)
+
+
 def test_rotary_in_a_graph():
     gen = torch.Generator().manual_seed(9)
     q, k, v = _rows(64, 16, 8, gen)

@@ -158,8 +158,30 @@ def test_in_a_graph_with_growing_lengths_and_own_workspace(kind):
         _check(c, out, 100, 4)
 
 
+def test_pinned_host_queries_and_output_and_four_dims():
+    for kind in ("bf16", "e4m3"):
+        c = _case(kind, [700, 30], 8, 2, 31)
+        want = _run(c, 100, 4)
+        q, out = c["q"].cpu().pin_memory(), torch.zeros(2, 8, 128, dtype=torch.bfloat16).pin_memory()
+        got = _run({**c, "q": q}, 100, 4, out=out)
+        torch.cuda.synchronize()
+        assert got.data_ptr() == out.data_ptr() and bits_equal(out, want)
+        four = _run({**c, "q": c["q"][:, None]}, 100, 4)
+        assert four.shape == (2, 1, 8, 128) and bits_equal(four[:, 0], want)
+
+
 def test_refusals():
     c = _case("bf16", [100, 30], 8, 2, 29)
+    with pytest.raises(RuntimeError, match="pinned"):
+        _run({**c, "q": c["q"].cpu()}, 10, 0)
+    with pytest.raises(RuntimeError, match="cache_seqlens"):
+        _run({**c, "lens": c["lens"][:1]}, 10, 0)
+    with pytest.raises(RuntimeError, match="block_table"):
+        _run({**c, "bt": c["bt"].long()}, 10, 0)
+    with pytest.raises(RuntimeError, match="out must"):
+        _run(c, 10, 0, out=torch.zeros(2, 8, 128, device="cuda"))
+    with pytest.raises(RuntimeError, match="key must"):
+        ops.paged_attn_decode_append(c["q"], c["q"], c["q"], c["k"], c["v"], c["lens"], c["bt"], SCALE, window=5)
     with pytest.raises(RuntimeError, match="window"):
         _run(c, 0, 0)
     with pytest.raises(RuntimeError, match="sinks"):

@@ -215,6 +215,65 @@ def test_waits_that_run_out_are_reported(kind, chunks):
     assert bits_equal(_run(c, 500, 4), want)
 
 
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+def test_pages_outside_of_the_pool_and_narrow_tables_read_as_zeros(kind):
+    c = _case(kind, [(700, 130), (600, 3)], 8, 2, 83)
+    clean = {x: c[x].clone() for x in "kv"}
+    top = 448 * c["vs"].amax().double() if kind == "e4m3" else c["v"].abs().amax().double()
+    for x in "kv":
+        for b in (0, 1):
+            c[x][c["tables"][b][1]] = 0
+    want = _run(c, 600, 4)
+    for x in "kv":
+        c[x].copy_(clean[x])
+    bt = c["bt"]
+    for bad in (-1, bt.max().item() + 50, 2 ** 31 - 1, -2 ** 31):
+        c["bt"] = bt.clone()
+        c["bt"][:2, 1] = bad
+        if kind == "bf16":
+            assert bits_equal(_run(c, 600, 4), want)
+        else:
+            # a page without a place has no V scale either, so the f16 probabilities are taken in other units: half a step
+            # (2^-11) of each on either side, and half a step (2^-8) of the result on either side
+            plain64.check(_run(c, 600, 4), want.double(), 2.0 ** -7 * want.double().abs() + 2.0 ** -10 * top)
+    # keys behind the table's columns
+    c["bt"] = bt
+    for x in "kv":
+        for b in (0, 1):
+            c[x][c["tables"][b][2]] = 0
+    want = _run(c, 600, 4)
+    for x in "kv":
+        c[x].copy_(clean[x])
+    c["bt"] = bt[:, :2].contiguous()
+    got = _run(c, 600, 4)
+    assert torch.isfinite(got).all()
+    plain64.check(got, want.double(), 2.0 ** -7 * want.double().abs() + 2.0 ** (-10 if kind == "e4m3" else -7) * top)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+def test_queries_that_are_not_finite_stay_their_own(kind):
+    """A NaN or an infinity in one query's row gives NaN there and nowhere else, split or not."""
+    for chunks in ([(700, 300)], [(4000, 5)]):
+        c = _case(kind, chunks, 8, 2, 89)
+        want = _run(c, 3000, 4)
+        c["q"][2, 3, 17] = float("nan")
+        c["q"][4, 5, 0] = float("inf")
+        got = _run(c, 3000, 4)
+        assert torch.isnan(got[2, 3]).all() and torch.isnan(got[4, 5]).all()
+        got[2, 3], got[4, 5] = want[2, 3], want[4, 5]
+        assert bits_equal(got, want)
+
+
+def test_sixteen_byte_aligned_queries_and_output():
+    c = _case("e4m3", [(500, 200)], 8, 2, 97)
+    want = _run(c, 300, 4)
+    buf = torch.zeros(2, c["q"].numel() + 8, dtype=torch.bfloat16, device="cuda")
+    q, out = (b[8:].view(c["q"].shape) for b in buf)
+    assert q.data_ptr() % 32 == 16
+    q.copy_(c["q"])
+    assert bits_equal(_run({**c, "q": q}, 300, 4, out=out), want)
+
+
 def test_refusals():
     c = _case("e4m3", [(300, 10)], 8, 2, 79)
     for kw, match in ((dict(window=0), "window"), (dict(window=5, sinks=-1), "sinks"), (dict(sinks=3), "sinks"),
