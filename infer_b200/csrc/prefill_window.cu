@@ -19,7 +19,7 @@
 //   warps finish the current one.  Launched one by one, a CTA cost about 6 us beyond its tiles, a third of the time of a
 //   window of 1024 keys.
 // Few rows.  When the (row block, kv head, sequence) triples do not fill the GPU, the key tiles of a row block are split over
-//   the CTAs of a cluster (up to 16), which join their parts through distributed shared memory: maxima and sums first, then
+//   the CTAs of a cluster (2 to 16), which join their parts through distributed shared memory: maxima and sums first, then
 //   every CTA scales its accumulator and leaves it in shared memory, and the rows are summed in turn.  No scratch in global
 //   memory, no second kernel.
 // e4m3.  S = Q K^T runs on the raw bytes of K (kind::f8f6f4, no conversion): a bf16 value has 8 significant bits, so it is
@@ -38,6 +38,7 @@
 //
 // Every wait is bounded; one that runs out raises the abort flag, every role drains to the common epilogue, tensor memory
 // is freed and the status word of the prefill kernels is set.
+#include <algorithm>
 #include <atomic>
 #include <mutex>
 
@@ -684,8 +685,8 @@ __global__ void __launch_bounds__(PwCfg<FP8>::threads, 1) prefill_window_kernel(
         if (left == 0) tiles += n_all;                             // this query tile has no rows
         const bool any_tile = left > 0;
         if (FP8 && any_tile) {
-            // this thread's row of Q: one row block's tiles take 256 threads about a microsecond; by the converters, four warps
-            // that also yield to these, they took six
+            // this thread's row of Q: one row block's tiles take 256 threads 1.8 us; by the converters, four warps that also
+            // yield to these, they took 6.5
             if (!tc_wait(bar(PW_Q_FULL), q_uses & 1, s_abort, p.wait_limit)) ok = false;
             if (ok) {
                 c_row = p.scale_log2 * split_q_row(base + C::q + g * kPwTile, r);
@@ -919,10 +920,13 @@ __global__ void __launch_bounds__(PwCfg<FP8>::threads, 1) prefill_window_kernel(
     if (threadIdx.x == 0 && *s_abort && p.status) atomicExch(p.status, 0x5AFE0006);
 }
 
-// What a launch over clusters needs to know of a device: how many clusters of 2, 4, 8 and 16 CTAs fit at a time.
+// What a launch over clusters needs to know of a device: how many clusters of 2 .. 16 CTAs fit at a time (their sizes do not
+// divide the GPCs evenly: 74, 45, 33, 26, 22, 15, 15, 15, 11 and 7 from 11 CTAs on).
+constexpr int kPwMaxSplits = 16;
 struct PwDevice {
     std::atomic<bool> ready{false};
-    int clusters[4] = {0, 0, 0, 0};
+    int clusters[kPwMaxSplits + 1] = {};
+    int sm_count = 0;
 };
 
 // The launch configuration; attr has to outlive it.
@@ -961,42 +965,66 @@ static int prefill_device(const PwDevice** out) {
     const int smem = PwCfg<FP8>::total + 1024;
     IB_CUDA(cudaFuncSetAttribute(prefill_window_kernel<FP8>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     IB_CUDA(cudaFuncSetAttribute(prefill_window_kernel<FP8>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-    for (int i = 0; i < 4; ++i) {
+    IB_CUDA(cudaDeviceGetAttribute(&d.sm_count, cudaDevAttrMultiProcessorCount, dev));
+    for (int size = 2; size <= kPwMaxSplits; ++size) {
         cudaLaunchAttribute attr;
-        const int size = 2 << i;
         const cudaLaunchConfig_t cfg = prefill_config(dim3(1, size, 1), PwCfg<FP8>::threads, smem, size, nullptr, &attr);
         int n = 0;
         if (cudaOccupancyMaxActiveClusters(&n, prefill_window_kernel<FP8>, &cfg) != cudaSuccess) {
             (void)cudaGetLastError();
             n = 0;
         }
-        d.clusters[i] = n;
+        d.clusters[size] = n;
     }
     d.ready.store(true, std::memory_order_release);
     return INFER_OK;
 }
 
-// Over how many CTAs the key tiles of a row block are spread: the largest cluster size of which all row blocks run at the
-// same time and that leaves every CTA three tiles or more (a tile takes about 1.6 us, the join 4).
-static int prefill_splits(const PwDevice& d, int64_t blocks, int64_t max_k, int tokens, int window, int sinks) {
+// Over how many CTAs the key tiles of a row block are spread: the number that an estimate of the time makes best.  Measured,
+// e4m3, us, with the choice in brackets:
+//     rows behind keys (heads)          1        2      4      5      7      8      10
+//     45 behind 300 (32 / 8)          [12.8]  17.1   13.6   14.3   15.3   14.1   15.8
+//     45 behind 600                    17.7   19.6   15.8   16.6   15.4  [14.3]  15.9
+//     45 behind 8000                  106.8   63.7   37.0   33.3   28.5  [25.5]  25.8
+//     4 x 60 behind 9900 (18 / 3)     131.4   78.3   45.5  [41.5]  66.7   59.2   75.3     a second wave from 6 on
+//     8 x 16 behind 1500 (32 / 8)      23.3  [20.8]  31.6   42.9   66.9   63.2   84.0
+//     2 x 200 behind 900 (40 / 8)     [23.5]  26.1   39.1   52.6   87.7   78.8  109.2
+//     1200, 4 x 1 behind 8000 (8 / 2) 123.3  [73.4]  88.7  100.1  135.3  125.9  163.5     most row blocks lie behind their sequence
+static int prefill_splits(const PwDevice& d, int64_t blocks, int64_t empty, int64_t max_k, int tokens, int window, int sinks) {
     int64_t tiles = (max_k + kPwKeys - 1) / kPwKeys;
     if (window > 0) {
         const int64_t seen = (int64_t(window) + 2 * tokens + kPwKeys - 1) / kPwKeys + 1 + (int64_t(sinks) + kPwKeys - 1) / kPwKeys;
         if (seen < tiles) tiles = seen;
     }
-    for (int i = 3; i >= 0; --i)
-        if (blocks <= d.clusters[i] && tiles >= int64_t(3) * (2 << i)) return 2 << i;
-    return 1;
+    // us: a key tile, the set-up, a row block, a join at least, a cluster whose row block lies behind its sequence; a cluster
+    // whose size is no power of two and one of more than eight CTAs start later
+    constexpr double kTile = 1.5, kFirst = 6., kNext = 2., kJoin = 3.5, kEmpty = 3., kOdd = 1., kWide = 1.5;
+    const int64_t turns = (blocks + d.sm_count - 1) / d.sm_count;
+    double best = kFirst + double(turns) * (double(tiles) * kTile + kNext);
+    int splits = 1;
+    for (int s = 2; s <= kPwMaxSplits; ++s) {
+        if (d.clusters[s] <= 0) continue;
+        const int64_t waves = (blocks + d.clusters[s] - 1) / d.clusters[s];
+        const double one = kFirst + kNext + kJoin + 6. / s + double((tiles + s - 1) / s) * kTile + (s & (s - 1) ? kOdd : 0.) + (s > 8 ? kWide : 0.);
+        const double t = double(waves) * one + double(empty) / d.clusters[s] * kEmpty;
+        if (t < best) {
+            best = t;
+            splits = s;
+        }
+    }
+    return splits;
 }
 
 template <bool FP8>
-static int launch_prefill_window(PwParams& p, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, int max_q, int max_k,
-                                 int window, int batch, cudaStream_t st) {
+static int launch_prefill_window(PwParams& p, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, int64_t total_q,
+                                 int max_q, int max_k, int window, int batch, cudaStream_t st) {
     const PwDevice* d = nullptr;
     const int rc = prefill_device<FP8>(&d);
     if (rc != INFER_OK) return rc;
     const int64_t row_blocks = (int64_t(max_q) + 2 * p.tokens - 1) / (2 * p.tokens);
-    p.splits = prefill_splits(*d, row_blocks * p.n_kv_heads * batch, max_k, p.tokens, window, p.sinks);
+    // row blocks that hold rows: no more than this, whatever the lengths
+    const int64_t filled = std::min(row_blocks * batch, total_q / (2 * p.tokens) + batch);
+    p.splits = prefill_splits(*d, filled * p.n_kv_heads, (row_blocks * batch - filled) * p.n_kv_heads, max_k, p.tokens, window, p.sinks);
     cudaLaunchAttribute attr;
     const cudaLaunchConfig_t cfg = prefill_config(dim3(unsigned(row_blocks), p.n_kv_heads * p.splits, batch), PwCfg<FP8>::threads,
                                                   PwCfg<FP8>::total + 1024, p.splits, st, &attr);
@@ -1042,8 +1070,10 @@ static int paged_prefill_window(const infer_kv_pool_t* pool, void* out, const vo
                            uint32_t(p.group), uint32_t(p.tokens));
     if (rc != INFER_OK) return rc;
     if (pool->dtype == INFER_KV_E4M3)
-        return launch_prefill_window<true>(p, mq, pool->maps[3].k, pool->maps[3].v, max_seqlen_q, max_seqlen_k, window, batch, st);
-    return launch_prefill_window<false>(p, mq, pool->maps[3].k, pool->maps[3].v, max_seqlen_q, max_seqlen_k, window, batch, st);
+        return launch_prefill_window<true>(p, mq, pool->maps[3].k, pool->maps[3].v, total_q, max_seqlen_q, max_seqlen_k, window,
+                                           batch, st);
+    return launch_prefill_window<false>(p, mq, pool->maps[3].k, pool->maps[3].v, total_q, max_seqlen_q, max_seqlen_k, window,
+                                           batch, st);
 }
 
 }  // namespace ib
