@@ -2,7 +2,7 @@
 //
 // A decode step's rotary_append or load_kvcache runs 2-4 us on the GPU; checked and launched from Python through ctypes the
 // call cost the host 12-14 us (an output tensor 2.4, the current stream 3.1, a ctypes call with 18 arguments 1.6, every
-// look at a tensor's type, shape or address 0.1), from here 4-5.  The module is bound to libinfer_b200.so by address, so
+// look at a tensor's type, shape or address 0.1), from here 5-6.  The module is bound to libinfer_b200.so by address, so
 // that there is one library in the process, the one that infer_b200/_lib.py has loaded.
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAGuard.h>

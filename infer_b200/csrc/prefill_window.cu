@@ -13,7 +13,10 @@
 //   1.4 tiles instead of four a third full, and a tile spans few positions, so that a window cuts its key range close.
 // Keys.  A CTA walks the tiles that hold a key visible to any of its rows: those of the sinks, then those from the start
 //   of its first row's window on.  Block-table entries of other pages are never read.  V rows that no row of the CTA sees
-//   are cleared before the tensor core reads them: P is 0 there, but 0 times a stale NaN is not.
+//   are cleared before the tensor core reads them: P is 0 there, but 0 times a stale NaN is not.  bf16: up to 64 sinks go into
+//   the rows of the window's first tile that lie in front of the window, where there are enough of them, instead of a tile of
+//   their own (16 sequences of 2048 rows, a window of 200 and 20 sinks 173 -> 146 us, of 1024 and four 3-8 %); an e4m3
+//   tile has one scale.
 // Many CTAs.  A CTA that is done takes over one that has not been launched yet (clusterlaunchcontrol): barriers, tensor
 //   memory and roles stay, and the Q and first K tiles of the next row block are loaded (and converted) while the softmax
 //   warps finish the current one.  Launched one by one, a CTA cost about 6 us beyond its tiles, a third of the time of a
@@ -53,7 +56,7 @@ constexpr int kPwHalf = 128 * 128;            // bytes of one [128 rows][64 elem
 constexpr int kPwTile = 2 * kPwHalf;          // 32 KiB: one Q, K or V tile of 16-bit elements
 constexpr int kPwRaw = 128 * 128;             // 16 KiB: one K or V tile of e4m3 bytes
 constexpr int kPwRing = 8;                    // entries of the tile ring: one lives from its K's load to its P V product, 7 tiles at most
-// A tile's entry: whether some row of the CTA sees only part of it, its first key; e4m3: k scale, what O is multiplied by in
+// A tile's entry: whether some row of the CTA sees only part of it (2: and its first rows are the sinks), its first key; e4m3: k scale, what O is multiplied by in
 // front of this tile (1 as a rule), what the V scale adds to the exponents of P, what takes it out of a row sum again, the V
 // scale that O is expressed in from there on; the rows that some query sees, [0, sink_end) and [begin, end).
 enum PwTileEntry { PT_CUT, PT_KEY0, PT_K_SCALE, PT_O_FACTOR, PT_UP, PT_DOWN, PT_V_REF, PT_SINK_END = 8, PT_BEGIN, PT_END, PT_INTS = 16 };
@@ -136,6 +139,17 @@ struct PwParams {
     uint32_t wait_limit;
     int stall_producer;
 };
+
+// Boxes of 16, 32 and 64 token rows.
+constexpr int kPwParts = 3;
+template <bool FP8>
+struct PwParts {
+    CUtensorMap k[kPwParts], v[kPwParts];
+};
+template <>
+struct PwParts<true> {};         // an e4m3 tile has one scale
+__device__ __forceinline__ const CUtensorMap* part_of(const PwParts<false>& p, bool v) { return v ? p.v : p.k; }
+__device__ __forceinline__ const CUtensorMap* part_of(const PwParts<true>&, bool) { return nullptr; }
 
 // tc_wait for warps that wait most of the time and can be late: they sleep between looks, since their polling takes issue slots
 // from the softmax warps (the converters polling like the others: 507 us, sleeping: 495 us for 148 x 8 row blocks).
@@ -232,7 +246,8 @@ __device__ __forceinline__ float split_q_row(uint32_t tile, int t) {
 template <bool FP8>
 __global__ void __launch_bounds__(PwCfg<FP8>::threads, 1) prefill_window_kernel(PwParams p, const __grid_constant__ CUtensorMap map_q,
                                                                                 const __grid_constant__ CUtensorMap map_k,
-                                                                                const __grid_constant__ CUtensorMap map_v) {
+                                                                                const __grid_constant__ CUtensorMap map_v,
+                                                                                const __grid_constant__ PwParts<FP8> parts) {
     using C = PwCfg<FP8>;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -336,8 +351,18 @@ __global__ void __launch_bounds__(PwCfg<FP8>::threads, 1) prefill_window_kernel(
                         const int first_key = windowed ? max(pos_lo - p.window + 1, 0) : 0;
                         const int sinks = windowed ? min(p.sinks, lk) : 0;
                         int n_sink = (sinks + kPwKeys - 1) / kPwKeys;
-                        const int skip = max(first_key / kPwKeys - n_sink, 0);
+                        int skip = max(first_key / kPwKeys - n_sink, 0);
                         if (skip == 0) n_sink = 0;
+                        // sinks in the rows of the window's first tile that lie in front of the window: 0, or 16, 32, 64 rows
+                        int sink_rows = 0;
+                        if (!FP8 && sinks > 0 && sinks <= 64 && first_key >= kPwKeys) {
+                            const int rows = sinks <= 16 ? 16 : sinks <= 32 ? 32 : 64;
+                            if (rows <= first_key % kPwKeys) {
+                                sink_rows = rows;
+                                n_sink = 0;
+                                skip = first_key / kPwKeys;
+                            }
+                        }
                         const int n_all = pos_hi < 0 ? 0 : pos_hi / kPwKeys + 1 - skip;
                         const int per_split = (n_all + p.splits - 1) / p.splits;
                         const int x0 = min(n_all, split * per_split), n = min(n_all, x0 + per_split) - x0;
@@ -372,18 +397,36 @@ __global__ void __launch_bounds__(PwCfg<FP8>::threads, 1) prefill_window_kernel(
                         }
                         if (n > 0) {
                             const int32_t* table = p.block_tables + int64_t(b) * p.bt_stride;
-                            auto page_of = [&](int j) {                     // -1: outside of the table or of the pool
-                                const int idx = j < n ? tile_at(j) * kPwKeys / p.block_size : 0;
+                            auto page_at = [&](int key) {                   // -1: outside of the table or of the pool
+                                const int idx = key / p.block_size;
                                 const int page = idx < p.bt_stride ? table[idx] : -1;
                                 return page >= 0 && page < p.num_blocks ? page : -1;
                             };
+                            auto page_of = [&](int j) { return page_at(j < n ? tile_at(j) * kPwKeys : 0); };
                             auto scale_of = [&](const float* scale, int page) {
                                 return FP8 && page >= 0 ? scale[int64_t(page) * p.n_kv_heads + kvh] : 0.f;
                             };
                             // a page is looked up two tiles ahead and its scales one tile ahead: neither load is waited for
+                            const int sink_page = sink_rows > 0 && x0 == 0 ? page_at(0) : -1;
                             int page = page_of(0), page_next = page_of(1), v_slot = 0;
                             float k_scale = scale_of(p.k_scale, page), v_scale = scale_of(p.v_scale, page);
                             constexpr int lag = FP8 ? 0 : 1;
+                            // a tile of K or V; the window's first with the sinks in its first rows
+                            auto load = [&](uint32_t dst, const CUtensorMap* map, const CUtensorMap* part, uint32_t full, int j, int from) {
+                                if constexpr (FP8) {
+                                    tma_load_3d(dst, map, full, 0, kvh, from);
+                                } else if (x0 + j > 0 || sink_rows == 0) {
+                                    tma_load_3d(dst, map, full, 0, kvh, from);
+                                    tma_load_3d(dst + kPwHalf, map, full, 64, kvh, from);
+                                } else {
+                                    for (int half = 0; half < 2; ++half, dst += kPwHalf) {
+                                        int i = sink_rows >> 5;             // 16, 32, 64: 0, 1, 2
+                                        tma_load_3d(dst, &part[i], full, half * 64, kvh, sink_page >= 0 ? sink_page * p.block_size : -kPwKeys);
+                                        for (int r = sink_rows; r < kPwKeys; r *= 2, ++i)
+                                            tma_load_3d(dst + r * 128, &part[i], full, half * 64, kvh, from + r);
+                                    }
+                                }
+                            };
                             float v_ref = 0.f;                              // e4m3: V scale that O is expressed in, 0 = none yet
                             // order K0, K1, V0, K2, V1, ...: K of the next tile is needed before V of this one.  e4m3: K0, V0, K1,
                             // V1, ...: V has the conversion in front of it
@@ -403,13 +446,15 @@ __global__ void __launch_bounds__(PwCfg<FP8>::threads, 1) prefill_window_kernel(
                                     }
                                     // the copy first; the tile's entry is written while it runs and released by the arrival below,
                                     // without which the barrier cannot complete
-                                    const uint32_t dst = base + C::k + s * C::k_bytes;
-                                    tma_load_3d(dst, &map_k, bar(PW_K_FULL, s), 0, kvh, slot);
-                                    if constexpr (!FP8) tma_load_3d(dst + kPwHalf, &map_k, bar(PW_K_FULL, s), 64, kvh, slot);
+                                    load(base + C::k + s * C::k_bytes, &map_k, part_of(parts, false), bar(PW_K_FULL, s), j, slot);
                                     volatile int* t = s_ring + (kc % kPwRing) * PT_INTS;
                                     t[PT_KEY0] = key0;
                                     t[PT_CUT] = key0 + kPwKeys - 1 > pos_lo || (windowed && key0 <= pos_hi - p.window && key0 + kPwKeys > sinks);
                                     t[PT_SINK_END] = sinks - key0;
+                                    if (!FP8 && x0 + j == 0 && sink_rows > 0) {
+                                        t[PT_CUT] = 2;
+                                        t[PT_SINK_END] = sinks;
+                                    }
                                     t[PT_BEGIN] = first_key - key0;
                                     t[PT_END] = pos_hi + 1 - key0;
                                     if constexpr (FP8) {
@@ -440,8 +485,7 @@ __global__ void __launch_bounds__(PwCfg<FP8>::threads, 1) prefill_window_kernel(
                                         const uint32_t full = bar(FP8 ? PW_RAW_FULL : PW_V_FULL, s);
                                         const uint32_t dst = FP8 ? base + C::raw + s * kPwRaw : base + C::v + s * kPwTile;
                                         mbar_expect_tx(full, C::k_bytes);
-                                        tma_load_3d(dst, &map_v, full, 0, kvh, v_slot);
-                                        if constexpr (!FP8) tma_load_3d(dst + kPwHalf, &map_v, full, 64, kvh, v_slot);
+                                        load(dst, &map_v, part_of(parts, true), full, j - lag, v_slot);
                                         ++vc;
                                     } else ok = false;
                                 }
@@ -723,12 +767,13 @@ __global__ void __launch_bounds__(PwCfg<FP8>::threads, 1) prefill_window_kernel(
                 // keys behind a row's own position, or in front of its window and behind the sinks: -infinity
                 const int tile_tok = ie[PI_TOK0] + g * p.tokens;   // first token of the query tile
                 const int pos = ie[PI_SHIFT] + min(tile_tok + r / p.group, min(ie[PI_LQ], tile_tok + p.tokens) - 1);
+                const int sinks = !FP8 && head.x == 2 ? p.sinks : p.sinks - int(head.y);      // from the tile's first row on
                 const int start = ie[PI_WINDOWED] ? pos - p.window + 1 : -0x40000000;
                 auto low_bits = [](int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; };
 #pragma unroll
                 for (int w = 0; w < 4; ++w) {
                     const int k0 = int(head.y) + w * 32;
-                    const uint32_t seen = low_bits(pos + 1 - k0) & (~low_bits(start - k0) | low_bits(p.sinks - k0));
+                    const uint32_t seen = low_bits(pos + 1 - k0) & (~low_bits(start - k0) | low_bits(sinks - w * 32));
 #pragma unroll
                     for (int i = 0; i < 32; ++i)
                         if (!(seen & (1u << i))) sv[w * 32 + i] = 0xff800000u;
@@ -1016,7 +1061,7 @@ static int prefill_splits(const PwDevice& d, int64_t blocks, int64_t empty, int6
 }
 
 template <bool FP8>
-static int launch_prefill_window(PwParams& p, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, int64_t total_q,
+static int launch_prefill_window(PwParams& p, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const PwParts<FP8>& parts, int64_t total_q,
                                  int max_q, int max_k, int window, int batch, cudaStream_t st) {
     const PwDevice* d = nullptr;
     const int rc = prefill_device<FP8>(&d);
@@ -1028,7 +1073,7 @@ static int launch_prefill_window(PwParams& p, const CUtensorMap& mq, const CUten
     cudaLaunchAttribute attr;
     const cudaLaunchConfig_t cfg = prefill_config(dim3(unsigned(row_blocks), p.n_kv_heads * p.splits, batch), PwCfg<FP8>::threads,
                                                   PwCfg<FP8>::total + 1024, p.splits, st, &attr);
-    IB_CUDA(cudaLaunchKernelEx(&cfg, prefill_window_kernel<FP8>, PwParams(p), mq, mk, mv));
+    IB_CUDA(cudaLaunchKernelEx(&cfg, prefill_window_kernel<FP8>, PwParams(p), mq, mk, mv, parts));
     return check_launch();
 }
 
@@ -1070,9 +1115,14 @@ static int paged_prefill_window(const infer_kv_pool_t* pool, void* out, const vo
                            uint32_t(p.group), uint32_t(p.tokens));
     if (rc != INFER_OK) return rc;
     if (pool->dtype == INFER_KV_E4M3)
-        return launch_prefill_window<true>(p, mq, pool->maps[3].k, pool->maps[3].v, total_q, max_seqlen_q, max_seqlen_k, window,
-                                           batch, st);
-    return launch_prefill_window<false>(p, mq, pool->maps[3].k, pool->maps[3].v, total_q, max_seqlen_q, max_seqlen_k, window,
+        return launch_prefill_window<true>(p, mq, pool->maps[3].k, pool->maps[3].v, PwParts<true>{}, total_q, max_seqlen_q,
+                                           max_seqlen_k, window, batch, st);
+    PwParts<false> parts;
+    for (int i = 0; i < kPwParts; ++i) {
+        parts.k[i] = pool->maps[i].k;
+        parts.v[i] = pool->maps[i].v;
+    }
+    return launch_prefill_window<false>(p, mq, pool->maps[3].k, pool->maps[3].v, parts, total_q, max_seqlen_q, max_seqlen_k, window,
                                            batch, st);
 }
 

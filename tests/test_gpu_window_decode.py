@@ -75,7 +75,7 @@ def test_edges(kind, hkv, window, sinks):
 @pytest.mark.parametrize("kind", ["bf16", "e4m3"])
 @pytest.mark.parametrize("group", [1, 2, 3, 5, 6, 7, 8])
 def test_groups(kind, group):
-    c = _case(kind, [900, 33, 0, 1500], 3 * group, 3, group)
+    c = _case(kind, [900, 33, 0, 1500], 5 * group, 5, group)
     out = torch.full_like(c["q"], 7.0)
     got = _run(c, 300, 5, out=out)
     _check(c, got, 300, 5)

@@ -79,6 +79,26 @@ def test_edges(kind, hq, hkv, window, sinks):
     _check(c, _run(c, window, sinks), window, sinks)
 
 
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("sinks", [1, 15, 16, 17, 32, 33, 63, 64, 65])
+@pytest.mark.parametrize("window", [40, 128, 300])
+def test_sinks_in_front_of_the_window(kind, sinks, window):
+    """The window's first tile with more, as many and fewer rows in front of the window than there are sinks; the sinks' page
+    also one that lies outside of the pool: rows of zeros."""
+    chunks = [(window + 127 + x + 2, 2) for x in (0, 1, 15, 16, 17, 31, 32, 33, 63, 64, 65, 100, 126, 127, 128, 144, 300)]
+    c = _case(kind, chunks + [(1500, 600), (900, 140)], 6, 2, sinks, poison=(window, sinks))
+    _check(c, _run(c, window, sinks), window, sinks)
+    c = _case(kind, [(1000, 3), (1040, 70)], 6, 2, sinks)
+    for b, outside in ((0, -1), (1, c["k"].shape[0])):
+        c["bt"][b, 0] = outside
+        c["tables"][b][0] = c["k"].shape[0]
+    got = _run(c, window, sinks)
+    for x in "kv":                                       # what the kernel has to take it for: one more page, of zeros
+        c[x] = torch.cat([c[x], torch.zeros_like(c[x][:1])])
+        c[x + "s"] = None if c[x + "s"] is None else torch.cat([c[x + "s"], torch.ones_like(c[x + "s"][:1])])
+    _check(c, got, window, sinks)
+
+
 @pytest.mark.parametrize("group", [1, 2, 3, 4, 5, 6, 7, 8, 16, 128])
 @pytest.mark.parametrize("kind", ["bf16", "e4m3"])
 def test_groups(kind, group):
@@ -122,6 +142,17 @@ def test_split_over_the_keys(kind, window, sinks, hq, hkv):
         got = _run(c, window, sinks)
         _check(c, got, window, sinks)
         assert bits_equal(_run(c, window, sinks), got)
+
+
+@pytest.mark.parametrize("batch,hkv", [(14, 5), (8, 5), (6, 5), (5, 5), (3, 7), (2, 7), (11, 1), (1, 7), (1, 1)])
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+def test_every_number_of_parts(kind, batch, hkv):
+    """From 70 row blocks down to one: parts of 2, 3, 4, 5 and more thread blocks, up to 16, over 20 to 24 key tiles."""
+    c = _case(kind, [(2500 + 40 * b, 3 + b) for b in range(batch)], 2 * hkv, hkv, batch)
+    window = None if kind == "e4m3" else 10 ** 6
+    got = _run(c, window)
+    _check(c, got, window)
+    assert bits_equal(_run(c, window), got)
 
 
 @pytest.mark.parametrize("kind", ["bf16", "e4m3"])
