@@ -8,8 +8,8 @@
 // Bound by HBM: per row and head 128 elements read and 256 bytes written, for K and for V.  Eight lanes take one (row,
 // head), sixteen elements per lane: 32-byte stores (and, for bf16, loads), which need the addresses at 32 bytes; two
 // 16-byte ones otherwise.  32768 rows of 8 heads out of an e4m3 pool: 34.9 us with a cold L2, 5.77 TB/s of the bytes that
-// have to move (32.8 in a graph); 40.5 us with 16-byte stores, 43 us with eight elements per lane and four rows of sixteen lanes each in flight.  Two to
-// four units per lane gain nothing (34.6-35.6 us) and cost a small call a microsecond.
+// have to move (32.8-34.6 in a graph); 40.5 us with 16-byte stores, 43 us with eight elements per lane and four rows of
+// sixteen lanes each in flight.  Two to four units per lane gain nothing (34.6-35.6 us) and cost a small call a microsecond.
 #include "common.cuh"
 
 namespace ib {
