@@ -14,6 +14,8 @@
 #include <mutex>
 #include <utility>
 
+#include <algorithm>
+
 #include "decode_common.cuh"
 
 namespace ib {
@@ -32,9 +34,17 @@ constexpr int kMergeSlotFloats = 36 * 32;         // 32 accumulators + up to two
 // row r belongs to query head hg * rows + r.
 __device__ __forceinline__ void merge_if_last(const DecodeParams& p, const int* s_tp, int ng, const Segment& sg,
                                               int chunk, int rows, volatile int* s_flag) {
-    // first real tile of the (b, hg) in the padded numbering; the CTAs c0..c1 hold its real tiles
-    const int first = ng * s_tp[sg.b] + sg.hg * (sg.ntiles + p.seg_overhead) + p.seg_overhead;
-    const int c0 = first / chunk, c1 = (first + sg.ntiles - 1) / chunk;
+    // the CTAs c0..c1 hold the real tiles of the (b, hg)
+    int c0, c1;
+    if (chunk == 0) {                            // equal parts (see equal_part)
+        c0 = int(blockIdx.x) / p.parts * p.parts;
+        c1 = c0 + (sg.ntiles - 1) / ((sg.ntiles + p.parts - 1) / p.parts);
+    } else {
+        // its first real tile in the padded numbering
+        const int first = ng * s_tp[sg.b] + sg.hg * (sg.ntiles + p.seg_overhead) + p.seg_overhead;
+        c0 = first / chunk;
+        c1 = (first + sg.ntiles - 1) / chunk;
+    }
     asm volatile("bar.sync 1, 256;" ::: "memory");          // every partial store of this CTA is ordered before ...
     if (threadIdx.x == 0) {
         __threadfence();                                     // ... this fence, which is cumulative: they are visible before the ticket is
@@ -162,17 +172,28 @@ __global__ void __launch_bounds__(kTmaThreads, 1) decode_tma_kernel(DecodeParams
     // launches never share an SM - each takes nearly all of its shared memory - so nothing is lost.)
     if (p.new_k != nullptr) pdl_wait();
     uint8_t* s_rem = smem + TmaSmem::rem;
-    build_tile_prefix<WINDOW>(p.context_lens, p.batch, TT, s_tp, s_scan, s_rem, p.seg_overhead, p.window,
-                              p.sinks);                                    // ends with __syncthreads
+    const int ng = p.n_kv_heads / HPC;
+    const bool equal = WINDOW && p.parts > 0;
+    Segment part = {};
+    if (equal) {
+        part = equal_part(p, ng, TT);
+        __syncthreads();
+    } else {
+        build_tile_prefix<WINDOW>(p.context_lens, p.batch, TT, s_tp, s_scan, s_rem, p.seg_overhead, p.window,
+                                  p.sinks);                                // ends with __syncthreads
+    }
     // Everything above only reads step metadata; the pools and q may still be written by the
     // kernel in front of this one (the append) when this kernel was launched programmatically.
     pdl_launch_dependents();
     pdl_wait();
 
-    const int ng = p.n_kv_heads / HPC;
-    const int total = ng * s_tp[p.batch];
-    const int chunk = max(1, (total + int(gridDim.x) - 1) / int(gridDim.x));
-    const int lo = min(total, int(blockIdx.x) * chunk), hi = min(total, lo + chunk);
+    int lo = 0, hi = part.span, chunk = 0;
+    if (!equal) {
+        const int total = ng * s_tp[p.batch];
+        chunk = max(1, (total + int(gridDim.x) - 1) / int(gridDim.x));
+        lo = min(total, int(blockIdx.x) * chunk);
+        hi = min(total, lo + chunk);
+    }
 
     if (warp == kConsumerWarps) {
         // ------------------------------------------------------------ producer
@@ -182,7 +203,7 @@ __global__ void __launch_bounds__(kTmaThreads, 1) decode_tma_kernel(DecodeParams
         uint32_t it = 0;
         bool ok = true;
         for (int g = lo; g < hi && ok;) {
-            const Segment sg = locate_segment(s_tp, p.batch, ng, g, hi, p.seg_overhead);
+            const Segment sg = equal ? part : locate_segment(s_tp, p.batch, ng, g, hi, p.seg_overhead);
             const int32_t* table = p.block_tables + int64_t(sg.b) * p.bt_stride;
             int ctx = 0;
             WindowTiles win;
@@ -261,7 +282,7 @@ __global__ void __launch_bounds__(kTmaThreads, 1) decode_tma_kernel(DecodeParams
     // A wait that runs out only clears `ok`: the warp keeps walking the same tiles and
     // barriers as its siblings (without computing) so that no named barrier is left short.
     for (int g = lo; g < hi;) {
-        const Segment sg = locate_segment(s_tp, p.batch, ng, g, hi, p.seg_overhead);
+        const Segment sg = equal ? part : locate_segment(s_tp, p.batch, ng, g, hi, p.seg_overhead);
         if (sg.t0 == sg.t1) {                      // only padding of this (b, hg) lies in the range
             g += sg.span;
             continue;
@@ -528,14 +549,26 @@ __global__ void __launch_bounds__(kTmaThreads, 1) decode_tma_fp8_kernel(DecodePa
         fence_proxy_async();
     }
     uint8_t* s_rem = smem + L::rem;
-    build_tile_prefix<WINDOW>(p.context_lens, p.batch, TT, s_tp, s_scan, s_rem, p.seg_overhead, p.window, p.sinks);
+    const int ng = p.n_kv_heads / HPC;
+    const bool equal = WINDOW && p.parts > 0;
+    Segment part = {};
+    if (equal) {
+        part = equal_part(p, ng, TT);
+        __syncthreads();
+    } else {
+        build_tile_prefix<WINDOW>(p.context_lens, p.batch, TT, s_tp, s_scan, s_rem, p.seg_overhead, p.window,
+                                  p.sinks);                                // ends with __syncthreads
+    }
     pdl_launch_dependents();
     pdl_wait();
 
-    const int ng = p.n_kv_heads / HPC;
-    const int total = ng * s_tp[p.batch];
-    const int chunk = max(1, (total + int(gridDim.x) - 1) / int(gridDim.x));
-    const int lo = min(total, int(blockIdx.x) * chunk), hi = min(total, lo + chunk);
+    int lo = 0, hi = part.span, chunk = 0;
+    if (!equal) {
+        const int total = ng * s_tp[p.batch];
+        chunk = max(1, (total + int(gridDim.x) - 1) / int(gridDim.x));
+        lo = min(total, int(blockIdx.x) * chunk);
+        hi = min(total, lo + chunk);
+    }
 
     if (warp == W) {
         // ------------------------------------------------------------ producer
@@ -545,7 +578,7 @@ __global__ void __launch_bounds__(kTmaThreads, 1) decode_tma_fp8_kernel(DecodePa
         uint32_t it = 0;
         bool ok = true;
         for (int g = lo; g < hi && ok;) {
-            const Segment sg = locate_segment(s_tp, p.batch, ng, g, hi, p.seg_overhead);
+            const Segment sg = equal ? part : locate_segment(s_tp, p.batch, ng, g, hi, p.seg_overhead);
             const int32_t* table = p.block_tables + int64_t(sg.b) * p.bt_stride;
             int ctx = 0;
             WindowTiles win;
@@ -632,7 +665,7 @@ __global__ void __launch_bounds__(kTmaThreads, 1) decode_tma_fp8_kernel(DecodePa
     bool ok = true;
 
     for (int g = lo; g < hi;) {
-        const Segment sg = locate_segment(s_tp, p.batch, ng, g, hi, p.seg_overhead);
+        const Segment sg = equal ? part : locate_segment(s_tp, p.batch, ng, g, hi, p.seg_overhead);
         if (sg.t0 == sg.t1) {                      // only padding of this (b, hg) lies in the range
             g += sg.span;
             continue;
@@ -867,6 +900,7 @@ __global__ void __launch_bounds__(kTmaThreads, 1) decode_tma_fp8_kernel(DecodePa
 struct DecodeConfig {
     int hpc;          // kv heads per tile
     int grid;
+    int parts = 0;    // windowed: CTAs per (sequence, head group), 0 = equal ranges of all tiles
     int rows;         // partial rows per scratch slot
 };
 
@@ -973,6 +1007,40 @@ struct Window {
     int window = 0, sinks = 0;
 };
 
+// A windowed call whose sequences times kv heads fit into the grid gives each of them CTAs of its own (equal_part), as long as
+// a CTA gets no more than twelve tiles of the longest one the window allows (lengths far apart are better off with equal
+// ranges).  How many: an estimate in us, 1.3 a tile, 1.0 for a merge and 0.24 for each of its parts; a lone part is charged for
+// the tokens it sees.  Measured in a graph, us, ranges -> parts: bf16, 32 / 8 heads, 9 sequences, a window of 256 11.0 -> 8.2;
+// 16 / 8 heads, one sequence, a window of 100 7.8 -> 6.8, of 1000 8.8 -> 8.9 (a part per tile; two tiles 9.9, three 10.5), of
+// 5000 12.0 -> 11.6; e4m3, 32 / 4 heads, one sequence, a window of 256 14.9 -> 7.4, of 5000 55 -> 11.0; 32 / 8 heads, 18
+// sequences, a window of 1000 14.2 -> 10.6.
+// e4m3 tiles of one head then, with parts as with ranges: fewer and smaller partials, more CTAs (18 sequences, a window of 5000,
+// ranges, 40.2 -> 34.0); with more sequences tiles of four heads are faster (32 of them, a window of 1000, 21.3 against 25.7).
+static void window_config(DecodeConfig& c, const infer_kv_pool* pool, int batch, int group, int64_t bt_stride, const Window& win) {
+    constexpr int kMostTiles = 12;
+    const bool fp8 = pool->dtype == INFER_KV_E4M3;
+    const int64_t segments = int64_t(batch) * pool->n_kv_heads;
+    if (segments > c.grid) return;
+    c.hpc = 1;
+    c.rows = group;
+    const int64_t tile = fp8 ? kFp8TileTokens : kTileBytes / 256;
+    int64_t tiles = (int64_t(win.window) + 2 * tile - 2) / tile + (int64_t(win.sinks) + tile - 1) / tile;
+    tiles = std::min(tiles, (bt_stride * pool->block_size + tile - 1) / tile);
+    const int64_t most = std::min(c.grid / segments, tiles);
+    double best = 0.;
+    for (int64_t k = 1; k <= most; ++k) {
+        const int64_t each = (tiles + k - 1) / k, used = (tiles + each - 1) / each;
+        if (each > kMostTiles) continue;
+        const double t = used > 1 ? 1.3 * double(each) + 1.0 + 0.24 * double(used)
+                                  : 1.3 * std::min(double(tiles), (double(win.window) + win.sinks) / double(tile) + 1.);
+        if (c.parts == 0 || t < best) {
+            c.parts = int(k);
+            best = t;
+        }
+    }
+    if (c.parts > 0) c.grid = int(segments) * c.parts;
+}
+
 static int paged_decode(const infer_kv_pool_t* pool, void* out, const void* q, const int32_t* context_lens,
                         const int32_t* block_tables, int64_t bt_stride, int batch, int n_q_heads, float softmax_scale,
                         void* workspace, size_t workspace_bytes, cudaStream_t st, int force_hpc, uint32_t wait_limit,
@@ -991,7 +1059,8 @@ static int paged_decode(const infer_kv_pool_t* pool, void* out, const void* q, c
     if (group > kMaxGroup) return INFER_ERR_GEOMETRY;
     if (!aligned16(out) || !aligned16(q)) return INFER_ERR_ALIGN;
     if (batch == 0) return INFER_OK;
-    const DecodeConfig cfg = decode_config(pool, n_q_heads, workspace_bytes, force_hpc);
+    DecodeConfig cfg = decode_config(pool, n_q_heads, workspace_bytes, force_hpc);
+    if (win.window > 0) window_config(cfg, pool, batch, group, bt_stride, win);
     const DecodeLayout lay = decode_layout(cfg.grid, cfg.rows);
     if (!workspace || !aligned16(workspace) || workspace_bytes < lay.total) return INFER_ERR_WORKSPACE;
 
@@ -1015,6 +1084,7 @@ static int paged_decode(const infer_kv_pool_t* pool, void* out, const void* q, c
     p.wait_limit = wait_limit;
     p.stall_producer = stall_producer;
     p.seg_overhead = kSegOverheadTiles;
+    p.parts = cfg.parts;
     p.window = win.window;
     p.sinks = win.sinks;
     p.new_k = static_cast<const __nv_bfloat16*>(rows.k);

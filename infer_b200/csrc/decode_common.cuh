@@ -46,6 +46,7 @@ struct DecodeParams {
     float scale_log2; // softmax_scale * log2(e)
     uint32_t wait_limit;   // polls before a barrier wait gives up
     int stall_producer;    // self-test only: the producer arms no copy, so every wait runs out
+    int parts;             // windowed kernels: CTAs per (sequence, head group) when every one has its own, else 0
     int seg_overhead;      // what starting and finishing a (sequence, head group) costs a CTA, in tiles (see below)
     int window, sinks;     // windowed kernels only: the last `window` keys and the first `sinks` ones are visible
     // fused append (bf16 pools): the step's new rows [batch][n_kv_heads][128], row b going to position
@@ -164,6 +165,22 @@ __device__ __forceinline__ Segment locate_segment(const int* s_tp, int batch, in
     s.ntiles = padded - seg_overhead;
     s.t0 = max(v0 - seg_overhead, 0);
     s.t1 = max(v1 - seg_overhead, 0);
+    return s;
+}
+
+// The part of this CTA when every (sequence, head group) has p.parts CTAs of its own, with as many tiles each: no numbering
+// of all tiles, nothing carried from one sequence to the next.  span = 0: nothing to do.
+__device__ __forceinline__ Segment equal_part(const DecodeParams& p, int ng, int tile_tokens) {
+    const int seg = int(blockIdx.x) / p.parts, i = int(blockIdx.x) - seg * p.parts;
+    Segment s;
+    s.b = seg / ng;
+    s.hg = seg - s.b * ng;
+    const int len = p.context_lens[s.b];
+    s.ntiles = len > 0 ? window_tiles(len, tile_tokens, p.window, p.sinks).count : 0;
+    const int each = (s.ntiles + p.parts - 1) / p.parts;
+    s.t0 = min(s.ntiles, i * each);
+    s.t1 = min(s.ntiles, s.t0 + each);
+    s.span = s.t0 < s.t1;
     return s;
 }
 
