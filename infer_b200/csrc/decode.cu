@@ -176,7 +176,7 @@ __global__ void __launch_bounds__(kTmaThreads, 1) decode_tma_kernel(DecodeParams
     const bool equal = WINDOW && p.parts > 0;
     Segment part = {};
     if (equal) {
-        part = equal_part(p, ng, TT);
+        part = equal_part(p, ng, TT, blockIdx.x);      // the first one's length is under way during the set-up
         __syncthreads();
     } else {
         build_tile_prefix<WINDOW>(p.context_lens, p.batch, TT, s_tp, s_scan, s_rem, p.seg_overhead, p.window,
@@ -187,7 +187,7 @@ __global__ void __launch_bounds__(kTmaThreads, 1) decode_tma_kernel(DecodeParams
     pdl_launch_dependents();
     pdl_wait();
 
-    int lo = 0, hi = part.span, chunk = 0;
+    int lo = blockIdx.x, hi = p.batch * ng * p.parts, chunk = 0;      // equal parts
     if (!equal) {
         const int total = ng * s_tp[p.batch];
         chunk = max(1, (total + int(gridDim.x) - 1) / int(gridDim.x));
@@ -203,7 +203,7 @@ __global__ void __launch_bounds__(kTmaThreads, 1) decode_tma_kernel(DecodeParams
         uint32_t it = 0;
         bool ok = true;
         for (int g = lo; g < hi && ok;) {
-            const Segment sg = equal ? part : locate_segment(s_tp, p.batch, ng, g, hi, p.seg_overhead);
+            const Segment sg = !equal ? locate_segment(s_tp, p.batch, ng, g, hi, p.seg_overhead) : g == lo ? part : equal_part(p, ng, TT, g);
             const int32_t* table = p.block_tables + int64_t(sg.b) * p.bt_stride;
             int ctx = 0;
             WindowTiles win;
@@ -282,7 +282,7 @@ __global__ void __launch_bounds__(kTmaThreads, 1) decode_tma_kernel(DecodeParams
     // A wait that runs out only clears `ok`: the warp keeps walking the same tiles and
     // barriers as its siblings (without computing) so that no named barrier is left short.
     for (int g = lo; g < hi;) {
-        const Segment sg = equal ? part : locate_segment(s_tp, p.batch, ng, g, hi, p.seg_overhead);
+        const Segment sg = !equal ? locate_segment(s_tp, p.batch, ng, g, hi, p.seg_overhead) : g == lo ? part : equal_part(p, ng, TT, g);
         if (sg.t0 == sg.t1) {                      // only padding of this (b, hg) lies in the range
             g += sg.span;
             continue;
@@ -553,7 +553,7 @@ __global__ void __launch_bounds__(kTmaThreads, 1) decode_tma_fp8_kernel(DecodePa
     const bool equal = WINDOW && p.parts > 0;
     Segment part = {};
     if (equal) {
-        part = equal_part(p, ng, TT);
+        part = equal_part(p, ng, TT, blockIdx.x);      // the first one's length is under way during the set-up
         __syncthreads();
     } else {
         build_tile_prefix<WINDOW>(p.context_lens, p.batch, TT, s_tp, s_scan, s_rem, p.seg_overhead, p.window,
@@ -562,7 +562,7 @@ __global__ void __launch_bounds__(kTmaThreads, 1) decode_tma_fp8_kernel(DecodePa
     pdl_launch_dependents();
     pdl_wait();
 
-    int lo = 0, hi = part.span, chunk = 0;
+    int lo = blockIdx.x, hi = p.batch * ng * p.parts, chunk = 0;      // equal parts
     if (!equal) {
         const int total = ng * s_tp[p.batch];
         chunk = max(1, (total + int(gridDim.x) - 1) / int(gridDim.x));
@@ -578,7 +578,7 @@ __global__ void __launch_bounds__(kTmaThreads, 1) decode_tma_fp8_kernel(DecodePa
         uint32_t it = 0;
         bool ok = true;
         for (int g = lo; g < hi && ok;) {
-            const Segment sg = equal ? part : locate_segment(s_tp, p.batch, ng, g, hi, p.seg_overhead);
+            const Segment sg = !equal ? locate_segment(s_tp, p.batch, ng, g, hi, p.seg_overhead) : g == lo ? part : equal_part(p, ng, TT, g);
             const int32_t* table = p.block_tables + int64_t(sg.b) * p.bt_stride;
             int ctx = 0;
             WindowTiles win;
@@ -665,7 +665,7 @@ __global__ void __launch_bounds__(kTmaThreads, 1) decode_tma_fp8_kernel(DecodePa
     bool ok = true;
 
     for (int g = lo; g < hi;) {
-        const Segment sg = equal ? part : locate_segment(s_tp, p.batch, ng, g, hi, p.seg_overhead);
+        const Segment sg = !equal ? locate_segment(s_tp, p.batch, ng, g, hi, p.seg_overhead) : g == lo ? part : equal_part(p, ng, TT, g);
         if (sg.t0 == sg.t1) {                      // only padding of this (b, hg) lies in the range
             g += sg.span;
             continue;
@@ -1007,38 +1007,51 @@ struct Window {
     int window = 0, sinks = 0;
 };
 
-// A windowed call whose sequences times kv heads fit into the grid gives each of them CTAs of its own (equal_part), as long as
-// a CTA gets no more than twelve tiles of the longest one the window allows (lengths far apart are better off with equal
-// ranges).  How many: an estimate in us, 1.3 a tile, 1.0 for a merge and 0.24 for each of its parts; a lone part is charged for
-// the tokens it sees.  Measured in a graph, us, ranges -> parts: bf16, 32 / 8 heads, 9 sequences, a window of 256 11.0 -> 8.2;
-// 16 / 8 heads, one sequence, a window of 100 7.8 -> 6.8, of 1000 8.8 -> 8.9 (a part per tile; two tiles 9.9, three 10.5), of
-// 5000 12.0 -> 11.6; e4m3, 32 / 4 heads, one sequence, a window of 256 14.9 -> 7.4, of 5000 55 -> 11.0; 32 / 8 heads, 18
-// sequences, a window of 1000 14.2 -> 10.6.
-// e4m3 tiles of one head then, with parts as with ranges: fewer and smaller partials, more CTAs (18 sequences, a window of 5000,
-// ranges, 40.2 -> 34.0); with more sequences tiles of four heads are faster (32 of them, a window of 1000, 21.3 against 25.7).
+// How a windowed call hands out its tiles, and in an e4m3 pool the heads of one: equal parts (equal_part: CTAs of their own for
+// each (sequence, head group), or whole ones in turn where there are more than CTAs) or equal ranges of all tiles, whichever an
+// estimate in us says is faster when every sequence fills the window.  Equal parts only where a CTA's part has no more than
+// 18 tiles: lengths far apart are better off with ranges.  Estimates, fitted to calls of 1 to 256 sequences: a tile 1.3; a whole
+// (sequence, head group) 3.6 beside (e4m3 4.6), a merge 1.0 and 0.24 per part; ranges 1.1 a tile and 5.5 (e4m3 1.3 and 7) and 0.5
+// for every part that the longest is cut into.
+// Measured in a graph, us, ranges -> parts, bf16, 32 / 8 heads: 9 sequences, a window of 256 11.0 -> 8.2; 32 sequences, 128 18.6
+// -> 13.0, 1024 33.0 -> 31.5, 2048 50.8 (ranges; 51.4); 64 sequences, 256 30.1 -> 28.2, 1024 56.3 (ranges; 61).  One sequence, 16 /
+// 8 heads, 100 7.8 -> 6.8, 1000 8.8 -> 8.9 (a part per tile; two tiles 9.9, three 10.5), 5000 12.0 -> 11.6.
+// e4m3, 32 / 8 heads: 18 sequences, 1024 15.8 -> 11.8 (tiles of one head); 32, 512 16.6 -> 12.2 (of two); 64, 256 18.4 -> 12.1,
+// 1024 34.4 -> 28.0, 128, 512 37.6 -> 33.8 (of four).  Ranges: of one head where those fit into the grid (18 sequences, 5000,
+// 34.0 against 40.2: fewer and smaller partials), else of four (32 sequences, 1024, 21.3 against 25.7).
 static void window_config(DecodeConfig& c, const infer_kv_pool* pool, int batch, int group, int64_t bt_stride, const Window& win) {
-    constexpr int kMostTiles = 12;
+    constexpr int kMostTiles = 18;
     const bool fp8 = pool->dtype == INFER_KV_E4M3;
-    const int64_t segments = int64_t(batch) * pool->n_kv_heads;
-    if (segments > c.grid) return;
-    c.hpc = 1;
-    c.rows = group;
-    const int64_t tile = fp8 ? kFp8TileTokens : kTileBytes / 256;
-    int64_t tiles = (int64_t(win.window) + 2 * tile - 2) / tile + (int64_t(win.sinks) + tile - 1) / tile;
-    tiles = std::min(tiles, (bt_stride * pool->block_size + tile - 1) / tile);
-    const int64_t most = std::min(c.grid / segments, tiles);
-    double best = 0.;
-    for (int64_t k = 1; k <= most; ++k) {
-        const int64_t each = (tiles + k - 1) / k, used = (tiles + each - 1) / each;
-        if (each > kMostTiles) continue;
-        const double t = used > 1 ? 1.3 * double(each) + 1.0 + 0.24 * double(used)
-                                  : 1.3 * std::min(double(tiles), (double(win.window) + win.sinks) / double(tile) + 1.);
-        if (c.parts == 0 || t < best) {
-            c.parts = int(k);
-            best = t;
+    const int64_t keys = bt_stride * pool->block_size;
+    auto tiles_of = [&](int64_t tile) {          // of a (sequence, head group), at most
+        const int64_t n = (int64_t(win.window) + 2 * tile - 2) / tile + (int64_t(win.sinks) + tile - 1) / tile;
+        return std::min(n, (keys + tile - 1) / tile);
+    };
+    auto tile_tokens = [&](int hpc) { return int64_t(fp8 ? kFp8TileTokens / hpc : kTileBytes / 256); };
+    const int widest = fp8 && int64_t(batch) * pool->n_kv_heads <= c.grid ? 1 : c.hpc;
+    int64_t segments = int64_t(batch) * (pool->n_kv_heads / widest);
+    const int64_t longest = tiles_of(tile_tokens(widest)) + kSegOverheadTiles, chunk = (segments * longest + c.grid - 1) / c.grid;
+    double best = (fp8 ? 1.3 * double(chunk) + 7. : 1.1 * double(chunk) + 5.5) + 0.5 * double(longest) / double(chunk);
+    const int grid = c.grid;
+    c.hpc = widest;
+    for (int hpc = widest; hpc >= 1; hpc /= 2) {
+        segments = int64_t(batch) * (pool->n_kv_heads / hpc);
+        const int64_t tile = tile_tokens(hpc), tiles = tiles_of(tile), most = std::max<int64_t>(grid / segments, 1);
+        for (int64_t k = 1; k <= most && k <= tiles; ++k) {
+            const int64_t each = (tiles + k - 1) / k, used = (tiles + each - 1) / each;
+            if (each > kMostTiles) continue;
+            const double seen = used > 1 ? double(each) : std::min(double(tiles), (double(win.window) + win.sinks) / double(tile) + 1.);
+            const double t = double((segments + grid - 1) / grid) * ((fp8 ? 4.6 : 3.6) + 1.3 * seen) +
+                             (used > 1 ? 1.0 + 0.24 * double(used) : 0.);
+            if (t < best) {
+                best = t;
+                c.hpc = hpc;
+                c.parts = int(k);
+                c.grid = int(std::min<int64_t>(segments * k, grid));
+            }
         }
     }
-    if (c.parts > 0) c.grid = int(segments) * c.parts;
+    c.rows = c.hpc * group;
 }
 
 static int paged_decode(const infer_kv_pool_t* pool, void* out, const void* q, const int32_t* context_lens,

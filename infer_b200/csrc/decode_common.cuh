@@ -168,10 +168,11 @@ __device__ __forceinline__ Segment locate_segment(const int* s_tp, int batch, in
     return s;
 }
 
-// The part of this CTA when every (sequence, head group) has p.parts CTAs of its own, with as many tiles each: no numbering
-// of all tiles, nothing carried from one sequence to the next.  span = 0: nothing to do.
-__device__ __forceinline__ Segment equal_part(const DecodeParams& p, int ng, int tile_tokens) {
-    const int seg = int(blockIdx.x) / p.parts, i = int(blockIdx.x) - seg * p.parts;
+// Part g of the equal parts, p.parts for every (sequence, head group): no numbering of all tiles, and nothing is carried from
+// one sequence to the next.  CTA c takes the parts c, c + grid, ...; more than one only of whole (sequence, head group)s.
+// t0 == t1: nothing to do.
+__device__ __forceinline__ Segment equal_part(const DecodeParams& p, int ng, int tile_tokens, int g) {
+    const int seg = g / p.parts, i = g - seg * p.parts;
     Segment s;
     s.b = seg / ng;
     s.hg = seg - s.b * ng;
@@ -180,7 +181,7 @@ __device__ __forceinline__ Segment equal_part(const DecodeParams& p, int ng, int
     const int each = (s.ntiles + p.parts - 1) / p.parts;
     s.t0 = min(s.ntiles, i * each);
     s.t1 = min(s.ntiles, s.t0 + each);
-    s.span = s.t0 < s.t1;
+    s.span = gridDim.x;
     return s;
 }
 
