@@ -1011,9 +1011,9 @@ struct Window {
 // each (sequence, head group), or whole ones in turn where there are more than CTAs) or equal ranges of all tiles, whichever an
 // estimate in us says is faster when every sequence fills the window.  Equal parts only where a CTA's part has no more than
 // twelve tiles: lengths far apart are better off with ranges (e4m3, 64 sequences, a window of 1024, 18 tiles of four heads: all
-// full 28.0 against 33.6, one long and 63 of 40 keys 25.0 against 14.3; bf16, 18 sequences, ten tiles, 13.5 against 12.9).  Estimates, fitted to calls of 1 to 256 sequences: a tile 1.3; a whole
-// (sequence, head group) 3.6 beside (e4m3 4.6), a merge 1.0 and 0.24 per part; ranges 1.1 a tile and 5.5 (e4m3 1.3 and 7) and 0.5
-// for every part that the longest is cut into.
+// full 28.0 against 33.6, one long and 63 of 40 keys 25.0 against 14.3; bf16, 18 sequences, ten tiles, 13.5 against 12.9).
+// Estimates, fitted to calls of 1 to 256 sequences: a tile 1.3; a whole (sequence, head group) 3.6 beside (e4m3 4.6), a merge
+// 1.0 and 0.24 per part; ranges 1.1 a tile and 5.5 (e4m3 1.3 and 7) and 0.5 for every part that the longest is cut into.
 // Measured in a graph, us, ranges -> parts, bf16, 32 / 8 heads: 9 sequences, a window of 256 11.0 -> 8.2; 32 sequences, 128 18.6
 // -> 13.0, 1024 33.0 -> 31.5, 2048 50.8 (ranges; 51.4); 64 sequences, 256 30.1 -> 28.2, 1024 56.3 (ranges; 61).  One sequence, 16 /
 // 8 heads, 100 7.8 -> 6.8, 1000 8.8 -> 8.9 (a part per tile; two tiles 9.9, three 10.5), 5000 12.0 -> 11.6.

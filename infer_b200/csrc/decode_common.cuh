@@ -18,6 +18,8 @@
 // a partial then takes a ticket from the counter of that (b, hg) (indexed by the first CTA
 // of its span); the CTA that draws the last ticket merges slot 1 of the first CTA with slot
 // 0 of the following ones and writes the output rows.  No CTA waits for another.
+// Windowed calls may cut every (sequence, head group) into p.parts equal parts instead (equal_part): the segments of one then
+// are the consecutive CTAs' from a multiple of p.parts on, with the same slots and tickets.
 #pragma once
 
 #include "common.cuh"

@@ -56,9 +56,10 @@ constexpr int kPwHalf = 128 * 128;            // bytes of one [128 rows][64 elem
 constexpr int kPwTile = 2 * kPwHalf;          // 32 KiB: one Q, K or V tile of 16-bit elements
 constexpr int kPwRaw = 128 * 128;             // 16 KiB: one K or V tile of e4m3 bytes
 constexpr int kPwRing = 8;                    // entries of the tile ring: one lives from its K's load to its P V product, 7 tiles at most
-// A tile's entry: whether some row of the CTA sees only part of it (2: and its first rows are the sinks), its first key; e4m3: k scale, what O is multiplied by in
-// front of this tile (1 as a rule), what the V scale adds to the exponents of P, what takes it out of a row sum again, the V
-// scale that O is expressed in from there on; the rows that some query sees, [0, sink_end) and [begin, end).
+// A tile's entry: whether some row of the CTA sees only part of it (2: and its first rows are the sinks), its first key; e4m3: k
+// scale, what O is multiplied by in front of this tile (1 as a rule), what the V scale adds to the exponents of P, what takes it
+// out of a row sum again, the V scale that O is expressed in from there on; the rows that some query sees, [0, sink_end) and
+// [begin, end).
 enum PwTileEntry { PT_CUT, PT_KEY0, PT_K_SCALE, PT_O_FACTOR, PT_UP, PT_DOWN, PT_V_REF, PT_SINK_END = 8, PT_BEGIN, PT_END, PT_INTS = 16 };
 // a row block's entry in the ring of two: number of key tiles (-1: no more row blocks), whether the second query tile has
 // rows, first row of q, rows and first key position of the sequence, first token of the block, kv head, part, windowed
@@ -1061,8 +1062,8 @@ static int prefill_splits(const PwDevice& d, int64_t blocks, int64_t empty, int6
 }
 
 template <bool FP8>
-static int launch_prefill_window(PwParams& p, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const PwParts<FP8>& parts, int64_t total_q,
-                                 int max_q, int max_k, int window, int batch, cudaStream_t st) {
+static int launch_prefill_window(PwParams& p, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
+                                 const PwParts<FP8>& parts, int64_t total_q, int max_q, int max_k, int window, int batch, cudaStream_t st) {
     const PwDevice* d = nullptr;
     const int rc = prefill_device<FP8>(&d);
     if (rc != INFER_OK) return rc;

@@ -117,3 +117,22 @@ def test_load_refusals():
         ops.load_kvcache(k, k, slots, k_out=torch.zeros(3 * 256 + 4, dtype=torch.bfloat16, device="cuda")[4:].view(3, 2, 128))
     with pytest.raises(ValueError):
         ops.load_kvcache(k.view(torch.uint8)[..., :128].contiguous(), k.view(torch.uint8)[..., :128].contiguous(), slots)
+
+
+def test_pools_released_and_made_again():
+    """Handles that were given back are not used again, and pools of another type at the same addresses are others."""
+    cache = torch.randn(2, 2, 256, 2, 128, device="cuda").bfloat16()
+    slots = torch.tensor([3, 400, 3], dtype=torch.int32, device="cuda")
+    for _ in range(2):
+        k, v = ops.load_kvcache(cache[0], cache[1], slots)
+        assert bits_equal(k, cache[0].view(-1, 2, 128)[slots.long()]) and bits_equal(v, cache[1].view(-1, 2, 128)[slots.long()])
+        ops.release_pools()
+    half = cache.view(torch.uint8).view(2, 2, 512, 2, 128)           # the same memory as e4m3 pages of 512 rows
+    with pytest.raises(ValueError):
+        ops.load_kvcache(half[0], half[1], slots)
+    one = torch.ones(2, 2, device="cuda")
+    k, _ = ops.load_kvcache(half[0], half[1], slots, one, one)
+    want = half[0].view(torch.float8_e4m3fn).view(-1, 2, 128)[slots.long()].float().bfloat16()
+    assert torch.equal(k.float().nan_to_num(7.0), want.float().nan_to_num(7.0))
+    k, _ = ops.load_kvcache(cache[0], cache[1], slots)
+    assert bits_equal(k, cache[0].view(-1, 2, 128)[slots.long()])
