@@ -860,21 +860,41 @@ __global__ void __launch_bounds__(PwCfg<FP8>::threads, 1) prefill_window_kernel(
 #pragma unroll
             for (int c = 0; c < 4; ++c) tc_ld32(o_addr + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&v[c * 32]));
             tc_wait_ld();
-            if (live) {
-                __nv_bfloat16* dst = p.out + row * kHeadDim;
-                if (!any) {
+            if (!any) {
 #pragma unroll
-                    for (int i = 0; i < 128; ++i) v[i] = 0u;
-                }
-                auto two = [&](int i) { return pack_bf16(__uint_as_float(v[i]) * f, __uint_as_float(v[i + 1]) * f); };
+                for (int i = 0; i < 128; ++i) v[i] = 0u;
+            }
+            // two lanes write a row of either together, 64 bytes next to each other: a store touches 16 lines instead of 32 (16
+            // sequences of 2048 rows, a window of 1024: e4m3 354 -> 335 us, bf16 286 -> 281; ten rows 7.1 -> 7.4)
+            uint32_t w[64];
 #pragma unroll
-                for (int i = 0; i < 128; i += 16) {
-                    const Bytes32 w = {make_uint4(two(i), two(i + 2), two(i + 4), two(i + 6)),
-                                       make_uint4(two(i + 8), two(i + 10), two(i + 12), two(i + 14))};
-                    // a lane's row is 256 bytes away from its neighbour's: whole 32-byte sectors halve what the stores take
-                    if (p.out_at32) store32<true>(dst + i, w);
-                    else store32<false>(dst + i, w);
+            for (int i = 0; i < 64; ++i) w[i] = pack_bf16(__uint_as_float(v[2 * i]) * f, __uint_as_float(v[2 * i + 1]) * f);
+            const bool odd = lane & 1;
+            const int64_t at = live ? row : -1, other = __shfl_xor_sync(0xffffffffu, at, 1);
+            const int64_t row_even = odd ? other : at, row_odd = odd ? at : other;
+#pragma unroll
+            for (int c = 0; c < 64; c += 16) {                     // words c .. c + 7 are the even lane's to write, c + 8 .. the odd one's
+                uint32_t own[8], got[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    own[i] = odd ? w[c + 8 + i] : w[c + i];
+                    got[i] = __shfl_xor_sync(0xffffffffu, odd ? w[c + i] : w[c + 8 + i], 1);
                 }
+                auto put = [&](int64_t r, const uint32_t* x) {
+                    if (r < 0) return;
+                    __nv_bfloat16* dst = p.out + r * kHeadDim + 2 * c + (odd ? 16 : 0);
+                    const Bytes32 y = {make_uint4(x[0], x[1], x[2], x[3]), make_uint4(x[4], x[5], x[6], x[7])};
+                    if (p.out_at32) store32<true>(dst, y);
+                    else store32<false>(dst, y);
+                };
+                uint32_t first[8], second[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    first[i] = odd ? got[i] : own[i];              // of the even lane's row
+                    second[i] = odd ? own[i] : got[i];
+                }
+                put(row_even, first);
+                put(row_odd, second);
             }
             tc_fence_before();
         }
