@@ -865,7 +865,8 @@ __global__ void __launch_bounds__(PwCfg<FP8>::threads, 1) prefill_window_kernel(
                 for (int i = 0; i < 128; ++i) v[i] = 0u;
             }
             // two lanes write a row of either together, 64 bytes next to each other: a store touches 16 lines instead of 32 (16
-            // sequences of 2048 rows, a window of 1024: e4m3 354 -> 335 us, bf16 286 -> 281; ten rows 7.1 -> 7.4)
+            // sequences of 2048 rows, a window of 1024: e4m3 354 -> 335 us, bf16 286 -> 281; ten rows 7.1 -> 7.4; four
+            // lanes, 128 bytes, 346 and 283: the exchange costs more)
             uint32_t w[64];
 #pragma unroll
             for (int i = 0; i < 64; ++i) w[i] = pack_bf16(__uint_as_float(v[2 * i]) * f, __uint_as_float(v[2 * i + 1]) * f);
