@@ -210,14 +210,20 @@ INFER_API int infer_paged_prefill(const infer_kv_pool_t* pool, void* out, const 
  * effect).  The alignment of queries and keys is that of infer_paged_prefill; a query that sees no key (a sequence with
  * fewer keys than queries) gives zeros, rows of out that belong to no sequence are left alone, and block-table entries
  * of pages without a visible key are not read; a page id outside of the pool, or a key behind the table's columns, counts
- * as rows of zeros.  Values that no query of a sequence sees may be anything; a NaN or an infinity that only some of a
- * chunk's queries see may reach the others (0 times it is NaN).  Up to 128 query heads per kv head.  max_seqlen_q has to cover the longest
- * chunk; max_seqlen_k (the longest context) only guides over how many thread blocks few rows' keys are split.
+ * as rows of zeros.  A row of block_tables has bt_stride columns here; ..._columns takes their number on its own, for a
+ * table whose rows lie in wider ones: entries behind a row's columns are not read.  Values that no query of a sequence
+ * sees may be anything; a NaN or an infinity that only some of a chunk's queries see may reach the others (0 times it
+ * is NaN).  Up to 128 query heads per kv head.  max_seqlen_q has to cover the longest chunk; max_seqlen_k (the longest
+ * context) only guides over how many thread blocks few rows' keys are split.
  * softmax_scale: a positive finite number. */
 INFER_API int infer_paged_prefill_window(const infer_kv_pool_t* pool, void* out, const void* q, int64_t total_q,
                         const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, const int32_t* block_tables,
                         int64_t bt_stride, int batch, int max_seqlen_q, int max_seqlen_k, int n_q_heads,
                         float softmax_scale, int window, int sinks, void* stream);
+INFER_API int infer_paged_prefill_window_columns(const infer_kv_pool_t* pool, void* out, const void* q, int64_t total_q,
+                        const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, const int32_t* block_tables,
+                        int64_t bt_stride, int64_t bt_columns, int batch, int max_seqlen_q, int max_seqlen_k,
+                        int n_q_heads, float softmax_scale, int window, int sinks, void* stream);
 
 /* Dense causal attention.  Replaces flash_attn_prefill_impl
  * (src/operators/flashattn/flashattn.cu:269-328; schema src/bindings.cpp:9):

@@ -41,9 +41,9 @@ INFER_API int infer_selftest_paged_prefill(const infer_kv_pool_t* pool, void* ou
                                  void* stream, int kernel, uint32_t wait_limit, int stall_producer);
 INFER_API int infer_selftest_paged_prefill_window(const infer_kv_pool_t* pool, void* out, const void* q, int64_t total_q,
                                  const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k,
-                                 const int32_t* block_tables, int64_t bt_stride, int batch, int max_seqlen_q,
-                                 int max_seqlen_k, int n_q_heads, float softmax_scale, int window, int sinks,
-                                 void* stream, uint32_t wait_limit, int stall_producer);
+                                 const int32_t* block_tables, int64_t bt_stride, int64_t bt_columns, int batch,
+                                 int max_seqlen_q, int max_seqlen_k, int n_q_heads, float softmax_scale, int window,
+                                 int sinks, void* stream, uint32_t wait_limit, int stall_producer);
 INFER_API int infer_selftest_flash_attn_prefill(const void* q, const void* k, const void* v, void* o, int batch,
                                       int n_q_heads, int n_kv_heads, int seq_len, void* stream, int kernel);
 

@@ -43,6 +43,8 @@ SIGNATURES = {
     "infer_paged_prefill": (_i32, [_vp, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _f32, _vp]),
     "infer_paged_prefill_window": (_i32, [_vp, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _f32, _i32, _i32,
                                           _vp]),
+    "infer_paged_prefill_window_columns": (_i32, [_vp, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i32, _i32, _i32, _i32, _f32, _i32,
+                                                  _i32, _vp]),
     "infer_flash_attn_prefill": (_i32, [_vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _vp]),
     "infer_paged_decode_status": (_i32, [_vp, _vp]),
     "infer_prefill_status": (_i32, [_vp]),
@@ -72,8 +74,8 @@ SELFTEST_SIGNATURES = {
                                            _i32, _u32, _i32]),
     "infer_selftest_paged_prefill": (_i32, [_vp, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _f32, _vp,
                                             _i32, _u32, _i32]),
-    "infer_selftest_paged_prefill_window": (_i32, [_vp, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _f32, _i32,
-                                                   _i32, _vp, _u32, _i32]),
+    "infer_selftest_paged_prefill_window": (_i32, [_vp, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i32, _i32, _i32, _i32, _f32,
+                                                   _i32, _i32, _vp, _u32, _i32]),
     "infer_selftest_flash_attn_prefill": (_i32, [_vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _vp, _i32]),
 }
 

@@ -9,6 +9,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <algorithm>
 #include <climits>
 #include <stdexcept>
 #include <string>
@@ -29,7 +30,7 @@ struct Library {
     decltype(&infer_rotary_embed) rotary_embed = nullptr;
     decltype(&infer_paged_decode_window) decode_window = nullptr;
     decltype(&infer_paged_decode_append_window) decode_append_window = nullptr;
-    decltype(&infer_paged_prefill_window) prefill_window = nullptr;
+    decltype(&infer_paged_prefill_window_columns) prefill_window = nullptr;
     decltype(&infer_selftest_paged_prefill_window) prefill_window_test = nullptr;
     decltype(&infer_strerror) strerror = nullptr;
     decltype(&infer_last_cuda_error) last_cuda_error = nullptr;
@@ -52,7 +53,7 @@ void bind_library(const pybind11::dict& d) {
     bind_one(lib.rotary_embed, d, "infer_rotary_embed");
     bind_one(lib.decode_window, d, "infer_paged_decode_window");
     bind_one(lib.decode_append_window, d, "infer_paged_decode_append_window");
-    bind_one(lib.prefill_window, d, "infer_paged_prefill_window");
+    bind_one(lib.prefill_window, d, "infer_paged_prefill_window_columns");
     bind_one(lib.prefill_window_test, d, "infer_selftest_paged_prefill_window");
     bind_one(lib.strerror, d, "infer_strerror");
     bind_one(lib.last_cuda_error, d, "infer_last_cuda_error");
@@ -97,11 +98,12 @@ const T* vector(const char* what, const char* name, const Tensor& x, int64_t n, 
     return static_cast<const T*>(x.data_ptr());
 }
 
-// A table of int32 rows of contiguous entries on the device, one per sequence.
-void table_rows(const char* what, const Tensor& t, int64_t batch, int64_t device) {
+// A table of int32 rows of contiguous entries on the device, one per sequence; returns their pitch in entries.
+int64_t table_rows(const char* what, const Tensor& t, int64_t batch, int64_t device) {
     if (t.scalar_type() != at::kInt || !on(t, device)) refuse(what, "block_table must be an int32 CUDA tensor on cuda:" + std::to_string(device));
     if (t.dim() != 2 || t.size(0) < batch || t.stride(1) != 1)
         refuse(what, "block_table must have a row of contiguous entries per sequence");
+    return t.size(0) > 1 ? t.stride(0) : std::max<int64_t>(t.size(1), 1);     // torch may report any stride for a dimension of one
 }
 
 // window and sinks as the library takes them, 0 = no window
@@ -221,13 +223,13 @@ Tensor decode_window(uintptr_t pool, int64_t device, int64_t n_kv_heads, const T
     reachable("out", o);
     if (lens.scalar_type() != at::kInt || !on(lens, device) || lens.numel() != b || !lens.is_contiguous())
         refuse(what, "cache_seqlens must be an int32 CUDA tensor with a length per sequence on cuda:" + std::to_string(device));
-    table_rows(what, table, b, device);
+    const int64_t table_pitch = table_rows(what, table, b, device);
     if (ws.scalar_type() != at::kByte || !on(ws, device) || !ws.is_contiguous()) refuse(what, "workspace must be a contiguous uint8 CUDA tensor");
     Launch l(device);
     const auto* cl = static_cast<const int32_t*>(lens.data_ptr());
     const auto* bt = static_cast<const int32_t*>(table.data_ptr());
     if (!key) {
-        check(lib.decode_window(pool_at(pool), o.data_ptr(), q.data_ptr(), cl, bt, table.stride(0), int(b), int(q.size(-2)), float(scale),
+        check(lib.decode_window(pool_at(pool), o.data_ptr(), q.data_ptr(), cl, bt, table_pitch, int(b), int(q.size(-2)), float(scale),
                                 win, sink, ws.data_ptr(), size_t(ws.numel()), l.stream),
               what);
     } else {
@@ -243,7 +245,7 @@ Tensor decode_window(uintptr_t pool, int64_t device, int64_t n_kv_heads, const T
             pitch[i] = b > 1 ? t.stride(0) : n_kv_heads * 128;
         }
         check(lib.decode_append_window(pool_at(pool), o.data_ptr(), q.data_ptr(), key->data_ptr(), value->data_ptr(), pitch[0], pitch[1],
-                                       cl, bt, table.stride(0), int(b), int(q.size(-2)), float(scale), win, sink, ws.data_ptr(),
+                                       cl, bt, table_pitch, int(b), int(q.size(-2)), float(scale), win, sink, ws.data_ptr(),
                                        size_t(ws.numel()), l.stream),
               what);
     }
@@ -266,7 +268,7 @@ Tensor prefill_window(uintptr_t pool, int64_t device, const Tensor& q, const Ten
     const int64_t batch = cu_q.numel() - 1;
     if (batch < 0 || cu_k.numel() != batch + 1 || !cu_q.is_contiguous() || !cu_k.is_contiguous())
         refuse(what, "cu_seqlens_q and cu_seqlens_k must be contiguous, batch + 1 values each");
-    table_rows(what, table, batch, device);
+    const int64_t table_pitch = table_rows(what, table, batch, device);
     if (batch > INT_MAX || max_q > INT_MAX || max_k > INT_MAX || max_q < 0 || max_k < 0) check(INFER_ERR_GEOMETRY, what);
     Launch l(device);
     const auto* cq = static_cast<const int32_t*>(cu_q.data_ptr());
@@ -274,12 +276,12 @@ Tensor prefill_window(uintptr_t pool, int64_t device, const Tensor& q, const Ten
     const auto* bt = static_cast<const int32_t*>(table.data_ptr());
     const int hq = int(q.size(1));
     if (prefill_test.wait_limit || prefill_test.stall_producer)
-        check(lib.prefill_window_test(pool_at(pool), o.data_ptr(), q.data_ptr(), q.size(0), cq, ck, bt, table.stride(0), int(batch),
-                                      int(max_q), int(max_k), hq, float(scale), win, sink, l.stream, prefill_test.wait_limit,
+        check(lib.prefill_window_test(pool_at(pool), o.data_ptr(), q.data_ptr(), q.size(0), cq, ck, bt, table_pitch, table.size(1),
+                                      int(batch), int(max_q), int(max_k), hq, float(scale), win, sink, l.stream, prefill_test.wait_limit,
                                       prefill_test.stall_producer),
               what);
     else
-        check(lib.prefill_window(pool_at(pool), o.data_ptr(), q.data_ptr(), q.size(0), cq, ck, bt, table.stride(0), int(batch),
+        check(lib.prefill_window(pool_at(pool), o.data_ptr(), q.data_ptr(), q.size(0), cq, ck, bt, table_pitch, table.size(1), int(batch),
                                  int(max_q), int(max_k), hq, float(scale), win, sink, l.stream),
               what);
     return o;

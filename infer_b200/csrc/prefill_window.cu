@@ -126,7 +126,8 @@ struct PwParams {
     const int32_t* cu_q;
     const int32_t* cu_k;
     const int32_t* block_tables;
-    int64_t bt_stride;
+    int64_t bt_stride;       // entries from one row of the table to the next ...
+    int64_t bt_columns;      // ... of which these are the table's own; none behind them is read
     const float* k_scale;
     const float* v_scale;
     int n_q_heads, n_kv_heads, group;
@@ -400,7 +401,7 @@ __global__ void __launch_bounds__(PwCfg<FP8>::threads, 1) prefill_window_kernel(
                             const int32_t* table = p.block_tables + int64_t(b) * p.bt_stride;
                             auto page_at = [&](int key) {                   // -1: outside of the table or of the pool
                                 const int idx = key / p.block_size;
-                                const int page = idx < p.bt_stride ? table[idx] : -1;
+                                const int page = idx < p.bt_columns ? table[idx] : -1;
                                 return page >= 0 && page < p.num_blocks ? page : -1;
                             };
                             auto page_of = [&](int j) { return page_at(j < n ? tile_at(j) * kPwKeys : 0); };
@@ -1100,14 +1101,14 @@ static int launch_prefill_window(PwParams& p, const CUtensorMap& mq, const CUten
 }
 
 static int paged_prefill_window(const infer_kv_pool_t* pool, void* out, const void* q, int64_t total_q, const int32_t* cu_seqlens_q,
-                                const int32_t* cu_seqlens_k, const int32_t* block_tables, int64_t bt_stride, int batch,
-                                int max_seqlen_q, int max_seqlen_k, int n_q_heads, float softmax_scale, int window, int sinks, cudaStream_t st,
-                                uint32_t wait_limit, int stall_producer) {
+                                const int32_t* cu_seqlens_k, const int32_t* block_tables, int64_t bt_stride, int64_t bt_columns,
+                                int batch, int max_seqlen_q, int max_seqlen_k, int n_q_heads, float softmax_scale, int window, int sinks,
+                                cudaStream_t st, uint32_t wait_limit, int stall_producer) {
     if (!(softmax_scale > 0.f) || !(softmax_scale < INFINITY) || window < 0 || sinks < 0) return INFER_ERR_GEOMETRY;
     if (!pool || !out || !q || !cu_seqlens_q || !cu_seqlens_k || !block_tables) return INFER_ERR_NULL;
     if (batch < 0 || n_q_heads <= 0 || n_q_heads % pool->n_kv_heads != 0 || n_q_heads / pool->n_kv_heads > kPwRows || bt_stride <= 0 ||
         max_seqlen_q < 0 || max_seqlen_k < 0 || batch > 65535 || n_q_heads > 65535 || total_q < 0 ||
-        total_q > int64_t(batch) * max_seqlen_q || total_q >= (int64_t(1) << 31))
+        total_q > int64_t(batch) * max_seqlen_q || total_q >= (int64_t(1) << 31) || bt_columns < 0)
         return INFER_ERR_GEOMETRY;
     if (!aligned16(out) || !aligned16(q)) return INFER_ERR_ALIGN;
     if (total_q == 0 || batch == 0) return INFER_OK;
@@ -1118,6 +1119,7 @@ static int paged_prefill_window(const infer_kv_pool_t* pool, void* out, const vo
     p.cu_k = cu_seqlens_k;
     p.block_tables = block_tables;
     p.bt_stride = bt_stride;
+    p.bt_columns = bt_columns;
     p.k_scale = pool->k_scale;
     p.v_scale = pool->v_scale;
     p.n_q_heads = n_q_heads;
@@ -1156,19 +1158,28 @@ int infer_paged_prefill_window(const infer_kv_pool_t* pool, void* out, const voi
                                const int32_t* cu_seqlens_k, const int32_t* block_tables, int64_t bt_stride, int batch,
                                int max_seqlen_q, int max_seqlen_k, int n_q_heads, float softmax_scale, int window, int sinks,
                                void* stream_) {
-    return ib::paged_prefill_window(pool, out, q, total_q, cu_seqlens_q, cu_seqlens_k, block_tables, bt_stride, batch, max_seqlen_q,
-                                    max_seqlen_k, n_q_heads, softmax_scale, window, sinks, static_cast<cudaStream_t>(stream_),
-                                    ib::kDefaultWaitLimit, 0);
+    return infer_paged_prefill_window_columns(pool, out, q, total_q, cu_seqlens_q, cu_seqlens_k, block_tables, bt_stride, bt_stride, batch,
+                                              max_seqlen_q, max_seqlen_k, n_q_heads, softmax_scale, window, sinks, stream_);
+}
+
+int infer_paged_prefill_window_columns(const infer_kv_pool_t* pool, void* out, const void* q, int64_t total_q,
+                                       const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, const int32_t* block_tables,
+                                       int64_t bt_stride, int64_t bt_columns, int batch, int max_seqlen_q, int max_seqlen_k,
+                                       int n_q_heads, float softmax_scale, int window, int sinks, void* stream_) {
+    return ib::paged_prefill_window(pool, out, q, total_q, cu_seqlens_q, cu_seqlens_k, block_tables, bt_stride, bt_columns, batch,
+                                    max_seqlen_q, max_seqlen_k, n_q_heads, softmax_scale, window, sinks,
+                                    static_cast<cudaStream_t>(stream_), ib::kDefaultWaitLimit, 0);
 }
 
 int infer_selftest_paged_prefill_window(const infer_kv_pool_t* pool, void* out, const void* q, int64_t total_q,
                                         const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, const int32_t* block_tables,
-                                        int64_t bt_stride, int batch, int max_seqlen_q, int max_seqlen_k, int n_q_heads,
-                                        float softmax_scale, int window, int sinks, void* stream_, uint32_t wait_limit,
-                                        int stall_producer) {
-    return ib::paged_prefill_window(pool, out, q, total_q, cu_seqlens_q, cu_seqlens_k, block_tables, bt_stride, batch, max_seqlen_q,
-                                    max_seqlen_k, n_q_heads, softmax_scale, window, sinks, static_cast<cudaStream_t>(stream_),
-                                    wait_limit ? wait_limit : ib::kDefaultWaitLimit, stall_producer);
+                                        int64_t bt_stride, int64_t bt_columns, int batch, int max_seqlen_q, int max_seqlen_k,
+                                        int n_q_heads, float softmax_scale, int window, int sinks, void* stream_,
+                                        uint32_t wait_limit, int stall_producer) {
+    return ib::paged_prefill_window(pool, out, q, total_q, cu_seqlens_q, cu_seqlens_k, block_tables, bt_stride, bt_columns, batch,
+                                    max_seqlen_q, max_seqlen_k, n_q_heads, softmax_scale, window, sinks,
+                                    static_cast<cudaStream_t>(stream_), wait_limit ? wait_limit : ib::kDefaultWaitLimit,
+                                    stall_producer);
 }
 
 }  // extern "C"
