@@ -1030,6 +1030,7 @@ static int prefill_device(const PwDevice** out) {
     *out = &d;
     if (d.ready.load(std::memory_order_acquire)) return INFER_OK;
     std::lock_guard<std::mutex> lock(mutex);
+    if (d.ready.load(std::memory_order_relaxed)) return INFER_OK;       // another thread was first: its counts may be in use by now
     const int smem = PwCfg<FP8>::total + 1024;
     IB_CUDA(cudaFuncSetAttribute(prefill_window_kernel<FP8>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     IB_CUDA(cudaFuncSetAttribute(prefill_window_kernel<FP8>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
