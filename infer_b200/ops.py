@@ -120,6 +120,8 @@ class KVPool:
                 raise ValueError("pools must be contiguous CUDA tensors [num_blocks, block_size, Hkv, head_dim]")
         if k_cache.shape != v_cache.shape or k_cache.dtype != v_cache.dtype:
             raise ValueError("k and v pools must agree in shape and dtype")
+        if k_cache.device != v_cache.device:
+            raise ValueError("k and v pools must live on the same GPU")
         fp8 = k_cache.dtype in (torch.uint8, torch.float8_e4m3fn)
         if not fp8 and k_cache.dtype != torch.bfloat16:
             raise ValueError("pools must be bf16 or e4m3 bytes")
@@ -128,6 +130,8 @@ class KVPool:
             for s in (k_scale, v_scale):
                 if s is None or s.dtype != torch.float32 or tuple(s.shape) != (nb, hkv) or not s.is_contiguous():
                     raise ValueError("e4m3 pools need contiguous fp32 scales [num_blocks, Hkv]")
+                if s.device != k_cache.device:
+                    raise ValueError("the scales of e4m3 pools must live on the pools' GPU")
         # The handle only borrows the tensors' memory (addresses and geometry): it keeps no
         # reference, so a cached handle never pins gigabytes of pool memory.
         self.fp8 = fp8
