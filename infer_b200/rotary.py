@@ -41,8 +41,8 @@ def rotary_frequencies(rot_dim: int, base: float = 10000.0, scaling: str | None 
         # index of the pair that makes n turns over the trained context
         at = lambda n: rot_dim * math.log(original_max_position / (2 * math.pi * n)) / (2 * math.log(base))
         low = max(0, math.floor(at(fast_turns)))
-        high = min(rot_dim // 2 - 1, math.ceil(at(slow_turns)))
-        slow = ((i - low) / max(high - low, 1e-3)).clamp(0, 1)
+        high = math.ceil(at(slow_turns))       # behind the last pair when even that one makes more than slow_turns turns
+        slow = ((i - low) / (high - low)).clamp(0, 1) if high > low else (i >= high).double()
         inv_freq = inv_freq * (1 - slow) + inv_freq / factor * slow
         attention_factor = 1 + 0.1 * math.log(factor)
     elif scaling not in (None, "ntk"):

@@ -70,3 +70,45 @@ def test_window_entry_points_check_window_and_scale_first():
         assert lib.infer_paged_decode_append_window(None, p, p, p, p, 128, 128, p, p, 4, 1, 8, scale, window, sinks, None, 0,
                                                     None) == _lib.ERR_GEOMETRY
     assert lib.infer_paged_decode_window(None, p, p, p, p, 4, 1, 8, 0.1, 5, 0, None, 0, None) == _lib.ERR_NULL
+
+
+def _ramp(rot_dim, base, context, fast, slow):
+    """How far pair i lies from the pair that makes ``fast`` turns over the context (0) to the one that makes ``slow`` (1), pairs
+    counted from the fastest, both ends moved outwards to whole pairs and the first to pair 0 at least."""
+    out = []
+    for i in range(rot_dim // 2):
+        first = max(0, math.floor(rot_dim / 2 * math.log(context / (2 * math.pi * fast), base)))
+        last = math.ceil(rot_dim / 2 * math.log(context / (2 * math.pi * slow), base))
+        out.append(min(1.0, max(0.0, (i - first) / (last - first))))
+    return torch.tensor(out, dtype=torch.float64)
+
+
+@pytest.mark.parametrize("base", [10000.0, 500000.0])
+@pytest.mark.parametrize("rot_dim", [16, 32, 64, 96, 128])
+@pytest.mark.parametrize("context", [300, 4096, 65536, 131072, 262144, 2 ** 22])
+@pytest.mark.parametrize("factor", [1.0, 4.0, 32.0])
+def test_yarn_at_contexts_short_and_long(context, rot_dim, base, factor):
+    """Pairs above fast_turns keep their frequency, pairs below slow_turns are divided by the factor, the ramp is between, also
+    where it ends behind the last pair: base 10000, 128 dims, 131072 positions, the slowest pair makes 2.41 turns."""
+    f, _ = rotary_frequencies(rot_dim, base)
+    g, _ = rotary_frequencies(rot_dim, base, "yarn", factor, context)
+    turns, ratio = context * f / (2 * math.pi), g / f
+    assert torch.allclose(ratio[turns > 32], torch.ones(1, dtype=torch.float64), rtol=1e-14, atol=0)
+    assert torch.allclose(ratio[turns < 1], torch.tensor([1 / factor], dtype=torch.float64), rtol=1e-14, atol=0)
+    want = 1 - (1 - 1 / factor) * _ramp(rot_dim, base, context, 32.0, 1.0)
+    assert torch.allclose(ratio, want, rtol=1e-12, atol=0)
+    if factor > 1:
+        assert bool((ratio[turns > 1 + 1e-9] > 1 / factor).all())
+
+
+def test_yarn_where_the_slowest_pair_is_on_the_ramp():
+    for rot_dim, context, ratio in ((128, 65536, 0.31), (128, 131072, 0.46)):
+        f, g = rotary_frequencies(rot_dim)[0], rotary_frequencies(rot_dim, scaling="yarn", factor=4.0, original_max_position=context)[0]
+        assert abs((g / f)[-1].item() - ratio) < 0.005
+
+
+@pytest.mark.parametrize("context", [1, 3, 6])
+def test_yarn_of_a_context_of_less_than_a_turn(context):
+    """No pair makes a turn: all are divided."""
+    f, g = rotary_frequencies(64)[0], rotary_frequencies(64, scaling="yarn", factor=8.0, original_max_position=context)[0]
+    assert torch.allclose(g, f / 8, rtol=1e-14, atol=0)
