@@ -513,6 +513,34 @@ struct Fp8Smem {
     static constexpr int total = tile + 16;
 };
 
+// One row of queries as f16, this lane's share (four lanes have a row: dims 16 c + 4 tig .. + 3, c = 0 .. 7), divided by a power
+// of two, which is returned, where bf16 reaches further than f16: a row whose largest value lies outside of [2^-3, 2^15) is
+// brought to [2^14, 2^15).  The others go in as they are: a value below 2^-17 then loses bits, 2^-25 of an absolute error,
+// 2^-22 of the row's largest at most.  (Dividing every row would change nothing else, all factors being powers of two.)  Rows
+// that are not finite stay as they are.
+__device__ __forceinline__ float queries_to_f16(const __nv_bfloat16* row, bool live, int tig, uint32_t (&qb)[8][2]) {
+    uint2 raw[8];
+#pragma unroll
+    for (int c = 0; c < 8; ++c) raw[c] = live ? *reinterpret_cast<const uint2*>(row + c * 16 + tig * 4) : make_uint2(0u, 0u);
+    auto pair = [](const uint32_t& v) { return *reinterpret_cast<const __nv_bfloat162*>(&v); };
+    __nv_bfloat162 top2 = __habs2(pair(raw[0].x));                     // largest magnitudes, NaN if there is one
+#pragma unroll
+    for (int c = 0; c < 8; ++c) top2 = __hmax2_nan(top2, __hmax2_nan(__habs2(pair(raw[c].x)), __habs2(pair(raw[c].y))));
+    uint32_t top = __bfloat16_as_ushort(__hmax_nan(__low2bfloat16(top2), __high2bfloat16(top2))) & 0x7fffu;
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));              // (a NaN is the largest as a whole number too)
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    const int field = int(top >> 7);                                   // exponent + 127
+    const int e = top == 0 || field == 255 || (field >= 127 - 3 && field < 127 + 15) ? 0 : max(field - (127 + 14), -126);
+    const uint32_t down = uint32_t(127 - e) << 7 | uint32_t(127 - e) << 23;          // 2^-e twice
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+        const __nv_bfloat162 x = __hmul2_rn(pair(raw[c].x), pair(down)), y = __hmul2_rn(pair(raw[c].y), pair(down));
+        qb[c][0] = pack_f16(__low2float(x), __high2float(x));
+        qb[c][1] = pack_f16(__low2float(y), __high2float(y));
+    }
+    return __uint_as_float(uint32_t(127 + e) << 23);
+}
+
 template <int HPC, bool WINDOW>
 __global__ void __launch_bounds__(kTmaThreads, 1) decode_tma_fp8_kernel(DecodeParams p,
                                                                           const __grid_constant__ CUtensorMap map_k,
@@ -677,20 +705,9 @@ __global__ void __launch_bounds__(kTmaThreads, 1) decode_tma_fp8_kernel(DecodePa
         // (2t, 2t+1, 2t+8, 2t+9) of a 16-dim chunk carry dims (4t, 4t+1, 4t+2, 4t+3): the order in
         // which ldmatrix hands out e4m3 bytes.
         uint32_t qb[8][2];
-        {
-            const __nv_bfloat16* qrow = p.q + (int64_t(sg.b) * p.n_q_heads + head * p.group + gid) * kHeadDim;
-#pragma unroll
-            for (int c = 0; c < 8; ++c) {
-                qb[c][0] = qb[c][1] = 0u;
-                if (gid < p.group) {
-                    const uint2 raw = *reinterpret_cast<const uint2*>(qrow + c * 16 + tig * 4);
-                    const __nv_bfloat162 x = *reinterpret_cast<const __nv_bfloat162*>(&raw.x);
-                    const __nv_bfloat162 y = *reinterpret_cast<const __nv_bfloat162*>(&raw.y);
-                    qb[c][0] = pack_f16(__low2float(x), __high2float(x));
-                    qb[c][1] = pack_f16(__low2float(y), __high2float(y));
-                }
-            }
-        }
+        const float unit = queries_to_f16(p.q + (int64_t(sg.b) * p.n_q_heads + head * p.group + gid) * kHeadDim, gid < p.group, tig, qb);
+        // factor of the scores of heads 2t and 2t + 1, without the page's scale (a row's lanes are four times its number on)
+        const float c_q[2] = {__shfl_sync(0xffffffffu, p.scale_log2 * unit, tig * 8), __shfl_sync(0xffffffffu, p.scale_log2 * unit, tig * 8 + 4)};
         float o[8][4];                           // O^T: tile c, rows (dims 16c + 2g, 16c + 2g + 1), columns (heads 2t, 2t+1)
 #pragma unroll
         for (int j = 0; j < 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
@@ -700,7 +717,7 @@ __global__ void __launch_bounds__(kTmaThreads, 1) decode_tma_fp8_kernel(DecodePa
         for (int t = sg.t0; t < sg.t1; ++t, ++it) {
             const uint32_t s = it % kStages, ph = (it / kStages) & 1;
             if (ok && !mbar_wait(full0 + s * 8, ph, p.wait_limit)) ok = false;
-            const float c_k = s_meta[(s * HPC + hl) * 2 + 0] * p.scale_log2;
+            const float ks = s_meta[(s * HPC + hl) * 2 + 0];
             const float vs = s_meta[(s * HPC + hl) * 2 + 1];
             const int row0 = tw * TPW;                      // this warp's tokens of the tile
             const int tok_w = (WINDOW ? s_tile[s] : t) * TT + row0;
@@ -746,6 +763,7 @@ __global__ void __launch_bounds__(kTmaThreads, 1) decode_tma_fp8_kernel(DecodePa
                 float pr[NH][2][2];
 #pragma unroll
                 for (int y = 0; y < 2; ++y) {
+                    const float c_k = ks * c_q[y];
                     float mx = fmaxf(sv[0][0][y], sv[0][1][y]);
                     if (NH == 2) mx = fmaxf(mx, fmaxf(sv[NH - 1][0][y], sv[NH - 1][1][y]));
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
