@@ -80,11 +80,11 @@ SELFTEST_SIGNATURES = {
 }
 
 _lib = None
-host_ops = None            # the module of csrc/host_ops.cpp, bound to the loaded library
+host_ops = None            # the module of csrc/host_ops.cpp once it is bound to the loaded library
 
 
 def load() -> C.CDLL:
-    global _lib, host_ops
+    global _lib
     if _lib is not None:
         return _lib
     if not LIB_PATH.exists():
@@ -95,15 +95,24 @@ def load() -> C.CDLL:
     for name, (res, args) in {**SIGNATURES, **SELFTEST_SIGNATURES}.items():
         fn = getattr(lib, name)
         fn.restype, fn.argtypes = res, args
-    try:
-        from . import _host_ops
-    except ImportError as e:
-        raise ImportError(f"infer_b200/_host_ops.so is missing or does not fit this PyTorch: build it with "
-                          f"`python -m infer_b200.build` ({e})") from e
-    _host_ops.bind_library({name: C.cast(getattr(lib, name), C.c_void_p).value for name in {**SIGNATURES, **SELFTEST_SIGNATURES}})
-    host_ops = _host_ops
     _lib = lib
     return lib
+
+
+def load_host_ops():
+    """The module of csrc/host_ops.cpp, which only the ops that are checked and launched there need: everything else goes
+    through ``load`` alone."""
+    global host_ops
+    if host_ops is None:
+        lib = load()
+        try:
+            from . import _host_ops
+        except ImportError as e:
+            raise ImportError(f"infer_b200/_host_ops.so is missing or does not fit this PyTorch: build it with "
+                              f"`python -m infer_b200.build` ({e})") from e
+        _host_ops.bind_library({name: C.cast(getattr(lib, name), C.c_void_p).value for name in {**SIGNATURES, **SELFTEST_SIGNATURES}})
+        host_ops = _host_ops
+    return host_ops
 
 
 def check(rc: int, what: str):

@@ -29,7 +29,9 @@ _CHECK = os.environ.get("INFER_B200_CHECK") == "1"    # debugging: read the devi
 
 
 # The raw stream and addresses as plain integers: a Stream object costs 3 us, a c_void_p per pointer 0.1.
-_raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+# (A PyTorch without CUDA has neither; the package, whose page allocator is host code, imports there too.)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda device: torch.cuda.current_stream(device).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def _stream():
@@ -250,9 +252,7 @@ def qk_norm_rope_append(q, k, v, q_norm_weight, k_norm_weight, eps, positions, c
 
 def _host_ops():
     """The module of csrc/host_ops.cpp: argument checks and launches of the ops below."""
-    if _lib.host_ops is None:
-        _lib.load()
-    return _lib.host_ops
+    return _lib.host_ops or _lib.load_host_ops()
 
 
 def load_kvcache(k_cache, v_cache, slot_mapping, k_scale=None, v_scale=None, k_out=None, v_out=None):
