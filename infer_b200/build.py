@@ -2,19 +2,22 @@
 
 ``python -m infer_b200.build`` compiles every ``csrc/*.cu`` with nvcc into one shared
 library next to this file, and ``csrc/host_ops.cpp`` with g++ against PyTorch's headers into
-a Python module beside it.  Either is rebuilt only when a source is newer than it.
+a Python module beside it.  Either is rebuilt only when a source of its own is newer than it, the
+module also when it was built for another PyTorch or Python.
 """
 from __future__ import annotations
 
 import os
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 HERE = Path(__file__).resolve().parent
 CSRC = HERE / "csrc"
 LIB = HERE / "libinfer_b200.so"
 HOST_OPS = HERE / "_host_ops.so"
+HOST_OPS_TARGET = HERE / "_host_ops.target"      # what the module was built for
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -31,17 +34,29 @@ def sources():
 def _stale() -> bool:
     if not LIB.exists():
         return True
-    newest = max(p.stat().st_mtime for p in list(CSRC.glob("*")) + [HERE.parent / "include" / "infer_b200.h"])
-    return newest > LIB.stat().st_mtime
+    own = [*sources(), *CSRC.glob("*.cuh"), *(HERE.parent / "include").glob("infer_b200*.h"), HERE.parent / "include" / "block_manager.hpp"]
+    return max(p.stat().st_mtime for p in own) > LIB.stat().st_mtime
+
+
+def host_ops_target() -> str:
+    """The PyTorch and the Python that a module built now fits."""
+    import torch
+    return f"torch {torch.__version__}, {sysconfig.get_config_var('SOABI')}"
+
+
+def _host_ops_stale(target: str) -> bool:
+    if not HOST_OPS.exists() or not HOST_OPS_TARGET.exists() or HOST_OPS_TARGET.read_text() != target:
+        return True
+    own = [CSRC / "host_ops.cpp", *(HERE.parent / "include").glob("infer_b200*.h")]
+    return max(p.stat().st_mtime for p in own) > HOST_OPS.stat().st_mtime
 
 
 def build_host_ops(force: bool = False) -> subprocess.Popen | None:
     """Starts the compiler on host_ops.cpp; None when the module is up to date."""
-    src = CSRC / "host_ops.cpp"
-    newest = max(p.stat().st_mtime for p in [src, *(HERE.parent / "include").glob("infer_b200*.h")])
-    if not force and HOST_OPS.exists() and HOST_OPS.stat().st_mtime >= newest:
+    src, target = CSRC / "host_ops.cpp", host_ops_target()
+    if not force and not _host_ops_stale(target):
         return None
-    import sysconfig
+    HOST_OPS_TARGET.unlink(missing_ok=True)
     import torch
     root = Path(torch.__file__).resolve().parent
     cuda = os.environ.get("CUDA_HOME", "/usr/local/cuda")
@@ -54,7 +69,11 @@ def build_host_ops(force: bool = False) -> subprocess.Popen | None:
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
-    host = build_host_ops(force)
+    host, why = None, ""
+    try:
+        host = build_host_ops(force)
+    except (ImportError, OSError) as e:          # no PyTorch or no compiler: the library is built all the same
+        why = str(e)
     try:
         build_library(force, verbose)
     finally:
@@ -62,8 +81,12 @@ def build(force: bool = False, verbose: bool = False) -> Path:
             out, _ = host.communicate()
             if host.returncode != 0 or verbose:
                 sys.stderr.write(f"--- host_ops.cpp\n{out}\n")
-    if host is not None and host.returncode != 0:
-        raise RuntimeError("g++ failed")
+            if host.returncode == 0:
+                HOST_OPS_TARGET.write_text(host_ops_target())
+            else:
+                why = "g++ failed"
+    if why:
+        raise RuntimeError(f"{LIB.name} is built, {HOST_OPS.name} is not, and the ops that it launches will refuse: {why}")
     return LIB
 
 
