@@ -30,6 +30,15 @@ INFER_API int infer_selftest_paged_decode(const infer_kv_pool_t* pool, void* out
                                 void* workspace, size_t workspace_bytes, void* stream,
                                 int heads_per_tile, uint32_t wait_limit, int stall_producer);
 
+/* infer_paged_decode_window, or infer_paged_decode_append_window where k and v are not null; wait_limit and
+ * stall_producer as above. */
+INFER_API int infer_selftest_paged_decode_window(const infer_kv_pool_t* pool, void* out, const void* q, const void* k,
+                                const void* v, int64_t k_row_stride, int64_t v_row_stride,
+                                const int32_t* context_lens, const int32_t* block_tables, int64_t bt_stride,
+                                int batch, int n_q_heads, float softmax_scale, int window, int sinks,
+                                void* workspace, size_t workspace_bytes, void* stream, uint32_t wait_limit,
+                                int stall_producer);
+
 /* infer_paged_prefill / infer_flash_attn_prefill on a chosen kernel.
  *   kernel          0 = the tcgen05 kernel (the product path); 1 = the mma.sync cross-check kernel
  *   wait_limit, stall_producer   as above (tcgen05 kernel only); the status is read with

@@ -72,6 +72,8 @@ _u32 = C.c_uint32
 SELFTEST_SIGNATURES = {
     "infer_selftest_paged_decode": (_i32, [_vp, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _f32, _vp, _sz, _vp,
                                            _i32, _u32, _i32]),
+    "infer_selftest_paged_decode_window": (_i32, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _vp, _i64, _i32, _i32, _f32, _i32, _i32,
+                                                  _vp, _sz, _vp, _u32, _i32]),
     "infer_selftest_paged_prefill": (_i32, [_vp, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _f32, _vp,
                                             _i32, _u32, _i32]),
     "infer_selftest_paged_prefill_window": (_i32, [_vp, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i32, _i32, _i32, _i32, _f32,

@@ -1263,6 +1263,25 @@ int infer_selftest_paged_decode(const infer_kv_pool_t* pool, void* out, const vo
                             wait_limit ? wait_limit : ib::kDefaultWaitLimit, stall_producer);
 }
 
+int infer_selftest_paged_decode_window(const infer_kv_pool_t* pool, void* out, const void* q, const void* k, const void* v,
+                                       int64_t k_row_stride, int64_t v_row_stride, const int32_t* context_lens,
+                                       const int32_t* block_tables, int64_t bt_stride, int batch, int n_q_heads,
+                                       float softmax_scale, int window, int sinks, void* workspace, size_t workspace_bytes,
+                                       void* stream_, uint32_t wait_limit, int stall_producer) {
+    if (!window_ok(window, sinks, softmax_scale)) return INFER_ERR_GEOMETRY;
+    ib::NewRows rows;
+    rows.k = k;
+    rows.v = v;
+    rows.k_stride = k_row_stride;
+    rows.v_stride = v_row_stride;
+    ib::Window win;
+    win.window = window;
+    win.sinks = sinks;
+    return ib::paged_decode(pool, out, q, context_lens, block_tables, bt_stride, batch, n_q_heads, softmax_scale, workspace,
+                            workspace_bytes, static_cast<cudaStream_t>(stream_), 0, wait_limit ? wait_limit : ib::kDefaultWaitLimit,
+                            stall_producer, rows, win);
+}
+
 int infer_paged_decode_status(const void* workspace, void* stream_) {
     using namespace ib;
     void* ws = const_cast<void*>(workspace);

@@ -31,16 +31,17 @@ struct Library {
     decltype(&infer_paged_decode_window) decode_window = nullptr;
     decltype(&infer_paged_decode_append_window) decode_append_window = nullptr;
     decltype(&infer_paged_prefill_window_columns) prefill_window = nullptr;
+    decltype(&infer_selftest_paged_decode_window) decode_window_test = nullptr;
     decltype(&infer_selftest_paged_prefill_window) prefill_window_test = nullptr;
     decltype(&infer_strerror) strerror = nullptr;
     decltype(&infer_last_cuda_error) last_cuda_error = nullptr;
 } lib;
 
-// What the prefill call is routed to while a test makes the kernel's waits run out (0, 0: the product entry point).
+// What the windowed calls are routed to while a test makes the kernels' waits run out (0, 0: the product entry points).
 struct {
     uint32_t wait_limit = 0;
     int stall_producer = 0;
-} prefill_test;
+} wait_test;
 
 template <class F>
 void bind_one(F& f, const pybind11::dict& d, const char* name) {
@@ -54,6 +55,7 @@ void bind_library(const pybind11::dict& d) {
     bind_one(lib.decode_window, d, "infer_paged_decode_window");
     bind_one(lib.decode_append_window, d, "infer_paged_decode_append_window");
     bind_one(lib.prefill_window, d, "infer_paged_prefill_window_columns");
+    bind_one(lib.decode_window_test, d, "infer_selftest_paged_decode_window");
     bind_one(lib.prefill_window_test, d, "infer_selftest_paged_prefill_window");
     bind_one(lib.strerror, d, "infer_strerror");
     bind_one(lib.last_cuda_error, d, "infer_last_cuda_error");
@@ -228,12 +230,8 @@ Tensor decode_window(uintptr_t pool, int64_t device, int64_t n_kv_heads, const T
     Launch l(device);
     const auto* cl = static_cast<const int32_t*>(lens.data_ptr());
     const auto* bt = static_cast<const int32_t*>(table.data_ptr());
-    if (!key) {
-        check(lib.decode_window(pool_at(pool), o.data_ptr(), q.data_ptr(), cl, bt, table_pitch, int(b), int(q.size(-2)), float(scale),
-                                win, sink, ws.data_ptr(), size_t(ws.numel()), l.stream),
-              what);
-    } else {
-        int64_t pitch[2];
+    int64_t pitch[2] = {0, 0};
+    if (key) {
         const Tensor* kv[2] = {&*key, &*value};
         for (int i = 0; i < 2; ++i) {
             const Tensor& t = *kv[i];
@@ -244,6 +242,18 @@ Tensor decode_window(uintptr_t pool, int64_t device, int64_t n_kv_heads, const T
             reachable(name, t);
             pitch[i] = b > 1 ? t.stride(0) : n_kv_heads * 128;
         }
+    }
+    if (wait_test.wait_limit || wait_test.stall_producer) {
+        check(lib.decode_window_test(pool_at(pool), o.data_ptr(), q.data_ptr(), key ? key->data_ptr() : nullptr,
+                                     key ? value->data_ptr() : nullptr, pitch[0], pitch[1], cl, bt, table_pitch, int(b), int(q.size(-2)),
+                                     float(scale), win, sink, ws.data_ptr(), size_t(ws.numel()), l.stream, wait_test.wait_limit,
+                                     wait_test.stall_producer),
+              what);
+    } else if (!key) {
+        check(lib.decode_window(pool_at(pool), o.data_ptr(), q.data_ptr(), cl, bt, table_pitch, int(b), int(q.size(-2)), float(scale),
+                                win, sink, ws.data_ptr(), size_t(ws.numel()), l.stream),
+              what);
+    } else {
         check(lib.decode_append_window(pool_at(pool), o.data_ptr(), q.data_ptr(), key->data_ptr(), value->data_ptr(), pitch[0], pitch[1],
                                        cl, bt, table_pitch, int(b), int(q.size(-2)), float(scale), win, sink, ws.data_ptr(),
                                        size_t(ws.numel()), l.stream),
@@ -275,10 +285,10 @@ Tensor prefill_window(uintptr_t pool, int64_t device, const Tensor& q, const Ten
     const auto* ck = static_cast<const int32_t*>(cu_k.data_ptr());
     const auto* bt = static_cast<const int32_t*>(table.data_ptr());
     const int hq = int(q.size(1));
-    if (prefill_test.wait_limit || prefill_test.stall_producer)
+    if (wait_test.wait_limit || wait_test.stall_producer)
         check(lib.prefill_window_test(pool_at(pool), o.data_ptr(), q.data_ptr(), q.size(0), cq, ck, bt, table_pitch, table.size(1),
-                                      int(batch), int(max_q), int(max_k), hq, float(scale), win, sink, l.stream, prefill_test.wait_limit,
-                                      prefill_test.stall_producer),
+                                      int(batch), int(max_q), int(max_k), hq, float(scale), win, sink, l.stream, wait_test.wait_limit,
+                                      wait_test.stall_producer),
               what);
     else
         check(lib.prefill_window(pool_at(pool), o.data_ptr(), q.data_ptr(), q.size(0), cq, ck, bt, table_pitch, table.size(1), int(batch),
@@ -291,9 +301,9 @@ Tensor prefill_window(uintptr_t pool, int64_t device, const Tensor& q, const Ten
 
 PYBIND11_MODULE(_host_ops, m) {
     m.def("bind_library", &bind_library);
-    m.def("set_prefill_test", [](uint32_t wait_limit, int stall_producer) {
-        prefill_test.wait_limit = wait_limit;
-        prefill_test.stall_producer = stall_producer;
+    m.def("set_wait_test", [](uint32_t wait_limit, int stall_producer) {
+        wait_test.wait_limit = wait_limit;
+        wait_test.stall_producer = stall_producer;
     });
     m.def("load_kvcache", &load_kvcache);
     m.def("rotary_append", &rotary_append);

@@ -32,13 +32,13 @@ def variant(decode_heads_per_tile: int = 0, prefill_kernel: int = 0, wait_limit:
     ops._call_decode, ops._call_prefill, ops._call_dense = decode, prefill, dense
     try:
         host_ops = _lib.load_host_ops()
-    except ImportError:                       # then there is no windowed prefill call to route
+    except ImportError:                       # then there are no windowed calls to route
         host_ops = None
     try:
         if host_ops is not None:
-            host_ops.set_prefill_test(wait_limit, stall_producer)
+            host_ops.set_wait_test(wait_limit, stall_producer)
         yield
     finally:
         ops._call_decode, ops._call_prefill, ops._call_dense = saved
         if host_ops is not None:
-            host_ops.set_prefill_test(0, 0)
+            host_ops.set_wait_test(0, 0)
