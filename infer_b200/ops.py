@@ -472,7 +472,7 @@ def register_torch_ops():
     lib.define("paged_attn_prefill(Tensor! out, Tensor q, Tensor k_cache, Tensor v_cache, Tensor cu_seqlens_q, "
                "Tensor cu_seqlens_k, int max_seqlen_q, int max_seqlen_k, float softmax_scale, Tensor block_table) -> ()")
     lib.define("paged_attn_decode_window(Tensor! out, Tensor q, Tensor k_cache, Tensor v_cache, Tensor cache_seqlens, "
-               "Tensor block_table, float softmax_scale, int window, int sinks, Tensor? k_scale=None, Tensor? v_scale=None) -> ()")
+               "Tensor block_table, float softmax_scale, int? window, int sinks, Tensor? k_scale=None, Tensor? v_scale=None) -> ()")
     lib.define("paged_attn_prefill_window(Tensor! out, Tensor q, Tensor k_cache, Tensor v_cache, Tensor cu_seqlens_q, "
                "Tensor cu_seqlens_k, int max_seqlen_q, int max_seqlen_k, float softmax_scale, Tensor block_table, int? window, "
                "int sinks, Tensor? k_scale=None, Tensor? v_scale=None) -> ()")
