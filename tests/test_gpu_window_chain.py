@@ -156,3 +156,62 @@ def test_torch_ops_of_the_new_kernels():
     infer_ops.rotary_append(out, q, kv, kv, pos, f, kc, vc, slots[:2], True, 1.0)
     want = ops.rotary_embedding(q, kv, pos, f, interleaved=True)
     assert torch.equal(out, want[0]) and torch.equal(kc[0, 100:102], want[1]) and torch.equal(vc[0, 100:102], kv)
+
+
+def _against_the_pools(attn, q, o, tables, lens, new, kind, decode, what):
+    """The layer's output against 64 bits on the values that the pools hold, with the bounds of the kernels' own tests: f16
+    probabilities over e4m3 pools, bf16 ones over bf16 pools.  Returns how many values another window or no sinks would have put
+    out of those bounds (worked out on the CPU)."""
+    at, told = 0, {"a shorter window": 0, "no sinks": 0, "nothing": 0}
+    for b, (n, m) in enumerate(zip(lens, new)):
+        k, v = (plain64.values(c, s, tables[b], n).cpu() for c, s in ((attn.k_cache, attn.k_scale), (attn.v_cache, attn.v_scale)))
+        rows, got = q[at:at + m].cpu(), o[at:at + m].view(m, HQ, 128).double().cpu()
+
+        def exact(window, sinks):
+            seen = plain64.visible(n, torch.arange(n - m, n), window, sinks)
+            if kind == "bf16":
+                return plain64.attention(rows, k, v, seen, attn.scale, plain64.E_BF16)
+            want, bound = plain64.attention(rows, k, v, seen, attn.scale, plain64.E_F16, 2.0 ** -25 if decode else 0.0)
+            return want, bound + (0.0 if decode else 2.0 ** -31 * n * v.abs().amax())
+
+        want, bound = exact(attn.window, attn.sinks)
+        plain64.check(got, want, bound, f"{what} sequence {b}")
+        for name, other in (("a shorter window", exact(attn.window - 1, attn.sinks)), ("no sinks", exact(attn.window, 0)),
+                            ("nothing", (torch.zeros_like(want), bound))):
+            told[name] += int(((got - other[0]).abs() > other[1]).sum())
+        at += m
+    return told
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+def test_chunks_then_decode_against_the_pools(kind):
+    """Chunked prefill, append and windowed decode through the layer, with bounds that a wrong window or lost sinks cannot meet; what
+    load_kvcache reads back is checked against the same pools by itself."""
+    gen = torch.Generator().manual_seed(6)
+    attn = _layer(kind, 9, 200, 4)
+    lens, tables = [0, 0, 0], [[4, 1, 7], [0, 5, 2], [3, 6, 8]]
+    rnd = lambda t, h: torch.randn(t, h, 128, generator=gen).bfloat16().cuda()
+    for step, new in enumerate(([300, 257, 1], [130, 256, 64])):
+        metadata.prepare_chunk(tables, lens, new, BS, "cuda")
+        q = rnd(sum(new), HQ)
+        o = attn(q, rnd(sum(new), HKV), rnd(sum(new), HKV))
+        reset_context()
+        lens = [n + m for n, m in zip(lens, new)]
+        told = _against_the_pools(attn, q, o, tables, lens, new, kind, False, f"chunk {step}")
+        assert min(told.values()) > 1000, told
+    for step in range(3):
+        lens = [n + 1 for n in lens]
+        slots = torch.tensor([metadata.chunk_slots(t, n - 1, n, BS)[0] for t, n in zip(tables, lens)], dtype=torch.int32).cuda()
+        set_context(False, slot_mapping=slots, context_lens=torch.tensor(lens, dtype=torch.int32).cuda(),
+                    block_tables=torch.tensor(tables, dtype=torch.int32).cuda())
+        q = rnd(3, HQ)
+        o = attn(q, rnd(3, HKV), rnd(3, HKV))
+        reset_context()
+        told = _against_the_pools(attn, q, o, tables, lens, [1, 1, 1], kind, True, f"step {step}")
+        assert min(told.values()) > 100, told
+    for t, n in zip(tables, lens):
+        slots = torch.tensor(metadata.chunk_slots(t, 0, n, BS), dtype=torch.int32, device="cuda")
+        back = ops.load_kvcache(attn.k_cache, attn.v_cache, slots, k_scale=attn.k_scale, v_scale=attn.v_scale)
+        for got, c, s in zip(back, (attn.k_cache, attn.v_cache), (attn.k_scale, attn.v_scale)):
+            # a product of 4 by 24 bits: exact in 64, rounded once to 32 bits and once to bf16
+            assert torch.equal(got, plain64.values(c, s, t, n).float().bfloat16())
