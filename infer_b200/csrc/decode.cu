@@ -513,11 +513,13 @@ struct Fp8Smem {
     static constexpr int total = tile + 16;
 };
 
-// One row of queries as f16, this lane's share (four lanes have a row: dims 16 c + 4 tig .. + 3, c = 0 .. 7), divided by a power
-// of two, which is returned, where bf16 reaches further than f16: a row whose largest value lies outside of [2^-3, 2^15) is
-// brought to [2^14, 2^15).  The others go in as they are: a value below 2^-17 then loses bits, 2^-25 of an absolute error,
-// 2^-22 of the row's largest at most.  (Dividing every row would change nothing else, all factors being powers of two.)  Rows
-// that are not finite stay as they are.
+// Rows of queries as f16, one per four lanes (dims 16 c + 4 tig .. + 3, c = 0 .. 7, are this lane's), divided by a power of two,
+// which is returned, where bf16 reaches further than f16: a row whose largest value lies outside of [2^-3, 2^15) is brought to
+// [2^14, 2^15).  The others go in as they are: a value below 2^-17 then loses bits, 2^-25 of an absolute error, 2^-22 of the
+// row's largest at most.  (Dividing every row would change nothing else, all factors being powers of two.)  Rows that are not
+// finite stay as they are.  Where every lane's largest value is in that range, the ordinary case, one vote settles it.  128 sequences
+// with a window of 256: 25.14 us without any of this, 25.33 with it; of 167 sequences of up to eight keys, three of them per thread
+// block in turn, 8.92 and 9.08 (9.12 with every row's exponent found first); long contexts and the benchmark's batch lose nothing.
 __device__ __forceinline__ float queries_to_f16(const __nv_bfloat16* row, bool live, int tig, uint32_t (&qb)[8][2]) {
     uint2 raw[8];
 #pragma unroll
@@ -527,18 +529,27 @@ __device__ __forceinline__ float queries_to_f16(const __nv_bfloat16* row, bool l
 #pragma unroll
     for (int c = 0; c < 8; ++c) top2 = __hmax2_nan(top2, __hmax2_nan(__habs2(pair(raw[c].x)), __habs2(pair(raw[c].y))));
     uint32_t top = __bfloat16_as_ushort(__hmax_nan(__low2bfloat16(top2), __high2bfloat16(top2))) & 0x7fffu;
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));              // (a NaN is the largest as a whole number too)
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    const int field = int(top >> 7);                                   // exponent + 127
-    const int e = top == 0 || field == 255 || (field >= 127 - 3 && field < 127 + 15) ? 0 : max(field - (127 + 14), -126);
-    const uint32_t down = uint32_t(127 - e) << 7 | uint32_t(127 - e) << 23;          // 2^-e twice
+    auto ordinary = [&] { return top >= (127u - 3u) << 7 && top < (127u + 15u) << 7; };
+    float unit = 1.f;
+    if (!__all_sync(0xffffffffu, !live || ordinary())) {
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));          // (a NaN is the largest as a whole number too)
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const int field = int(top >> 7);                               // exponent + 127
+        const int e = top == 0 || field == 255 || ordinary() ? 0 : max(field - (127 + 14), -126);
+        const uint32_t down = uint32_t(127 - e) << 7 | uint32_t(127 - e) << 23;      // 2^-e, twice
+        unit = __uint_as_float(uint32_t(127 + e) << 23);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+            const __nv_bfloat162 x = __hmul2_rn(pair(raw[c].x), pair(down)), y = __hmul2_rn(pair(raw[c].y), pair(down));
+            raw[c] = make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+        }
+    }
 #pragma unroll
     for (int c = 0; c < 8; ++c) {
-        const __nv_bfloat162 x = __hmul2_rn(pair(raw[c].x), pair(down)), y = __hmul2_rn(pair(raw[c].y), pair(down));
-        qb[c][0] = pack_f16(__low2float(x), __high2float(x));
-        qb[c][1] = pack_f16(__low2float(y), __high2float(y));
+        qb[c][0] = pack_f16(__low2float(pair(raw[c].x)), __high2float(pair(raw[c].x)));
+        qb[c][1] = pack_f16(__low2float(pair(raw[c].y)), __high2float(pair(raw[c].y)));
     }
-    return __uint_as_float(uint32_t(127 + e) << 23);
+    return unit;
 }
 
 template <int HPC, bool WINDOW>
@@ -769,8 +780,8 @@ __global__ void __launch_bounds__(kTmaThreads, 1) decode_tma_fp8_kernel(DecodePa
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-                    // with c_k == 0 (all-zero page) every visible logit is 0; masked ones stay -inf
-                    const float m_new = fmaxf(m_run[y], c_k > 0.f ? mx * c_k : 0.f);
+                    // with a scale of 0 (all-zero page) every visible logit is 0; masked ones stay -inf
+                    const float m_new = fmaxf(m_run[y], ks > 0.f ? mx * c_k : 0.f);
                     alpha[y] = fast_exp2(m_run[y] - m_new);
                     float rs = 0.f;
 #pragma unroll
