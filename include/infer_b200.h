@@ -97,10 +97,12 @@ INFER_API int infer_kv_load(const infer_kv_pool_t* pool, void* k_out, void* v_ou
 /* Rotary positions of q and k + KV append in one pass, bf16 pools.  The first rot_dim dims of every head (a multiple
  * of 16, at most 128) are rotated in pairs by the angle positions[t] * inv_freq[pair]: pairs (i, i + rot_dim / 2), or
  * (2i, 2i + 1) with interleaved != 0; the dims behind rot_dim are copied.  inv_freq: double [rot_dim / 2] on the
- * device, radians per position (context scaling is a matter of its values); the angle is reduced in 64 bits, so any
- * position below 2^52 keeps its digits.  cosine and sine are multiplied by factor.  q, k, v: bf16 [n_tokens, heads, 128]
- * with free row strides (ELEMENTS); q_out may be q itself.  k goes rotated and v unchanged to slot slot_mapping[t];
- * slots outside the pool are skipped (q_out is written all the same).  The rotation runs in fp32 and rounds once. */
+ * device, radians per position (context scaling is a matter of its values); the angle is reduced in 64 bits and off by
+ * at most 1.5 * 2^-52 of its turns position * inv_freq / 2 pi, for the fastest pairs less than 32-bit cosines are up to
+ * positions of about 2^29 and less than a step of bf16 up to about 2^40.  cosine and sine are multiplied by factor.
+ * q, k, v: bf16 [n_tokens, heads, 128] with free row strides (ELEMENTS); q_out may be q itself.  k goes rotated and v
+ * unchanged to slot slot_mapping[t]; slots outside the pool are skipped (q_out is written all the same).  The rotation
+ * runs in fp32 and rounds once. */
 INFER_API int infer_rotary_append(const infer_kv_pool_t* pool, void* q_out, int64_t q_out_row_stride, const void* q,
                         const void* k, const void* v, int64_t q_row_stride, int64_t k_row_stride, int64_t v_row_stride,
                         const int64_t* positions, const double* inv_freq, int rot_dim, int interleaved, float factor,
@@ -147,8 +149,9 @@ INFER_API int infer_decode_step_advance(int32_t* context_lens, int32_t* slot_map
  * flash_attn_decode stub (src/operators/flashattn/flashattn_decode.cu:1-13).
  * q, out: bf16 [batch, n_q_heads, 128] contiguous.  Any n_q_heads that is a multiple of the
  * pool's kv heads with at most 8 query heads per kv head (group sizes 1..8, e.g. 40 over 8).
- * Queries may have any finite size, over e4m3 pools too, whose products run on f16: rows that f16 would not hold are
- * scaled by a power of two and back.
+ * Queries may have any size that leaves the scores finite, over e4m3 pools too, whose products run on f16: rows that
+ * f16 would not hold are scaled by a power of two and back.
+ * A row of block_tables has an entry for every page of its context_lens[b] tokens; what lies behind a row is not checked.
  * q and out may also be pinned host memory given by its device-valid address (with unified addressing the
  * pointer itself): the kernel then reads the queries and writes the output rows over PCIe, which saves a
  * host-fed caller two copies.  The same holds for q, k, v and out of infer_paged_decode_append.
@@ -215,8 +218,12 @@ INFER_API int infer_paged_prefill(const infer_kv_pool_t* pool, void* out, const 
  * as rows of zeros.  A row of block_tables has bt_stride columns here; ..._columns takes their number on its own, for a
  * table whose rows lie in wider ones: entries behind a row's columns are not read.  Values that no query of a sequence
  * sees may be anything; a NaN or an infinity that only some of a chunk's queries see may reach the others (0 times it
- * is NaN).  Up to 128 query heads per kv head.  max_seqlen_q has to cover the longest chunk; max_seqlen_k (the longest
- * context) only guides over how many thread blocks few rows' keys are split.
+ * is NaN).  Up to 128 query heads per kv head.  max_seqlen_q has to cover the longest chunk
+ * (total_q, padding rows included, is at most batch * max_seqlen_q); max_seqlen_k (the longest context) only guides over
+ * how many thread blocks few rows' keys are split.  e4m3 pools: queries below 2^126 (a row with a larger value gives
+ * NaN); probabilities are f16 in units of the largest V scale met, so beside its roundings an output is off by up to
+ * 2^-31 per key of 448 times that scale, and the values of pages whose scale lies 2^20 and more below it keep few bits,
+ * also where the page with the large scale gets no weight.
  * softmax_scale: a positive finite number. */
 INFER_API int infer_paged_prefill_window(const infer_kv_pool_t* pool, void* out, const void* q, int64_t total_q,
                         const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, const int32_t* block_tables,

@@ -41,7 +41,7 @@ struct RotaryArgs {
 
 // Heads of one work item: four per load instruction, six or four instructions.  Swept, us at 6 / 5 / 4 / 3: half layout,
 // 32768 tokens of 48 heads 128 / 139 / 137 / 132; interleaved, 5001 tokens of 80 heads 40.2 / 38.9 / 35.9 / 38.2 (four loads
-// leave room for three blocks per SM; swept with 16-byte accesses, the 32-byte ones take 34.4).
+// leave room for three blocks per SM; swept with 16-byte accesses, in a graph; the 32-byte ones take 35.3-35.6 there).
 template <bool INTERLEAVED>
 constexpr int kRotQuads = INTERLEAVED ? 4 : 6;
 
