@@ -220,10 +220,9 @@ INFER_API int infer_paged_prefill(const infer_kv_pool_t* pool, void* out, const 
  * sees may be anything; a NaN or an infinity that only some of a chunk's queries see may reach the others (0 times it
  * is NaN).  Up to 128 query heads per kv head.  max_seqlen_q has to cover the longest chunk
  * (total_q, padding rows included, is at most batch * max_seqlen_q); max_seqlen_k (the longest context) only guides over
- * how many thread blocks few rows' keys are split.  e4m3 pools: queries below 2^126 (a row with a larger value gives
- * NaN); probabilities are f16 in units of the largest V scale met, so beside its roundings an output is off by up to
- * 2^-31 per key of 448 times that scale, and the values of pages whose scale lies 2^20 and more below it keep few bits,
- * also where the page with the large scale gets no weight.
+ * how many thread blocks few rows' keys are split.  e4m3 pools: probabilities are f16 in units of the largest V scale
+ * met, so beside its roundings an output is off by up to 2^-31 per key of 448 times that scale, and the values of pages
+ * whose scale lies 2^20 and more below it keep few bits, also where the page with the large scale gets no weight.
  * softmax_scale: a positive finite number. */
 INFER_API int infer_paged_prefill_window(const infer_kv_pool_t* pool, void* out, const void* q, int64_t total_q,
                         const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, const int32_t* block_tables,

@@ -188,10 +188,11 @@ __device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
 }
 
 // Row t of a Q tile, 128 bf16 in two halves of 64 dims, becomes two rows of 128 e4m3 values in the same place whose sum it is
-// up to a power of two, which is returned (NaN for a row with a value that is not finite, or of 2^126 and more, which leaves
-// no room for the power).  Chunk x (of 16) holds eight bf16; result c (of 8) is the first parts of chunks 2c and 2c + 1,
-// stored over chunk c, and their second parts, stored over chunk 8 + c.  The eight rows of a phase have a chunk at eight
-// different banks.
+// up to a power of two, which is returned (NaN for a row with a value that is not finite): the largest value goes into
+// [2^7, 2^8), that of a row below 2^-119 less far up, by 2^126.  (The power in two factors would lift those as well: 74.6 -> 79.1
+// us for a call of few key tiles a row block, since nothing runs beside the split.)  Chunk x (of 16) holds eight bf16; result c
+// (of 8) is the first parts of chunks 2c and 2c + 1, stored over chunk c, and their second parts, stored over chunk 8 + c.  The
+// eight rows of a phase have a chunk at eight different banks.
 // The split is arithmetic on bf16 bits: y = q * 2^-e * 2^-120 has the exponents of e4m3 (subnormal ones too), so the first part
 // is y cut to three bits of mantissa, the second the difference, and the byte of either its sign and bits 10 .. 4.
 __device__ __forceinline__ float split_q_row(uint32_t tile, int t) {
@@ -211,7 +212,7 @@ __device__ __forceinline__ float split_q_row(uint32_t tile, int t) {
     }
     const __nv_bfloat162 all = __hmax2_nan(__hmax2_nan(top2[0], top2[1]), __hmax2_nan(top2[2], top2[3]));
     const uint32_t top = __bfloat16_as_ushort(__hmax_nan(__low2bfloat16(all), __high2bfloat16(all))) & 0x7fffu;
-    const int e = min(max(int(top >> 7) - 127 - 7, -118), 118);
+    const int e = top == 0 ? 0 : max(int(top >> 7) - 127 - 7, -126);
     const uint32_t down = uint32_t(127 - e) << 7 | uint32_t(127 - e) << 23, tiny = 0x03800380u;      // 2^-e and 2^-120, twice
     auto bytes = [](uint32_t y0, uint32_t y1) {            // e4m3 of four bf16 scaled by 2^-120
         const uint32_t b0 = (y0 & 0x80008000u) | ((y0 << 4) & 0x7fff7fffu);
@@ -242,7 +243,7 @@ __device__ __forceinline__ float split_q_row(uint32_t tile, int t) {
         st_shared_v4(chunk(c), h);
         st_shared_v4(chunk(8 + c), l);
     }
-    return __uint_as_float(top < (127u + 126u) << 7 ? uint32_t(127 + e) << 23 : 0x7fffffffu);
+    return __uint_as_float(top < 255u << 7 ? uint32_t(127 + e) << 23 : 0x7fffffffu);
 }
 
 template <bool FP8>

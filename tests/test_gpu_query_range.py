@@ -73,3 +73,29 @@ def test_rows_that_are_not_finite_stay_their_own(window, sinks):
     assert torch.isnan(got[0, 3]).all() and torch.isnan(got[3, 9]).all()
     got[0, 3], got[3, 9] = want[0, 3], want[3, 9]
     assert bits_equal(got[live], want[live])
+
+
+@pytest.mark.parametrize("rows", [3, 200])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (100, 4)])
+@pytest.mark.parametrize("amplitude", [2.0 ** -124, 2.0 ** -118, 2.0 ** -112, 1e-30, 1.0, 2.0 ** 118, 2.0 ** 125])
+def test_prefill_amplitudes(amplitude, window, sinks, rows):
+    """The split of a query into two e4m3 values over all of bf16's range: exact for values down to 2^-10 of the row's largest,
+    off by 2^-16 of the largest below; rows under 2^-119 are lifted less, by 2^126, and off by 2^-9 (a cut, no rounding) in those units."""
+    gen = torch.Generator().manual_seed(rows)
+    (k, ks), (v, vs) = (plain64.e4m3_pool(3, 256, 2, gen, 0.5) for _ in range(2))
+    k, v, ks, vs = k.cuda(), v.cuda(), ks.cuda(), vs.cuda()
+    q = (torch.randn(rows, 8, 128, generator=gen).clamp(-4, 4) * amplitude).bfloat16().cuda()
+    q[1, 3] = 0.0
+    assert torch.isfinite(q).all()
+    n, scale = 700, SCALE / amplitude
+    cu_q, cu_k = (torch.tensor([0, x], dtype=torch.int32).cuda() for x in (rows, n))
+    got = ops.paged_attn_prefill(q, k, v, cu_q, cu_k, rows, n, scale, torch.tensor([[2, 0, 1]], dtype=torch.int32).cuda(), k_scale=ks,
+                                 v_scale=vs, window=window, sinks=sinks)
+    kk, vv = plain64.values(k, ks, [2, 0, 1], n), plain64.values(v, vs, [2, 0, 1], n)
+    seen = plain64.visible(n, torch.arange(n - rows, n, device="cuda"), window, sinks)
+    want, bound = plain64.attention(q, kk, vv, seen, scale, plain64.E_F16)
+    # that in every product of a score, twice over (its own and the sum's), and the f16 probabilities' absolute step
+    off = torch.maximum(q.double().abs().amax(-1) * 2.0 ** -16, torch.tensor(2.0 ** -135, dtype=torch.float64, device="cuda"))
+    top = off * kk.abs().sum(-1).amax(0).repeat_interleave(4)[None] * scale
+    bound = bound + (2 * top[..., None] * (1 + 2.0 ** -8) + 2.0 ** -31 * n) * vv.abs().amax()
+    plain64.check(got, want, bound)
