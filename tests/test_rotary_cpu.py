@@ -112,3 +112,14 @@ def test_yarn_of_a_context_of_less_than_a_turn(context):
     """No pair makes a turn: all are divided."""
     f, g = rotary_frequencies(64)[0], rotary_frequencies(64, scaling="yarn", factor=8.0, original_max_position=context)[0]
     assert torch.allclose(g, f / 8, rtol=1e-14, atol=0)
+
+
+def test_prefill_window_entry_points_check_arguments_first():
+    lib = _lib.load()
+    buf = C.create_string_buffer(64)
+    p = C.cast(buf, C.c_void_p)
+    for window, sinks, scale, want in ((-1, 0, 0.1, _lib.ERR_GEOMETRY), (5, -1, 0.1, _lib.ERR_GEOMETRY), (5, 0, 0.0, _lib.ERR_GEOMETRY),
+                                       (5, 0, float("nan"), _lib.ERR_GEOMETRY), (5, 0, float("inf"), _lib.ERR_GEOMETRY),
+                                       (5, 4, 0.1, _lib.ERR_NULL), (0, 0, 0.1, _lib.ERR_NULL)):
+        assert lib.infer_paged_prefill_window(None, p, p, 1, p, p, p, 4, 1, 1, 1, 8, scale, window, sinks, None) == want
+        assert lib.infer_paged_prefill_window_columns(None, p, p, 1, p, p, p, 4, 3, 1, 1, 1, 8, scale, window, sinks, None) == want
